@@ -1,0 +1,355 @@
+"""The operators on factor rows in device memory, as cases that can be timed and compared.
+
+  lookup     rows of a factor table by id, scaled (mascot.rows_lookup); also from a table held in 8 bits
+  gradient   its gradient: the rows of one table, each the sum over the places that looked it up, in their order
+             (mascot.rows_gradient)
+  pair       one training pass of the preference loss on pairs (user, preferred item, other item): losses, margins and
+             the gradients of both factor tables (mascot.pair_loss, mascot.pair_gradient)
+  quantize   rows to e4m3 with one power-of-two scale for each block of 128 (mascot.rows_quantize)
+  product    the scores of every row of one table against every row of another, both held that way
+             (mascot.rows_product)
+
+With `own` false, run() computes them from elementary torch operations; with `own` true it makes the library's calls.
+Formulas: R a table, s a scalar, x a row.
+  lookup     out[j] = s * R[id_j]; a row of zeros for an id of -1
+  gradient   dR[r] = s * sum of g[j] over j with id_j = r
+  pair       m = <P[u], Q[i] - Q[j]>,  z = beta * (m - reference),
+             loss = w * ((1 - eps) * log(1 + exp(-z)) + eps * log(1 + exp(z))),  c = dloss/dm = w * beta * (sigmoid(z) - (1 - eps)),
+             dP[u] += s * c * (Q[i] - Q[j]),  dQ[i] += s * c * P[u],  dQ[j] -= s * c * P[u]; a pair with an id of -1 adds nothing
+  quantize   scale = the smallest power of two with max|x| / scale <= 448 over the block (1 for a block of zeros), q = e4m3(x / scale)
+  product    out[a, b] = sum over blocks of 128 columns of scale_a * scale_b * sum of q_a * q_b
+"""
+import importlib
+import math
+
+import torch
+
+own = False
+BLOCK = 128
+TYPES = {"f32": torch.float32, "f16": torch.float16, "bf16": torch.bfloat16, "e4m3": torch.float8_e4m3fn}
+
+
+# ---- cases -------------------------------------------------------------------------------------------------------
+def _lookup(name, rows, width, n, table, out, ids, law, pad):
+    return dict(name=name, kind="lookup", rows=rows, width=width, n=n, table=table, out=out, ids=ids, law=law, pad=pad)
+
+
+def _gradient(name, rows, width, n, grad, out, ids, law, pad):
+    return dict(name=name, kind="gradient", rows=rows, width=width, n=n, grad=grad, out=out, ids=ids, law=law, pad=pad)
+
+
+def _pair(name, users, items, width, n, table, out, ids, law, pad, reference, smoothing, weighted):
+    return dict(name=name, kind="pair", users=users, items=items, width=width, n=n, table=table, out=out, ids=ids, law=law, pad=pad,
+                reference=reference, smoothing=smoothing, weighted=weighted)
+
+
+def _quantize(name, rows, width, source, block_rows):
+    return dict(name=name, kind="quantize", rows=rows, width=width, source=source, block_rows=block_rows)
+
+
+def _product(name, m, n, width, out, block_rows):
+    return dict(name=name, kind="product", m=m, n=n, width=width, out=out, block_rows=block_rows)
+
+
+def listed():
+    return [
+        # A serving request: the factors of some users, k = 64, from a table held in 8 bits.
+        _lookup("lookup_e4m3_k64", 10_000, 64, 1_000, "e4m3", "f32", "i32", 0.9, 0.0),
+        # A large batch against the largest table of the configurations, binary16 rows into fp32.
+        _lookup("lookup_k128_2m", 1_000_990, 128, 2_000_003, "f16", "f32", "i32", 1.0, 0.01),
+        # The gradient of a small batch: few rows are touched, and what counts is how many launches it takes.
+        _gradient("gradient_k64_4k", 10_000, 64, 4_096, "f32", "f32", "i64", 1.0, 0.0),
+        # A large batch with gradients in bf16, some places empty: long sums for the popular rows, few terms for most.
+        _gradient("gradient_k128_4m", 480_189, 128, 4_000_037, "bf16", "f32", "i32", 1.0, 0.01),
+        # A step of the smallest configuration.
+        _pair("pair_k64_4k", 10_000, 5_000, 64, 4_096, "f32", "f32", "i32", 1.0, 0.0, False, 0.0, False),
+        # A step of the 8M-rating configuration against a reference model, with smoothed labels and weights.
+        _pair("pair_k128_100k", 71_567, 10_681, 128, 100_003, "f32", "f32", "i64", 0.9, 0.01, True, 0.1, True),
+        # A large step on binary16 tables of the 100M-rating configuration.
+        _pair("pair_k128_1m", 480_189, 17_770, 128, 1_000_003, "f16", "f32", "i32", 1.1, 0.0, True, 0.0, False),
+        # The item table of the largest configuration, once after training.
+        _quantize("quantize_items_k128", 624_961, 128, "f32", 1),
+        # A wide table in bf16 with odd sizes, one scale for each square block.
+        _quantize("quantize_square", 16_411, 1_000, "bf16", 128),
+        # Scores of all items for one user: a single row against a table.
+        _product("product_one_user", 1, 624_961, 128, "f32", 1),
+        # Scores of all items for a batch of users, k = 128: what is written counts.
+        _product("product_users_k128", 4_096, 17_770, 128, "f16", 1),
+        # The same with a long sum: rows of 4096 columns and square blocks.
+        _product("product_wide", 4_096, 17_770, 4_096, "bf16", 128),
+    ]
+
+
+def draw(rng):
+    def logu(lo, hi):
+        return int(round(math.exp(rng.uniform(math.log(lo), math.log(hi)))))
+
+    kind = rng.choices(["lookup", "gradient", "pair", "quantize", "product"], [15, 25, 25, 10, 25])[0]
+    width = rng.choice([64, 64, 128, 128, 128, rng.randint(1, 512), logu(8, 512)])
+    ids, law, pad = rng.choice(["i32", "i64"]), rng.uniform(0.0, 1.3), rng.choice([0.0, 0.0, 0.02, 0.2])
+    half = ["f32", "f32", "f16", "bf16"]
+    if kind == "lookup":
+        return _lookup("", logu(1, 1_000_000), width, logu(1, 250_000_000 // max(width, 125)), rng.choice(half + ["e4m3"]), rng.choice(half), ids, law, pad)
+    if kind == "gradient":
+        return _gradient("", logu(1, 60_000_000 // max(width, 120)), width, logu(1, 500_000_000 // max(width, 128)), rng.choice(half), rng.choice(half), ids, law, pad)
+    if kind == "pair":
+        most = 60_000_000 // max(width, 120)
+        return _pair("", logu(1, most), logu(2, max(2, most // 20)), width, logu(1, 125_000_000 // max(width, 125)), rng.choice(half), rng.choice(["f32", "f32", "bf16"]), ids, law, pad,
+                     rng.random() < 0.5, rng.choice([0.0, 0.0, rng.uniform(0.0, 0.4)]), rng.random() < 0.3)
+    if kind == "quantize":
+        width = rng.choice([width, width, logu(64, 8192)])
+        return _quantize("", logu(1, 80_000_000 // max(width, 100)), width, rng.choice(half), rng.choice([1, 1, 128]))
+    width = rng.choice([width, width, logu(100, 8192)])
+    m = rng.choice([1, logu(1, 4096), logu(1, 4096), logu(64, 4096)])
+    n = logu(1, max(2, min(600_000, 70_000_000 // m, 160_000_000 // width, 290_000_000_000 // (m * max(width, 128)))))
+    return _product("", m, n, width, rng.choice(half), rng.choice([1, 1, 128]))
+
+
+# ---- inputs ------------------------------------------------------------------------------------------------------
+def _ids(n, rows, law, pad, dtype, gen):
+    """Ids of a popularity law (weights rank^-law, ranks dealt at random), a share of them -1."""
+    w = torch.arange(1, rows + 1, dtype=torch.float64, device="cuda").pow_(-law)
+    w = torch.cumsum(w[torch.randperm(rows, generator=gen, device="cuda")], 0)
+    u = torch.rand(n, generator=gen, device="cuda", dtype=torch.float64) * w[-1]
+    got = torch.searchsorted(w, u).clamp_(max=rows - 1)
+    if pad:
+        got[torch.rand(n, generator=gen, device="cuda") < pad] = -1
+    return got.to(torch.int32 if dtype == "i32" else torch.int64)
+
+
+def _normal(shape, std, dtype, gen):
+    """Values of a trained table: normal, rows of different size."""
+    size = torch.exp(0.5 * torch.randn(shape[0], 1, generator=gen, device="cuda"))
+    return (torch.randn(shape, generator=gen, device="cuda") * size * std).to(TYPES[dtype])
+
+
+def prepare(case, seed):
+    gen = torch.Generator(device="cuda")
+    gen.manual_seed(seed)
+    st, kind = dict(case), case["kind"]
+    width = case["width"]
+    if kind == "lookup":
+        st["scale"] = math.sqrt(width)
+        if case["table"] == "e4m3":
+            st["table"], st["table_scale"] = _plain_quantize(_normal((case["rows"], width), width ** -0.25, "f32", gen), 1)
+        else:
+            st["table"], st["table_scale"] = _normal((case["rows"], width), width ** -0.25, case["table"], gen), None
+        st["ids"] = _ids(case["n"], case["rows"], case["law"], case["pad"], case["ids"], gen)
+    elif kind == "gradient":
+        st["scale"] = math.sqrt(width)
+        st["ids"] = _ids(case["n"], case["rows"], case["law"], case["pad"], case["ids"], gen)
+        st["grad"] = _normal((case["n"], width), 1e-2, case["grad"], gen)
+    elif kind == "pair":
+        n = case["n"]
+        st["P"] = _normal((case["users"], width), width ** -0.25, case["table"], gen)
+        st["Q"] = _normal((case["items"], width), width ** -0.25, case["table"], gen)
+        st["u"] = _ids(n, case["users"], 0.5 * case["law"], case["pad"], case["ids"], gen)
+        st["i"] = _ids(n, case["items"], case["law"], 0.0, case["ids"], gen)
+        st["j"] = _ids(n, case["items"], 0.0, case["pad"], case["ids"], gen)
+        st["beta"], st["scale"] = 0.5, 1.0 / n
+        st["ref"] = torch.randn(n, generator=gen, device="cuda") if case["reference"] else None
+        st["w"] = torch.rand(n, generator=gen, device="cuda") + 0.5 if case["weighted"] else None
+    elif kind == "quantize":
+        st["x"] = _normal((case["rows"], width), 0.1, case["source"], gen)
+    else:
+        st["a"], st["a_scale"] = _plain_quantize(_normal((case["m"], width), width ** -0.25, "f32", gen), 1)
+        st["b"], st["b_scale"] = _plain_quantize(_normal((case["n"], width), width ** -0.25, "f32", gen), case["block_rows"])
+    return st
+
+
+# ---- plain forms -------------------------------------------------------------------------------------------------
+def _blocks(x, block_rows):
+    """[row blocks, block rows, column blocks, 128], filled up with zeros."""
+    rows, width = x.shape
+    up = x.new_zeros((-(-rows // block_rows) * block_rows, -(-width // BLOCK) * BLOCK))
+    up[:rows, :width] = x
+    return up.view(up.shape[0] // block_rows, block_rows, up.shape[1] // BLOCK, BLOCK)
+
+
+def _plain_quantize(x, block_rows):
+    """(e4m3 [rows, width] in rows of a multiple of 128 bytes, scales [column blocks, row blocks])"""
+    rows, width = x.shape
+    b = _blocks(x.float(), block_rows)
+    m, e = torch.frexp(b.abs().amax(dim=(1, 3)))                     # amax = m * 2^e, m in [0.5, 1); 448 = 0.875 * 2^9
+    e = torch.where(m == 0, torch.zeros_like(e), torch.where(m <= 0.875, e - 9, e - 8).clamp(min=-126))
+    scale = torch.ldexp(torch.ones_like(m), e)
+    q = (b / scale[:, None, :, None]).to(torch.float8_e4m3fn).view(-1, b.shape[2] * BLOCK)
+    return q[:rows, :width], scale.t().contiguous()
+
+
+def _plain_values(q, scale):
+    """The fp32 values of an e4m3 matrix with its scales."""
+    rows, width = q.shape
+    block_rows = 1 if scale.shape[1] == rows else BLOCK
+    each = scale.t().repeat_interleave(block_rows, 0)[:rows].repeat_interleave(BLOCK, 1)[:, :width]
+    return q.float() * each
+
+
+def _plain_lookup(st):
+    ids = st["ids"].long()
+    at = ids.clamp(min=0)
+    if st["table_scale"] is None:
+        rows = st["table"][at].float()
+    else:
+        rows = st["table"].view(torch.uint8)[at].view(torch.float8_e4m3fn).float()
+        rows = rows * st["table_scale"][:, at].t().repeat_interleave(BLOCK, 1)[:, :st["width"]]
+    return torch.where(ids[:, None] >= 0, rows * st["scale"], 0.0).to(TYPES[st["out"]])
+
+
+def _plain_gradient(st):
+    # popular rows are sums of 100,000 terms and more: 64 bits
+    ids = st["ids"].long()
+    sums = torch.zeros(st["rows"] + 1, st["width"], dtype=torch.float64, device="cuda")
+    sums.index_add_(0, torch.where(ids >= 0, ids, st["rows"]), st["grad"].double())
+    return (sums[:-1] * st["scale"]).to(TYPES[st["out"]])
+
+
+def _plain_pair(st):
+    u, i, j = st["u"].long(), st["i"].long(), st["j"].long()
+    there = (u >= 0) & (i >= 0) & (j >= 0)
+    u, i, j = u.clamp(min=0), i.clamp(min=0), j.clamp(min=0)
+    p, d = st["P"][u].float(), st["Q"][i].float() - st["Q"][j].float()
+    margin = torch.where(there, (p * d).sum(1), 0.0)
+    z = st["beta"] * (margin - st["ref"] if st["ref"] is not None else margin)
+    w = there.float() if st["w"] is None else torch.where(there, st["w"], 0.0)
+    eps, far = st["smoothing"], torch.log1p(torch.exp(-z.abs()))
+    loss = w * ((1 - eps) * (far + (-z).clamp(min=0)) + eps * (far + z.clamp(min=0)))
+    c = w * st["beta"] * (torch.where(z >= 0, 1 / (1 + torch.exp(-z.abs())), torch.exp(-z.abs()) / (1 + torch.exp(-z.abs()))) - (1 - eps))
+    # popular rows are sums of 100,000 terms and more: 64 bits
+    dP = torch.zeros(st["users"], st["width"], dtype=torch.float64, device="cuda")
+    dQ = torch.zeros(st["items"], st["width"], dtype=torch.float64, device="cuda")
+    dP.index_add_(0, u, (c[:, None] * d).double())
+    g = (c[:, None] * p).double()
+    dQ.index_add_(0, i, g)
+    dQ.index_add_(0, j, -g)
+    return {"loss": loss, "margin": margin, "dP": (dP * st["scale"]).to(TYPES[st["out"]]), "dQ": (dQ * st["scale"]).to(TYPES[st["out"]])}
+
+
+def _plain_product(st):
+    return (_plain_values(st["a"], st["a_scale"]) @ _plain_values(st["b"], st["b_scale"]).t()).to(TYPES[st["out"]])
+
+
+# ---- one pass ----------------------------------------------------------------------------------------------------
+_library = None
+
+
+def _mascot():
+    global _library
+    if _library is None:
+        _library = importlib.import_module("icdm-2021_mascot_b200.mascot")
+    return _library
+
+
+def run(st):
+    kind = st["kind"]
+    if own:
+        M = _mascot()
+        if kind == "lookup":
+            return M.rows_lookup(st["table"], st["ids"], scale=st["scale"], table_scale=st["table_scale"], out_dtype=TYPES[st["out"]])
+        if kind == "gradient":
+            return M.rows_gradient(st["grad"], st["ids"], st["rows"], scale=st["scale"], out_dtype=TYPES[st["out"]])
+        if kind == "pair":
+            loss, margin, c = M.pair_loss(st["P"], st["Q"], st["u"], st["i"], st["j"], beta=st["beta"], smoothing=st["smoothing"], reference=st["ref"], weight=st["w"])
+            dP, dQ = M.pair_gradient(st["P"], st["Q"], st["u"], st["i"], st["j"], c, scale=st["scale"], out_dtype=TYPES[st["out"]])
+            return {"loss": loss, "margin": margin, "dP": dP, "dQ": dQ}
+        if kind == "quantize":
+            q, scale = M.rows_quantize(st["x"], block_rows=st["block_rows"])
+            return {"q": q, "scale": scale}
+        return M.rows_product(st["a"], st["a_scale"], st["b"], st["b_scale"], out_dtype=TYPES[st["out"]])
+    if kind == "lookup":
+        return _plain_lookup(st)
+    if kind == "gradient":
+        return _plain_gradient(st)
+    if kind == "pair":
+        return _plain_pair(st)
+    if kind == "quantize":
+        q, scale = _plain_quantize(st["x"], st["block_rows"])
+        return {"q": q, "scale": scale}
+    return _plain_product(st)
+
+
+# ---- what a pass cannot do without -------------------------------------------------------------------------------
+def work(case):
+    size = {"f32": 4, "f16": 2, "bf16": 2, "e4m3": 1, "i32": 4, "i64": 8}
+    kind, w = case["kind"], case["width"]
+    if kind == "lookup":
+        per_row = w * size[case["table"]] + (4 * -(-w // BLOCK) if case["table"] == "e4m3" else 0)
+        return {"bytes": min(case["n"], case["rows"]) * per_row + case["n"] * (size[case["ids"]] + w * size[case["out"]]), "flops": case["n"] * w}
+    if kind == "gradient":
+        return {"bytes": case["n"] * (size[case["ids"]] + w * size[case["grad"]]) + case["rows"] * w * size[case["out"]], "flops": case["n"] * w}
+    if kind == "pair":
+        n = case["n"]
+        rows_in = min(n, case["users"]) + min(2 * n, case["items"])
+        per_pair = 3 * size[case["ids"]] + 8 + (4 if case["reference"] else 0) + (4 if case["weighted"] else 0)
+        return {"bytes": rows_in * w * size[case["table"]] + (case["users"] + case["items"]) * w * size[case["out"]] + n * per_pair, "flops": n * w * 9}
+    if kind == "quantize":
+        return {"bytes": case["rows"] * w * (size[case["source"]] + 1) + 4 * -(-case["rows"] // case["block_rows"]) * -(-w // BLOCK), "flops": 3 * case["rows"] * w}
+    m, n, blocks = case["m"], case["n"], -(-w // BLOCK)
+    return {"bytes": (m + n) * w + 4 * blocks * (m + -(-n // case["block_rows"])) + m * n * size[case["out"]], "flops": 2 * m * n * w}
+
+
+# ---- the same in 64 bits, from the definitions -------------------------------------------------------------------
+def _sorted_sums(ids, rows, terms):
+    """sums[r] = sum of terms[e] over e with ids[e] = r, as a product with the 0/1 matrix of the ids."""
+    keep = ids >= 0
+    ids, terms = ids[keep], terms[keep]
+    order = torch.argsort(ids, stable=True)
+    begin = torch.searchsorted(ids[order], torch.arange(rows + 1, device="cuda"))
+    ones = torch.sparse_csr_tensor(begin, order, torch.ones(order.numel(), dtype=torch.float64, device="cuda"), size=(rows, max(1, order.numel())))
+    return ones @ (terms if order.numel() else terms.new_zeros(1, terms.shape[1]))
+
+
+def _e4m3(y):
+    """The nearest numbers of four significant bits down to 2^-6, multiples of 2^-9 below, ties to even."""
+    e = torch.clamp(torch.floor(torch.log2(y.abs().clamp(min=2.0 ** -20))), min=-6.0)
+    step = torch.exp2(e - 3)
+    return torch.round(y / step) * step
+
+
+def _spread(scale, rows, width, block_rows):
+    """Each element's scale."""
+    r = torch.arange(rows, device="cuda") // block_rows
+    c = torch.arange(width, device="cuda") // BLOCK
+    return scale.double()[c[None, :], r[:, None]]
+
+
+def exact(case, seed):
+    st = prepare(case, seed)
+    kind, w = case["kind"], case["width"]
+    if kind == "lookup":
+        table = st["table"].double()
+        if st["table_scale"] is not None:
+            table = table * _spread(st["table_scale"], case["rows"], w, 1)
+        table = torch.cat([table * st["scale"], table.new_zeros(1, w)])        # id -1: the last row
+        return table[st["ids"].long()]
+    if kind == "gradient":
+        return _sorted_sums(st["ids"].long(), case["rows"], st["grad"].double()) * st["scale"]
+    if kind == "pair":
+        u, i, j = st["u"].long(), st["i"].long(), st["j"].long()
+        gone = torch.minimum(torch.minimum(u, i), j) < 0
+        P, Q = st["P"].double(), st["Q"].double()
+        p, d = P[u], Q[i].sub_(Q[j])
+        margin = torch.einsum("nk,nk->n", p, d).masked_fill(gone, 0.0)
+        z = st["beta"] * (margin - (st["ref"].double() if st["ref"] is not None else 0.0))
+        w_ = (st["w"].double() if st["w"] is not None else torch.ones_like(z)).masked_fill(gone, 0.0)
+        eps = st["smoothing"]
+        loss = -w_ * ((1 - eps) * torch.nn.functional.logsigmoid(z) + eps * torch.nn.functional.logsigmoid(-z))
+        c = w_ * st["beta"] * (torch.sigmoid(z) - (1 - eps)) * st["scale"]
+        dP = _sorted_sums(u.masked_fill(gone, -1), case["users"], d.mul_(c[:, None]))
+        del d
+        p.mul_(c[:, None])
+        dQ = _sorted_sums(i.masked_fill(gone, -1), case["items"], p) - _sorted_sums(j.masked_fill(gone, -1), case["items"], p)
+        return {"loss": loss, "margin": margin, "dP": dP, "dQ": dQ}
+    if kind == "quantize":
+        x = st["x"].double()
+        rows, by = case["rows"], case["block_rows"]
+        r = torch.arange(rows, device="cuda") // by
+        c = torch.arange(w, device="cuda") // BLOCK
+        rb, cb = -(-rows // by), -(-w // BLOCK)
+        top = torch.zeros(cb * rb, dtype=torch.float64, device="cuda")
+        top.scatter_reduce_(0, (c[None, :] * rb + r[:, None]).reshape(-1), x.abs().reshape(-1), "amax")
+        scale = torch.where(top > 0, torch.exp2(torch.ceil(torch.log2(top / 448.0)).clamp(min=-126.0)), 1.0).view(cb, rb)
+        return {"q": _e4m3(x / _spread(scale, rows, w, by)), "scale": scale}
+    a = st["a"].double() * _spread(st["a_scale"], case["m"], w, 1)
+    b = st["b"].double() * _spread(st["b_scale"], case["n"], w, case["block_rows"])
+    return a @ b.t()
