@@ -301,8 +301,8 @@ def _sorted_sums(ids, rows, terms):
 
 def _e4m3(y):
     """The nearest numbers of four significant bits down to 2^-6, multiples of 2^-9 below, ties to even."""
-    e = torch.clamp(torch.floor(torch.log2(y.abs().clamp(min=2.0 ** -20))), min=-6.0)
-    step = torch.exp2(e - 3)
+    _, e = torch.frexp(y)                                                 # 2^(e - 1) <= |y| < 2^e
+    step = torch.ldexp(torch.ones_like(y), (e - 1).clamp(min=-6) - 3)
     return torch.round(y / step) * step
 
 
@@ -348,7 +348,8 @@ def exact(case, seed):
         rb, cb = -(-rows // by), -(-w // BLOCK)
         top = torch.zeros(cb * rb, dtype=torch.float64, device="cuda")
         top.scatter_reduce_(0, (c[None, :] * rb + r[:, None]).reshape(-1), x.abs().reshape(-1), "amax")
-        scale = torch.where(top > 0, torch.exp2(torch.ceil(torch.log2(top / 448.0)).clamp(min=-126.0)), 1.0).view(cb, rb)
+        m, e = torch.frexp(top / 448.0)                                   # a power of two has m = 0.5
+        scale = torch.where(top > 0, torch.ldexp(torch.ones_like(top), torch.where(m == 0.5, e - 1, e).clamp(min=-126)), 1.0).view(cb, rb)
         return {"q": _e4m3(x / _spread(scale, rows, w, by)), "scale": scale}
     a = st["a"].double() * _spread(st["a_scale"], case["m"], w, 1)
     b = st["b"].double() * _spread(st["b_scale"], case["n"], w, case["block_rows"])
