@@ -19,7 +19,7 @@ BIN = os.path.join(HERE, "bin")
 NVCC_FLAGS = ["-O3", "-std=c++17", "-gencode", "arch=compute_100a,code=sm_100a", "-lineinfo", "--no-compress",
               "-Xcompiler", "-fPIC", "-Xcompiler", "-fvisibility=hidden"]
 
-LIB_SOURCES = ["mascot_api.cu", "setup.cu", "shard.cu", "train_kernels.cu", "eval_kernels.cu", "prep_kernels.cu", "host_copy.cu", "device_pool.cu", "probe.cu"]
+LIB_SOURCES = ["mascot_api.cu", "setup.cu", "shard.cu", "train_kernels.cu", "eval_kernels.cu", "prep_kernels.cu", "host_copy.cu", "device_pool.cu", "probe.cu", "row_ops.cu", "row_gradient.cu", "row_product.cu"]
 CLI_SOURCES = {"quantized_mf": "quantized_mf.cpp", "test_mf": "test_mf.cpp", "convert_ratings": "convert_ratings.cpp"}
 
 

@@ -28,6 +28,8 @@ EXPORTS = [
     "mascot_stats_apply", "mascot_item_rows", "mascot_sync", "mascot_get_stream", "mascot_eval_sq_error", "mascot_train_epoch_streamed",
     "mascot_release_scratch", "mascot_release_cached", "mascot_comm_unique_id", "mascot_shard_init", "mascot_shard_set_ratings", "mascot_shard_train_epoch",
     "mascot_shard_eval_rmse", "mascot_shard_gather_factors", "mascot_shard_info", "mascot_shard_schedule", "mascot_probe_read_bandwidth", "mascot_get_timings", "mascot_get_worker_count",
+    "mascot_rows_lookup", "mascot_rows_gradient", "mascot_rows_gradient_workspace", "mascot_pair_loss", "mascot_pair_gradient",
+    "mascot_pair_gradient_workspace", "mascot_rows_quantize", "mascot_rows_product",
 ]
 
 COMM_ID_BYTES = 128
@@ -53,6 +55,16 @@ class EpochStats(C.Structure):
     ]
 
 
+class Rows(C.Structure):
+    """mascot_rows: a matrix in device memory."""
+    _fields_ = [("data", C.c_void_p), ("rows", C.c_uint64), ("stride", C.c_uint64), ("width", C.c_uint32), ("type", C.c_uint32)]
+
+
+class Ids(C.Structure):
+    """mascot_ids: a vector of ids in device memory."""
+    _fields_ = [("data", C.c_void_p), ("count", C.c_uint64), ("bits", C.c_uint32), ("reserved", C.c_uint32)]
+
+
 class MascotError(RuntimeError):
     def __init__(self, status, message):
         super().__init__(f"libmascot status {status}: {message}")
@@ -73,6 +85,15 @@ def load():
         L.mascot_last_error.argtypes = [C.c_void_p]
         L.mascot_status_string.restype = C.c_char_p
         L.mascot_status_string.argtypes = [C.c_int]
+        rows, ids, ptr = C.POINTER(Rows), C.POINTER(Ids), C.c_void_p
+        L.mascot_rows_lookup.argtypes = [rows, ptr, C.c_uint32, ids, C.c_float, rows, ptr, ptr]
+        L.mascot_rows_gradient.argtypes = [rows, ids, C.c_float, rows, C.c_int, ptr, C.c_uint64, ptr, ptr]
+        L.mascot_rows_gradient_workspace.argtypes = [C.c_uint64, C.c_uint64, C.c_uint32, C.POINTER(C.c_uint64)]
+        L.mascot_pair_loss.argtypes = [rows, rows, ids, ids, ids, C.c_float, C.c_float, ptr, ptr, ptr, ptr, ptr, ptr, ptr]
+        L.mascot_pair_gradient.argtypes = [rows, rows, ids, ids, ids, ptr, C.c_float, rows, rows, C.c_int, ptr, C.c_uint64, ptr, ptr]
+        L.mascot_pair_gradient_workspace.argtypes = [C.c_uint64, C.c_uint64, C.c_uint64, C.c_uint32, C.POINTER(C.c_uint64)]
+        L.mascot_rows_quantize.argtypes = [rows, C.c_uint32, rows, ptr, ptr]
+        L.mascot_rows_product.argtypes = [rows, ptr, rows, ptr, C.c_uint32, rows, ptr, ptr]
         ver, csz, ssz = C.c_uint32(), C.c_uint32(), C.c_uint32()
         L.mascot_abi_info(C.byref(ver), C.byref(csz), C.byref(ssz))
         if (csz.value, ssz.value) != (C.sizeof(Config), C.sizeof(EpochStats)):
@@ -395,3 +416,211 @@ def rmse_host(P, Q, test, k, device=0):
     if rc != OK:
         raise MascotError(rc, L.mascot_last_error(None).decode())
     return v.value
+
+
+# ---- operators on factor rows in device memory: torch tensors in, torch tensors out, on torch's current stream ----
+# Outputs that the caller does not hand over, and scratch, come from torch's allocator, so that the calls can be captured
+# into a torch.cuda.graph.  `flags` is an int32 tensor of one element that gathers FLAG_BAD_ID and FLAG_GAVE_UP.
+
+F32, F16, BF16, E4M3 = 0, 1, 2, 3
+FLAG_BAD_ID, FLAG_GAVE_UP = 1, 2
+_ops = None
+
+
+class _Ops:
+    """torch and what the calls below look up in it, once."""
+    def __init__(self):
+        import torch
+        self.torch = torch
+        self.types = {torch.float32: F32, torch.float16: F16, torch.bfloat16: BF16, torch.float8_e4m3fn: E4M3}
+        self.bits = {torch.int32: 32, torch.int64: 64}
+
+
+def _torch_ops():
+    global _ops
+    if _ops is None:
+        _ops = _Ops()
+    return _ops
+
+
+def _refuse(message):
+    raise MascotError(ERR_BAD_ARG, message)
+
+
+def _rows(what, t, device):
+    """The Rows of a 2-d tensor on `device` whose rows are contiguous."""
+    kind = _torch_ops().types.get(t.dtype)
+    if kind is None:
+        _refuse(f"{what}: must be float32, float16, bfloat16 or float8_e4m3fn, not {t.dtype}")
+    if t.dim() != 2:
+        _refuse(f"{what}: must have two dimensions")
+    if t.device != device:
+        _refuse(f"{what}: is on {t.device}, not on {device}")
+    rows, width = t.shape
+    stride, step = t.stride()
+    if width > 1 and step != 1:
+        _refuse(f"{what}: elements of a row must lie one after the other")
+    if rows > 1 and stride < width:
+        _refuse(f"{what}: rows overlap")
+    return Rows(t.data_ptr(), rows, stride if rows > 1 else max(width, stride), width, kind)
+
+
+def _id_vector(what, t, device):
+    bits = _torch_ops().bits.get(t.dtype)
+    if bits is None:
+        _refuse(f"{what}: must be int32 or int64, not {t.dtype}")
+    if t.dim() != 1 or (t.shape[0] > 1 and t.stride(0) != 1):
+        _refuse(f"{what}: must be a contiguous vector")
+    if t.device != device:
+        _refuse(f"{what}: is on {t.device}, not on {device}")
+    return Ids(t.data_ptr(), t.shape[0], bits, 0)
+
+
+def _plain(what, t, dtype, device, shape):
+    """Address of a contiguous tensor of that type, device and shape; None stays None."""
+    if t is None:
+        return None
+    if t.dtype != dtype or t.device != device or tuple(t.shape) != tuple(shape) or not t.is_contiguous():
+        _refuse(f"{what}: must be a contiguous {dtype} tensor of shape {tuple(shape)} on {device}")
+    return t.data_ptr()
+
+
+def _flag_word(flags, device):
+    return _plain("flags", flags, _torch_ops().torch.int32, device, (1,))
+
+
+def _device_of(what, t):
+    if not t.is_cuda:
+        _refuse(f"{what}: must be on a GPU; libmascot has no CPU path")
+    return t.device
+
+
+def _call(device, name, *args):
+    """A call on `device`, on torch's current stream there."""
+    cuda = _torch_ops().torch.cuda
+    f = getattr(load(), name)
+    if cuda.current_device() == device.index:
+        rc = f(*args, cuda.current_stream(device).cuda_stream)
+    else:
+        with cuda.device(device):
+            rc = f(*args, cuda.current_stream(device).cuda_stream)
+    if rc != OK:
+        raise MascotError(rc, load().mascot_last_error(None).decode())
+
+
+def _result(what, out, shape, dtype, device):
+    if out is None:
+        return _torch_ops().torch.empty(shape, dtype=dtype, device=device)
+    if tuple(out.shape) != tuple(shape):
+        _refuse(f"{what}: must have shape {tuple(shape)}")
+    if dtype is not None and out.dtype != dtype:
+        _refuse(f"{what}: must be {dtype}")
+    return out
+
+
+def _scale_rows(what, scale, rows, width, device):
+    """Rows that share a scale (1 or 128), by the shape of `scale`: [column blocks, row blocks]."""
+    blocks = -(-width // 128)
+    each = 128 if rows > 1 and tuple(scale.shape) == (blocks, -(-rows // 128)) else 1
+    return each, _plain(what, scale, _torch_ops().torch.float32, device, (blocks, -(-rows // each)))
+
+
+def rows_lookup(table, ids, scale=1.0, table_scale=None, out=None, out_dtype=None, flags=None):
+    """out[j] = scale * table[ids[j]], zeros where ids[j] is -1 (mascot_rows_lookup).  A float8_e4m3fn table comes with its
+    scales, `table_scale` of rows_quantize; the result is float32 then unless out_dtype says otherwise."""
+    device = _device_of("table", table)
+    t, i = _rows("table", table, device), _id_vector("ids", ids, device)
+    each, ts = 0, None
+    if table_scale is not None:
+        each, ts = _scale_rows("table_scale", table_scale, t.rows, t.width, device)
+    if out_dtype is None and out is None:
+        out_dtype = _torch_ops().torch.float32 if t.type == E4M3 else table.dtype
+    out = _result("out", out, (i.count, t.width), out_dtype, device)
+    _call(device, "mascot_rows_lookup", t, ts, each, i, scale, _rows("out", out, device), _flag_word(flags, device))
+    return out
+
+
+def _workspace(workspace, name, device, *sizes):
+    need = C.c_uint64()
+    if getattr(load(), name)(*sizes, C.byref(need)) != OK:
+        _refuse(load().mascot_last_error(None).decode())
+    if workspace is None:
+        workspace = _torch_ops().torch.empty(need.value, dtype=_torch_ops().torch.uint8, device=device)
+    elif not workspace.is_contiguous() or workspace.device != device:
+        _refuse(f"workspace: must be a contiguous tensor on {device}")
+    return workspace, workspace.data_ptr(), workspace.numel() * workspace.element_size()
+
+
+def rows_gradient(grad, ids, rows, scale=1.0, out=None, out_dtype=None, accumulate=False, workspace=None, flags=None):
+    """out[r] = scale * sum of grad[j] over the j with ids[j] == r, for r < rows (mascot_rows_gradient); with `accumulate` added
+    to what `out` holds."""
+    device = _device_of("grad", grad)
+    g, i = _rows("grad", grad, device), _id_vector("ids", ids, device)
+    if accumulate and out is None:
+        _refuse("accumulate: needs an out")
+    out = _result("out", out, (rows, g.width), out_dtype if out_dtype is not None or out is not None else grad.dtype, device)
+    keep, ws, size = _workspace(workspace, "mascot_rows_gradient_workspace", device, i.count, rows, g.width)
+    _call(device, "mascot_rows_gradient", g, i, scale, _rows("out", out, device), 1 if accumulate else 0, ws, size, _flag_word(flags, device))
+    return out
+
+
+def pair_loss(P, Q, users, preferred, other, beta=1.0, smoothing=0.0, reference=None, weight=None, flags=None):
+    """(loss, margin, coef) of the preference loss on pairs, fp32 vectors (mascot_pair_loss)."""
+    device = _device_of("P", P)
+    torch = _torch_ops().torch
+    p, q = _rows("P", P, device), _rows("Q", Q, device)
+    u, i, j = _id_vector("users", users, device), _id_vector("preferred", preferred, device), _id_vector("other", other, device)
+    n = u.count
+    ref, w = _plain("reference", reference, torch.float32, device, (n,)), _plain("weight", weight, torch.float32, device, (n,))
+    loss, margin, coef = (torch.empty(n, dtype=torch.float32, device=device) for _ in range(3))
+    _call(device, "mascot_pair_loss", p, q, u, i, j, beta, smoothing, ref, w, loss.data_ptr(), margin.data_ptr(), coef.data_ptr(),
+          _flag_word(flags, device))
+    return loss, margin, coef
+
+
+def pair_gradient(P, Q, users, preferred, other, coef, scale=1.0, dP=None, dQ=None, out_dtype=None, accumulate=False, workspace=None, flags=None):
+    """(dP, dQ): gradients of the sum of scale * loss, from the coef of pair_loss (mascot_pair_gradient); with `accumulate`
+    added to what dP and dQ hold."""
+    device = _device_of("P", P)
+    p, q = _rows("P", P, device), _rows("Q", Q, device)
+    u, i, j = _id_vector("users", users, device), _id_vector("preferred", preferred, device), _id_vector("other", other, device)
+    if accumulate and (dP is None or dQ is None):
+        _refuse("accumulate: needs dP and dQ")
+    dP = _result("dP", dP, P.shape, out_dtype if out_dtype is not None or dP is not None else P.dtype, device)
+    dQ = _result("dQ", dQ, Q.shape, out_dtype if out_dtype is not None or dQ is not None else Q.dtype, device)
+    c = _plain("coef", coef, _torch_ops().torch.float32, device, (u.count,))
+    keep, ws, size = _workspace(workspace, "mascot_pair_gradient_workspace", device, u.count, p.rows, q.rows, p.width)
+    _call(device, "mascot_pair_gradient", p, q, u, i, j, c, scale, _rows("dP", dP, device), _rows("dQ", dQ, device), 1 if accumulate else 0, ws,
+          size, _flag_word(flags, device))
+    return dP, dQ
+
+
+def rows_quantize(x, block_rows=1, q=None, scale=None):
+    """(q, scale): x as float8_e4m3fn with a power-of-two scale for each block of `block_rows` (1 or 128) rows by 128 columns, scale
+    [column blocks, row blocks] (mascot_rows_quantize).  A q of the call's own making has rows of a multiple of 128 bytes."""
+    device = _device_of("x", x)
+    torch = _torch_ops().torch
+    r = _rows("x", x, device)
+    if q is None:
+        q = torch.empty((r.rows, -(-r.width // 128) * 128), dtype=torch.float8_e4m3fn, device=device)[:, :r.width]
+    else:
+        q = _result("q", q, (r.rows, r.width), torch.float8_e4m3fn, device)
+    shape = (-(-r.width // 128), -(-r.rows // block_rows) if block_rows > 0 else 0)
+    if scale is None:
+        scale = torch.empty(shape, dtype=torch.float32, device=device)
+    s = _plain("scale", scale, torch.float32, device, shape)
+    _call(device, "mascot_rows_quantize", r, block_rows, _rows("q", q, device), s)
+    return q, scale
+
+
+def rows_product(a, a_scale, b, b_scale, out=None, out_dtype=None, flags=None):
+    """out[m][n] = the product of row m of a and row n of b, both float8_e4m3fn with their scales (mascot_rows_product): a with one
+    for each row and 128 columns, b for each 1 or 128 rows; float32 unless out_dtype says otherwise."""
+    device = _device_of("a", a)
+    torch = _torch_ops().torch
+    x, y = _rows("a", a, device), _rows("b", b, device)
+    sa = _plain("a_scale", a_scale, torch.float32, device, (-(-x.width // 128), x.rows))
+    each, sb = _scale_rows("b_scale", b_scale, y.rows, y.width, device)
+    out = _result("out", out, (x.rows, y.rows), out_dtype if out_dtype is not None or out is not None else torch.float32, device)
+    _call(device, "mascot_rows_product", x, sa, y, sb, each, _rows("out", out, device), _flag_word(flags, device))
+    return out

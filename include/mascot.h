@@ -415,6 +415,92 @@ MASCOT_API int mascot_rmse_device(const float* d_P, const float* d_Q, uint32_t k
 MASCOT_API int mascot_rmse_device_noalloc(const float* d_P, const float* d_Q, uint32_t k, const mascot_rating* d_test,
                                           uint64_t n_test, double* rmse);
 
+/* ---- operators on factor rows in device memory ----
+ *
+ * For programs that keep factor tables of their own on the GPU: rows by id and their gradient, training from
+ * preferences instead of ratings, tables held in 8 bits and the scores of all items from them.  No counterpart in the
+ * reference.  Conventions of this section:
+ *   - buffers are device (or managed) memory of the current device, checked by address; the call queues its kernels on
+ *     `stream` (a cudaStream_t of that device, NULL = the default stream) and returns without waiting.  It allocates
+ *     nothing and keeps nothing, so it may be captured into a graph (make one call of the same kind and types before:
+ *     the first one loads the kernels);
+ *   - scratch comes from the caller (16-byte aligned, as many bytes as the *_workspace call says).  It holds nothing between
+ *     calls, but calls that may run at the same time - on two streams, in two graphs - need one each;
+ *   - sums are fp32 in an order that the arguments fix: equal calls give equal bits;
+ *   - a matrix is a mascot_rows: any width and any stride of at least the width.  Rows move in pieces of 8 to 32 bytes where base,
+ *     stride and width of every matrix of the call are multiples of them, else element by element;
+ *   - an id of -1 (all bits set) names no row.  Any other id outside the table is treated as -1, never used as an index, and
+ *     sets MASCOT_FLAG_BAD_ID in *flags (a device word that the caller clears; flags may be NULL);
+ *   - outputs may share no element with inputs or with each other. */
+
+enum { MASCOT_F32 = 0, MASCOT_F16 = 1, MASCOT_BF16 = 2, MASCOT_E4M3 = 3 };     /* element types */
+enum { MASCOT_FLAG_BAD_ID = 1, MASCOT_FLAG_GAVE_UP = 2 };                      /* bits of *flags */
+
+typedef struct mascot_rows {
+    void* data;
+    uint64_t rows;           /* below 2^31 */
+    uint64_t stride;         /* elements from one row to the next */
+    uint32_t width;          /* elements of a row, 1 .. 65536 */
+    uint32_t type;           /* MASCOT_F32 ... */
+} mascot_rows;
+
+typedef struct mascot_ids {
+    const void* data;        /* signed integers of `bits` bits, one after the other */
+    uint64_t count;          /* below 2^31 */
+    uint32_t bits;           /* 32 or 64 */
+    uint32_t reserved;       /* 0 */
+} mascot_ids;
+
+/* out[j] = scale * table[ids[j]], in fp32, rounded to the type of out; zeros where ids[j] names no row.  out has ids->count rows.
+ * A table of MASCOT_E4M3 comes with its scales (mascot_rows_quantize), `block_rows` = 1 or 128 rows to each; for the
+ * other types table_scale is NULL and block_rows 0. */
+MASCOT_API int mascot_rows_lookup(const mascot_rows* table, const float* table_scale, uint32_t block_rows, const mascot_ids* ids,
+                                  float scale, const mascot_rows* out, uint32_t* flags, void* stream);
+
+/* The gradient of a lookup: out[r] = scale * (sum of grad[j] over the j with ids[j] = r), in the order of j, for every row r of
+ * `out` (rows that no id names become zeros); with `accumulate` that is added to what out[r] holds, and rows that no id
+ * names are left as they are.  The ids are sorted by row, and each row is summed by itself, in fp32 and without
+ * atomics. */
+MASCOT_API int mascot_rows_gradient(const mascot_rows* grad, const mascot_ids* ids, float scale, const mascot_rows* out, int accumulate,
+                                    void* workspace, uint64_t workspace_bytes, uint32_t* flags, void* stream);
+/* Scratch of mascot_rows_gradient for `count` ids and an output of `rows` x `width`; a pure function. */
+MASCOT_API int mascot_rows_gradient_workspace(uint64_t count, uint64_t rows, uint32_t width, uint64_t* bytes);
+
+/* Preference loss on pairs: user users[b] prefers item preferred[b] to item other[b].  In a softmax over the items the
+ * difference of the two log probabilities is the difference of the two scores, so that with
+ *     m = <P[u], Q[i] - Q[j]>,  z = beta * (m - reference[b])
+ * loss[b] = w * ((1 - smoothing) * log(1 + exp(-z)) + smoothing * log(1 + exp(z))) and coef[b] = dloss/dm
+ * = w * beta * (sigmoid(z) - (1 - smoothing)).  margin[b] = m: of a frozen model's tables it is the `reference` of another
+ * call.  reference and weight may be NULL (0 and 1), and so may any of the three outputs but not all.  A pair with an id that
+ * names no row has loss, margin and coef 0; one of weight 0 has loss and coef 0, whatever its margin.  P and Q have one width and one type (not MASCOT_E4M3); 0 <= smoothing <= 1. */
+MASCOT_API int mascot_pair_loss(const mascot_rows* P, const mascot_rows* Q, const mascot_ids* users, const mascot_ids* preferred,
+                                const mascot_ids* other, float beta, float smoothing, const float* reference, const float* weight,
+                                float* loss, float* margin, float* coef, uint32_t* flags, void* stream);
+/* Gradients of sum over b of scale * loss[b], given coef of mascot_pair_loss:
+ *     dP[u] += scale * coef * (Q[i] - Q[j]),  dQ[i] += scale * coef * P[u],  dQ[j] -= scale * coef * P[u]
+ * from zero, or with `accumulate` onto what dP and dQ hold.  dP and dQ have the shapes of P and Q and one type of their own.
+ * A pair with an id that names no row adds nothing, whatever its coef, and neither does one of coef 0, whatever its rows. */
+MASCOT_API int mascot_pair_gradient(const mascot_rows* P, const mascot_rows* Q, const mascot_ids* users, const mascot_ids* preferred,
+                                    const mascot_ids* other, const float* coef, float scale, const mascot_rows* dP, const mascot_rows* dQ,
+                                    int accumulate, void* workspace, uint64_t workspace_bytes, uint32_t* flags, void* stream);
+/* Scratch of mascot_pair_gradient for `count` pairs; a pure function. */
+MASCOT_API int mascot_pair_gradient_workspace(uint64_t count, uint64_t n_users, uint64_t n_items, uint32_t width, uint64_t* bytes);
+
+/* Rows to 8 bits: q = e4m3(x / s), rounded to nearest even, with one scale s for each block of `block_rows` (1 or 128) rows by
+ * 128 columns, the smallest power of two (not below 2^-126) with |x| / s <= 448 for every finite x of the block, 1 where they
+ * are all zero.  The division is exact, so each value is rounded once.  NaN and infinities become NaN in their place alone.
+ * scale[c * ceil(rows / block_rows) + r] belongs to column block c, row block r.  Columns of q from the width to the next
+ * multiple of 16, as far as the stride reaches, become zeros. */
+MASCOT_API int mascot_rows_quantize(const mascot_rows* x, uint32_t block_rows, const mascot_rows* q, float* scale, void* stream);
+
+/* Scores of all pairs of rows: out[m][n] = sum over column blocks c of a_scale * b_scale * (sum of a[m] * b[n] within c), for two
+ * matrices of MASCOT_E4M3 of one width with any fp32 scales in the layout of mascot_rows_quantize: a with a scale for each row
+ * and block of 128 columns, b with b_block_rows = 1 or 128 rows to a scale.  Products of a block are summed by the tensor
+ * cores, blocks in fp32.  a and b: base and stride multiples of 16 bytes; out: a_rows x b_rows, any type but MASCOT_E4M3.
+ * Should a wait inside the kernel run out, MASCOT_FLAG_GAVE_UP is set in *flags and the scores it concerns are NaN. */
+MASCOT_API int mascot_rows_product(const mascot_rows* a, const float* a_scale, const mascot_rows* b, const float* b_scale,
+                                   uint32_t b_block_rows, const mascot_rows* out, uint32_t* flags, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

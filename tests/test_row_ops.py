@@ -1,0 +1,202 @@
+"""CPU tests of the operators on factor rows: what the C ABI refuses before it touches a GPU, and the pure functions.  Addresses are
+made up: nothing here is launched, with or without a GPU."""
+import ctypes as C
+
+import pytest
+
+AT = 1 << 44            # not an address of anything
+GAP = 1 << 36
+
+
+def rows(mascot, n, width, type_=0, at=0, stride=None, data=None):
+    return mascot.Rows(AT + at * GAP if data is None else data, n, width if stride is None else stride, width, type_)
+
+
+def ids(mascot, n, at=8, bits=32, data=None, reserved=0):
+    return mascot.Ids(AT + at * GAP if data is None else data, n, bits, reserved)
+
+
+def refused(mascot, rc, *words):
+    assert rc == mascot.ERR_BAD_ARG, rc
+    text = mascot.load().mascot_last_error(None).decode()
+    for w in words:
+        assert w in text, text
+
+
+def reached_the_device(mascot, rc):
+    """All arguments were taken: what is missing is a GPU, or memory of one at the made-up address."""
+    import torch
+    if torch.cuda.is_available():
+        refused(mascot, rc, "not memory of the current device")
+    else:
+        assert rc == mascot.ERR_NO_DEVICE
+
+
+def lookup(mascot, table, i, out, scales=None, block_rows=0):
+    return mascot.load().mascot_rows_lookup(table, scales, block_rows, i, 1.0, out, None, None)
+
+
+def test_lookup_refuses(mascot):
+    M = mascot
+    t, i, o = rows(M, 10, 64), ids(M, 5), rows(M, 5, 64, at=1)
+    reached_the_device(M, lookup(M, t, i, o))
+    refused(M, lookup(M, None, i, o), "table", "null")
+    refused(M, lookup(M, t, None, o), "ids", "null")
+    refused(M, lookup(M, t, i, None), "out", "null")
+    refused(M, lookup(M, rows(M, 10, 64, 7), i, o), "table")
+    refused(M, lookup(M, t, i, rows(M, 5, 64, M.E4M3, 1)), "out")
+    refused(M, lookup(M, rows(M, 10, 64, stride=63), i, o), "stride")
+    refused(M, lookup(M, rows(M, 10, 0), i, o), "width")
+    refused(M, lookup(M, rows(M, 10, 65537), i, o), "width")
+    refused(M, lookup(M, rows(M, 1 << 31, 64), i, o), "rows")
+    refused(M, lookup(M, rows(M, 10, 64, data=0), i, o), "table", "null")
+    refused(M, lookup(M, rows(M, 10, 64, data=AT + 2), i, o), "table", "address")
+    refused(M, lookup(M, t, ids(M, 5, bits=16), o), "bits")
+    refused(M, lookup(M, t, ids(M, 5, reserved=1), o), "reserved")
+    refused(M, lookup(M, t, ids(M, 5, data=AT + 8 * GAP + 4, bits=64), o), "ids", "address")
+    refused(M, lookup(M, t, i, rows(M, 6, 64, at=1)), "out", "each id")
+    refused(M, lookup(M, t, i, rows(M, 5, 32, at=1)), "out", "width")
+    refused(M, lookup(M, t, i, rows(M, 5, 64)), "overlap")
+    refused(M, lookup(M, t, i, rows(M, 5, 64, data=AT + 8 * GAP)), "overlap")
+    refused(M, lookup(M, rows(M, 10, 64, M.E4M3), i, o), "block_rows")
+    refused(M, lookup(M, rows(M, 10, 64, M.E4M3), i, o, None, 1), "table_scale")
+    refused(M, lookup(M, t, i, o, AT + 3 * GAP, 1), "MASCOT_E4M3")
+    reached_the_device(M, lookup(M, rows(M, 10, 64, M.E4M3), i, o, AT + 3 * GAP, 128))
+    # two column halves of one matrix share no element
+    reached_the_device(M, lookup(M, rows(M, 10, 64, stride=128), i, rows(M, 5, 64, stride=128, data=AT + 256)))
+    refused(M, lookup(M, rows(M, 10, 64, stride=128), i, rows(M, 5, 64, stride=128, data=AT + 252)), "overlap")
+    assert lookup(M, t, ids(M, 0), rows(M, 0, 64, at=1)) == M.OK       # nothing to do
+
+
+def test_gradient_refuses(mascot):
+    M = mascot
+
+    def call(g, i, o, ws=AT + 4 * GAP, size=1 << 30, accumulate=0):
+        return M.load().mascot_rows_gradient(g, i, 1.0, o, accumulate, ws, size, None, None)
+    g, i, o = rows(M, 5, 64), ids(M, 5), rows(M, 10, 64, at=1)
+    reached_the_device(M, call(g, i, o))
+    refused(M, call(rows(M, 5, 64, M.E4M3), i, o), "grad")
+    refused(M, call(rows(M, 4, 64), i, o), "grad", "each id")
+    refused(M, call(g, i, rows(M, 10, 65, at=1)), "out", "width")
+    refused(M, call(g, i, o, None), "workspace")
+    refused(M, call(g, i, o, size=100), "workspace")
+    refused(M, call(g, i, o, AT + 4 * GAP + 8), "workspace", "aligned")
+    refused(M, call(g, i, o, AT + GAP), "workspace", "overlap")
+    refused(M, call(g, i, o, AT), "workspace", "overlap")
+    refused(M, call(g, i, rows(M, 10, 64)), "overlap")
+    assert call(rows(M, 0, 64), ids(M, 0), o, accumulate=1) == M.OK
+    reached_the_device(M, call(rows(M, 0, 64), ids(M, 0), o, None, 0))          # clears the table
+
+
+def test_pair_loss_refuses(mascot):
+    M = mascot
+
+    def call(P, Q, u, i, j, beta=1.0, eps=0.0, outs=(AT + 5 * GAP, AT + 6 * GAP, AT + 7 * GAP), ref=None, w=None):
+        return M.load().mascot_pair_loss(P, Q, u, i, j, beta, eps, ref, w, *outs, None, None)
+    P, Q = rows(M, 10, 64), rows(M, 8, 64, at=1)
+    u, i, j = ids(M, 5, 8), ids(M, 5, 9), ids(M, 5, 10)
+    reached_the_device(M, call(P, Q, u, i, j))
+    reached_the_device(M, call(P, Q, u, i, i, outs=(None, AT + 5 * GAP, None)))
+    refused(M, call(P, rows(M, 8, 32, at=1), u, i, j), "one width")
+    refused(M, call(P, rows(M, 8, 64, M.F16, 1), u, i, j), "one type")
+    refused(M, call(P, rows(M, 8, 64, M.E4M3, 1), u, i, j), "Q")
+    refused(M, call(P, Q, u, ids(M, 4, 9), j), "one count")
+    for eps in (-0.1, 1.5, float("nan")):
+        refused(M, call(P, Q, u, i, j, eps=eps), "smoothing")
+    for beta in (float("inf"), float("nan")):
+        refused(M, call(P, Q, u, i, j, beta=beta), "beta")
+    refused(M, call(P, Q, u, i, j, outs=(None, None, None)), "no output")
+    refused(M, call(P, Q, u, i, j, outs=(AT + 5 * GAP, AT + 5 * GAP + 8, None)), "overlap")
+    refused(M, call(P, Q, u, i, j, outs=(AT + 5 * GAP, None, None), ref=AT + 5 * GAP), "reference", "overlap")
+    refused(M, call(P, Q, u, i, j, outs=(AT, None, None)), "P", "overlap")
+    refused(M, call(P, Q, u, i, j, outs=(AT + 5 * GAP + 2, None, None)), "address")
+    assert call(P, Q, ids(M, 0), ids(M, 0), ids(M, 0)) == M.OK
+
+
+def test_pair_gradient_refuses(mascot):
+    M = mascot
+
+    def call(P, Q, dP, dQ, u=ids(M, 5, 8), i=ids(M, 5, 9), j=ids(M, 5, 10), coef=AT + 11 * GAP, ws=AT + 4 * GAP, size=1 << 30):
+        return M.load().mascot_pair_gradient(P, Q, u, i, j, coef, 1.0, dP, dQ, 0, ws, size, None, None)
+    P, Q, dP, dQ = rows(M, 10, 64), rows(M, 8, 64, at=1), rows(M, 10, 64, at=2), rows(M, 8, 64, at=3)
+    reached_the_device(M, call(P, Q, dP, dQ))
+    refused(M, call(P, Q, dP, rows(M, 9, 64, at=3)), "shapes")
+    refused(M, call(P, Q, dP, rows(M, 8, 64, M.BF16, 3)), "one type")
+    refused(M, call(P, Q, dP, dP), "shapes")
+    refused(M, call(P, Q, dP, rows(M, 8, 64, at=2)), "dP", "dQ", "overlap")
+    refused(M, call(P, Q, rows(M, 10, 64, at=1), dQ), "overlap")
+    refused(M, call(P, Q, dP, dQ, coef=None), "coef")
+    refused(M, call(P, Q, dP, dQ, ws=AT + 11 * GAP), "coef", "overlap")
+    refused(M, call(P, Q, dP, dQ, size=64), "workspace")
+    refused(M, call(rows(M, 1 << 30, 64), rows(M, 1 << 30, 64, at=1), rows(M, 1 << 30, 64, at=2), rows(M, 1 << 30, 64, at=3)), "2^31")
+    # the two gradients may be columns of one matrix
+    reached_the_device(M, call(P, rows(M, 10, 64, at=1), rows(M, 10, 64, stride=128, at=2), rows(M, 10, 64, stride=128, data=AT + 2 * GAP + 256)))
+
+
+def test_quantize_and_product_refuse(mascot):
+    M = mascot
+
+    def quantize(x, q, block_rows=1, scale=AT + 5 * GAP):
+        return M.load().mascot_rows_quantize(x, block_rows, q, scale, None)
+    x, q = rows(M, 10, 100), rows(M, 10, 100, M.E4M3, 1, 112)
+    reached_the_device(M, quantize(x, q))
+    refused(M, quantize(x, rows(M, 10, 100, 0, 1)), "q", "E4M3")
+    refused(M, quantize(rows(M, 10, 100, M.E4M3), q), "x")
+    refused(M, quantize(x, rows(M, 10, 101, M.E4M3, 1)), "q", "shape")
+    refused(M, quantize(x, q, 2), "block_rows")
+    refused(M, quantize(x, q, scale=None), "scale")
+    refused(M, quantize(x, q, scale=AT), "overlap")
+    refused(M, quantize(x, rows(M, 10, 100, M.E4M3, data=AT)), "overlap")
+    assert quantize(rows(M, 0, 100), rows(M, 0, 100, M.E4M3, 1)) == M.OK
+
+    def product(a, b, o, each=1, sa=AT + 5 * GAP, sb=AT + 6 * GAP):
+        return M.load().mascot_rows_product(a, sa, b, sb, each, o, None, None)
+    a, b, o = rows(M, 6, 100, M.E4M3, 0, 112), rows(M, 10, 100, M.E4M3, 1, 112), rows(M, 6, 10, M.BF16, 2)
+    reached_the_device(M, product(a, b, o))
+    reached_the_device(M, product(a, b, o, 128))
+    refused(M, product(rows(M, 6, 100, M.F16), b, o), "a", "E4M3")
+    refused(M, product(a, rows(M, 10, 99, M.E4M3, 1, 112), o), "one width")
+    refused(M, product(a, b, rows(M, 6, 11, 0, 2)), "out")
+    refused(M, product(a, b, rows(M, 6, 10, M.E4M3, 2)), "out")
+    refused(M, product(a, b, rows(M, 6, 10, 0, 2, 9)), "out", "stride")
+    refused(M, product(a, b, o, 64), "b_block_rows")
+    refused(M, product(a, b, o, sa=None), "null")
+    refused(M, product(rows(M, 6, 100, M.E4M3, 0, 104), b, o), "16 bytes")
+    refused(M, product(a, rows(M, 10, 100, M.E4M3, stride=112, data=AT + GAP + 8), o), "16 bytes")
+    refused(M, product(a, b, rows(M, 6, 10, data=AT)), "overlap")
+    assert product(rows(M, 0, 100, M.E4M3, 0, 112), b, rows(M, 0, 10, 0, 2)) == M.OK
+
+
+def test_workspace_sizes(mascot):
+    M, n = mascot, C.c_uint64()
+    lib = M.load()
+    assert lib.mascot_rows_gradient_workspace(0, 1000, 64, C.byref(n)) == M.OK and n.value == 0
+    last = 0
+    for count in (1, 100, 12_288, 12_289, 1 << 20, 1 << 22):
+        assert lib.mascot_rows_gradient_workspace(count, 1000, 64, C.byref(n)) == M.OK
+        assert n.value > last
+        last = n.value
+    assert last < 64 * (1 << 22)                     # far less than the gradients themselves
+    for args in ((1 << 31, 10, 64), (10, 1 << 31, 64), (10, 10, 0), (10, 10, 1 << 20)):
+        refused(M, lib.mascot_rows_gradient_workspace(*args, C.byref(n)), "out of range")
+    refused(M, lib.mascot_rows_gradient_workspace(1, 1, 1, None), "null")
+    refused(M, lib.mascot_pair_gradient_workspace(1 << 30, 10, 10, 64, C.byref(n)), "out of range")
+    refused(M, lib.mascot_pair_gradient_workspace(10, 1 << 30, 1 << 30, 64, C.byref(n)), "out of range")
+    assert lib.mascot_pair_gradient_workspace(10, 10, 10, 64, C.byref(n)) == M.OK and n.value > 0
+
+
+def test_struct_layout(mascot):
+    assert C.sizeof(mascot.Rows) == 32 and C.sizeof(mascot.Ids) == 24
+
+
+def test_tensors_off_the_gpu_are_refused(mascot):
+    import torch
+    x = torch.zeros(3, 64)
+    i = torch.zeros(3, dtype=torch.int32)
+    q = x.to(torch.float8_e4m3fn)
+    s = torch.ones(1, 3)
+    for f in (lambda: mascot.rows_lookup(x, i), lambda: mascot.rows_gradient(x, i, 3), lambda: mascot.pair_loss(x, x, i, i, i),
+              lambda: mascot.pair_gradient(x, x, i, i, i, torch.zeros(3)), lambda: mascot.rows_quantize(x), lambda: mascot.rows_product(q, s, q, s)):
+        with pytest.raises(mascot.MascotError) as e:
+            f()
+        assert e.value.status == mascot.ERR_BAD_ARG and "GPU" in str(e.value)
