@@ -19,7 +19,7 @@ namespace mascot {
 namespace {
 
 constexpr int kItems = 128;                          // items of a tile: lanes of tensor memory
-constexpr int kEpilogueThreads = 256, kProductThreads = kEpilogueThreads + 64;
+constexpr int kEpilogueThreads = 256, kProductThreads = kEpilogueThreads + 128;      // three warpgroups
 constexpr int kItemTileBytes = kItems * kScaleBlock;
 constexpr long long kPatience = 1ll << 33;           // cycles (four seconds) that a wait may take
 
@@ -125,8 +125,10 @@ __global__ void __launch_bounds__(kProductThreads, 1) product_kernel(const __gri
     fence_after();
     const uint32_t tmem = *tmem_slot;
 
-    if (warp == kEpilogueThreads / 32) {                        // operands
-        if (lane == 0) {
+    // 384 threads are launched with 168 registers each; those that hold sums take what the others leave: 128 * 56 + 256 * 224
+    if (warp >= kEpilogueThreads / 32) {
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
+        if (warp == kEpilogueThreads / 32 && lane == 0) {       // operands
             uint32_t step = 0;
             bool ok = true;
             for (uint32_t t = blockIdx.x; ok && t < p.tiles; t += gridDim.x) {
@@ -143,8 +145,7 @@ __global__ void __launch_bounds__(kProductThreads, 1) product_kernel(const __gri
             for (uint32_t q = step > kStages ? step - kStages : 0; q < step; q++) ok &= barrier_wait(full + q % kStages, q / kStages & 1);
             if (!ok && p.flags) atomicOr(p.flags, (uint32_t)MASCOT_FLAG_GAVE_UP);
         }
-    } else if (warp == kEpilogueThreads / 32 + 1) {             // matrix instructions
-        if (lane == 0) {
+        if (warp == kEpilogueThreads / 32 + 1 && lane == 0) {   // matrix instructions
             // accumulators fp32 (1 << 4), both operands e4m3 (0) and K-major (0), N / 8, M / 16
             constexpr uint32_t idesc = 1u << 4 | (uint32_t)(UN / 8) << 17 | (uint32_t)(kItems / 16) << 24;
             uint32_t step = 0;
@@ -164,6 +165,7 @@ __global__ void __launch_bounds__(kProductThreads, 1) product_kernel(const __gri
             if (!ok && p.flags) atomicOr(p.flags, (uint32_t)MASCOT_FLAG_GAVE_UP);
         }
     } else {                                                    // scales, sums, scores
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 224;");
         const int half = warp / 4;
         const uint32_t lanes = (uint32_t)(warp % 4) * 32;
         const auto scales_of = [&](uint32_t t, uint32_t c, float& user, float& item) {      // this thread's share of a step's scales
@@ -179,7 +181,7 @@ __global__ void __launch_bounds__(kProductThreads, 1) product_kernel(const __gri
         float next_user, next_item;
         scales_of(blockIdx.x, 0, next_user, next_item);
         for (uint32_t t = blockIdx.x; t < p.tiles; t += gridDim.x) {
-            float sum[kHalf];
+            float sum[kHalf] = {};
             for (uint32_t c = 0; c < p.col_blocks; c++, step++) {
                 const int b = step % kBuffers;
                 const float item_scale = next_item;
@@ -200,9 +202,12 @@ __global__ void __launch_bounds__(kProductThreads, 1) product_kernel(const __gri
                         if (lane == 0) barrier_arrive(spare + b);
                     }
 #pragma unroll
-                    for (int k = 0; k < kRead; k++) {
-                        const float x = part[k] * item_scale, s = scale[half * kHalf + k0 + k];
-                        sum[k0 + k] = c == 0 ? x * s : fmaf(x, s, sum[k0 + k]);
+                    for (int k = 0; k < kRead; k += 4) {
+                        const float4 s = *reinterpret_cast<const float4*>(scale + half * kHalf + k0 + k);
+                        sum[k0 + k] = fmaf(part[k] * item_scale, s.x, sum[k0 + k]);
+                        sum[k0 + k + 1] = fmaf(part[k + 1] * item_scale, s.y, sum[k0 + k + 1]);
+                        sum[k0 + k + 2] = fmaf(part[k + 2] * item_scale, s.z, sum[k0 + k + 2]);
+                        sum[k0 + k + 3] = fmaf(part[k + 3] * item_scale, s.w, sum[k0 + k + 3]);
                     }
                 }
             }
