@@ -1,14 +1,19 @@
 // Scores of every row of one e4m3 matrix against every row of another, with a scale for each block of 128 columns.
 //
-// out[m][n] = sum over column blocks c of a_scale[c][m] * b_scale[c][n] * <a[m], b[n]> within c.  Rows of b (items) are the 128 lanes of
-// an accumulator in tensor memory and rows of a (users) its columns: what a warp reads back of one column is 32 consecutive
-// scores of one row of `out`, stored as they come, whatever the alignment of `out`.  Each block of 128 columns is one
+// out[m][n] = sum over column blocks c of a_scale[c][m] * b_scale[c][n] * <a[m], b[n]> within c.  Each block of 128 columns is one
 // accumulation of four tcgen05.mma of kind f8f6f4 (a block is 128 bytes of a row, one line of the 128-byte swizzle); its sum is read
-// back, scaled and added in fp32 registers while the tensor cores work on the next one in another part of tensor memory.
+// back from tensor memory, scaled and added in fp32 registers while the tensor cores work on the next one in another part of it.
 //
-// A block of threads is persistent and takes every gridDim.x-th tile of 128 items x UN users: one warp fetches operands by TMA, one
-// issues the matrix instructions, eight read back, scale and store: warps w and w + 4 the lanes 32 (w % 4) on, half of the users
-// each.  Users are the inner index of the tiles, so that an item tile is fetched from HBM once and from L2 after that.
+// A block of threads is persistent and takes every gridDim.x-th tile of 128 lanes x CN columns of an accumulator.  One warp fetches
+// operands by TMA, one issues the matrix instructions, one fetches scales, the others read back, scale and store: warp w the
+// lanes 32 (w % 4) on, and columns of the group w / 4.  Rows of a (users) are the inner index of the tiles, so that rows
+// of b (items) are fetched from HBM once and from L2 after that.  What differs is which side the lanes are (Mode):
+//   ONE     rows of 128 columns and less: items.  What a warp reads back of an accumulator's column is 32 consecutive scores of
+//           a user, stored as they come, whatever the alignment of `out`.  Nothing is summed up, so registers allow 16 such warps.
+//   ROWS    longer rows, a scale for each row of b, or few users: items too.  A column's scale is a broadcast from shared memory,
+//           whose 128 bytes to a warp bound the step at 4 CN cycles, twice what the matrix instructions take.
+//   SQUARE  longer rows, a scale for 128 rows of b: users.  The scale of a lane and half of the columns is one number, kept in a
+//           register; scores go through shared memory to be stored along the rows of `out`.
 #include <cuda.h>
 
 #include <algorithm>
@@ -18,23 +23,35 @@
 namespace mascot {
 namespace {
 
-constexpr int kItems = 128;                          // items of a tile: lanes of tensor memory
-constexpr int kEpilogueThreads = 256, kProductThreads = kEpilogueThreads + 128;      // three warpgroups
-constexpr int kItemTileBytes = kItems * kScaleBlock;
+enum Mode { ONE, ROWS, SQUARE };
+constexpr int kLanes = 128;                          // lanes of tensor memory
+constexpr int kLaneTileBytes = kLanes * kScaleBlock;
+constexpr int kScaleSteps = 8;                       // steps whose scales are under way or in use: a step may be shorter than a fetch from HBM
+constexpr int kStagePitch = 80;                      // bytes of a row's piece of 64 on its way through shared memory (SQUARE)
 constexpr long long kPatience = 1ll << 33;           // cycles (four seconds) that a wait may take
 
-__host__ __device__ constexpr int stages_for(int users) { return users == 256 ? 4 : users == 128 ? 6 : 8; }
-__host__ __device__ constexpr int buffers_for(int users) { return users == 256 ? 2 : 4; }      // accumulators in tensor memory
-__host__ __device__ constexpr int columns_for(int users) { return users * buffers_for(users); }    // powers of two, 64 to 512
-__host__ __device__ constexpr size_t smem_for(int users) {
-    return 1024 + (size_t)stages_for(users) * (kItemTileBytes + users * kScaleBlock) + 2 * users * 4 + 8 * (2 * stages_for(users) + 2 * buffers_for(users)) + 16;
-}
+template <int CN, Mode MODE> struct Shape {
+    static constexpr int stages = CN == 256 ? 4 : CN == 128 ? 6 : 8;
+    static constexpr int buffers = CN == 256 ? 2 : 4;                        // accumulators in tensor memory
+    static constexpr int tmem_columns = CN * buffers;                        // powers of two, 64 to 512
+    static constexpr int groups = MODE == ONE && CN >= 64 ? 4 : 2;           // of four warps that read back, CN / groups columns each
+    static constexpr int readers = 4 * groups, threads = 32 * readers + 128;
+    static constexpr int stage_bytes = kLaneTileBytes + CN * kScaleBlock;
+    static constexpr int step_scales = kLanes + (MODE == SQUARE ? 4 : CN);
+    static constexpr int transit = MODE == SQUARE ? readers * 32 * kStagePitch : 0;
+    static constexpr size_t smem = 1024 + (size_t)stages * stage_bytes + transit + kScaleSteps * step_scales * 4 + 8 * (2 * stages + 2 * buffers + 2 * kScaleSteps) + 16;
+};
 
+// One side of the product: the lanes' or the columns' rows.
+struct Side {
+    const float* scale;
+    uint32_t rows, scales, shift;                    // scales of a column block, rows to a scale (log2)
+};
 struct ProductArgs {
-    const float *a_scale, *b_scale;
+    Side lane, col;
     void* out;
-    size_t out_stride;
-    uint32_t m, n, col_blocks, n_scales, user_tiles, tiles;      // n_scales: scales of b in a column block
+    size_t lane_step, col_step;                      // elements of `out` from one row of a side to the next
+    uint32_t blocks, user_tiles, tiles;              // blocks of 128 columns
     uint32_t* flags;
 };
 
@@ -68,6 +85,11 @@ __device__ __forceinline__ void fetch_tile(const CUtensorMap* map, void* to, uin
                  "l"(map), "r"(col), "r"(row), "r"(smem_at(bar)) : "memory");
 }
 
+// A word on its way to shared memory, zero instead where it is not there.
+__device__ __forceinline__ void fetch_word(float* to, const float* from, bool there) {
+    asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(smem_at(to)), "l"(from), "r"(there ? 4 : 0) : "memory");
+}
+
 // Operand in shared memory, K-major rows of 128 bytes in the 128-byte swizzle, eight rows (1024 bytes) to a group.
 __device__ __forceinline__ uint64_t operand_desc(const void* tile) {
     return (uint64_t)((smem_at(tile) & 0x3ffffu) >> 4) | 1ull << 16 | (uint64_t)(1024 >> 4) << 32 | 1ull << 46 | 2ull << 61;
@@ -82,149 +104,233 @@ __device__ __forceinline__ void commit(uint64_t* bar) {        // arrives when t
 __device__ __forceinline__ void fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
 __device__ __forceinline__ void fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
 
-// N consecutive columns of the warp's 32 lanes.
-template <int N> __device__ __forceinline__ void read_columns(uint32_t tmem, float (&v)[N]) {
-    static_assert(N == 8 || N == 16 || N == 32, "");
-    uint32_t r[N];
-    if constexpr (N == 32)
-        asm volatile("tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];"
-            : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]),
-              "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31]) : "r"(tmem));
-    else if constexpr (N == 16)
+// Sixteen or eight consecutive columns of the warp's 32 lanes, under way until wait_columns.
+template <int N> __device__ __forceinline__ void read_columns(uint32_t tmem, uint32_t (&r)[N]) {
+    static_assert(N == 8 || N == 16, "");
+    if constexpr (N == 16)
         asm volatile("tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
             : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]) : "r"(tmem));
     else
         asm volatile("tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
             : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]) : "r"(tmem));
-    asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
-#pragma unroll
-    for (int k = 0; k < N; k++) v[k] = __uint_as_float(r[k]);
+}
+// The registers are operands, so that nothing that uses them is moved before the wait.
+template <int N> __device__ __forceinline__ void wait_columns(uint32_t (&r)[N]) {
+    if constexpr (N == 16)
+        asm volatile("tcgen05.wait::ld.sync.aligned;" : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]), "+r"(r[8]), "+r"(r[9]), "+r"(r[10]),
+            "+r"(r[11]), "+r"(r[12]), "+r"(r[13]), "+r"(r[14]), "+r"(r[15]) :: "memory");
+    else
+        asm volatile("tcgen05.wait::ld.sync.aligned;" : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]) :: "memory");
 }
 
-template <int UN, typename Out, bool SQUARE>
-__global__ void __launch_bounds__(kProductThreads, 1) product_kernel(const __grid_constant__ CUtensorMap item_map, const __grid_constant__ CUtensorMap user_map, const ProductArgs p) {
-    constexpr int kStages = stages_for(UN), kBuffers = buffers_for(UN), kStageBytes = kItemTileBytes + UN * kScaleBlock, kHalf = UN / 2, kRead = kHalf < 32 ? kHalf : 32;
+// Two products, two sums at once.
+__device__ __forceinline__ uint64_t pair_of(float x, float y) { return (uint64_t)__float_as_uint(y) << 32 | __float_as_uint(x); }
+__device__ __forceinline__ uint64_t pair_of(uint32_t x, uint32_t y) { return (uint64_t)y << 32 | x; }
+__device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) { uint64_t d; asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b)); return d; }
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) { uint64_t d; asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c)); return d; }
+
+__device__ __forceinline__ float half_of(uint64_t pair, int which) { return __uint_as_float((uint32_t)(pair >> 32 * which)); }
+
+// Stores the warp's 32 rows of NC scores, two to an element of v, along the rows: 64 bytes of each row at a time go through `transit`.
+// `out`: the first row's first score; rows and cols: how many there are of them.
+template <typename Out, int NC>
+__device__ __forceinline__ void store_rows(const uint64_t (&v)[NC / 2], uint8_t* transit, Out* out, size_t stride, int rows, int cols, int lane) {
+    constexpr int kPiece = 64 / sizeof(Out);                    // scores of a row's piece
+    const uint32_t odd = (uint32_t)(reinterpret_cast<uintptr_t>(out) | stride * sizeof(Out));
+#pragma unroll
+    for (int c0 = 0; c0 < NC; c0 += kPiece) {
+        Out mine[kPiece];
+#pragma unroll
+        for (int k = 0; k < kPiece; k++) mine[k] = from_float<Out>(half_of(v[(c0 + k) / 2], k & 1));
+        __syncwarp();
+#pragma unroll
+        for (int k = 0; k < 4; k++) reinterpret_cast<uint4*>(transit + lane * kStagePitch)[k] = reinterpret_cast<const uint4*>(mine)[k];
+        __syncwarp();
+        if (odd % 16 == 0 && c0 + kPiece <= cols) {             // 16 bytes a lane, eight rows at once
+#pragma unroll
+            for (int r0 = 0; r0 < 32; r0 += 8) {
+                const int r = r0 + lane / 4;
+                const uint4 x = *reinterpret_cast<const uint4*>(transit + r * kStagePitch + lane % 4 * 16);
+                if (r < rows) *reinterpret_cast<uint4*>(out + r * stride + c0 + lane % 4 * (16 / sizeof(Out))) = x;
+            }
+        } else if (odd % 4 == 0 && c0 + kPiece <= cols) {       // 4 bytes a lane, two rows at once
+#pragma unroll 4
+            for (int r0 = 0; r0 < 32; r0 += 2) {
+                const int r = r0 + lane / 16;
+                const uint32_t x = *reinterpret_cast<const uint32_t*>(transit + r * kStagePitch + lane % 16 * 4);
+                if (r < rows) *reinterpret_cast<uint32_t*>(out + r * stride + c0 + lane % 16 * (4 / sizeof(Out))) = x;
+            }
+        } else {
+            for (int r = 0; r < rows; r++)
+                if (lane < kPiece && c0 + lane < cols) out[r * stride + c0 + lane] = reinterpret_cast<const Out*>(transit + r * kStagePitch)[lane];
+        }
+    }
+}
+
+template <int CN, typename Out, Mode MODE>
+__global__ void __launch_bounds__(Shape<CN, MODE>::threads, 1) product_kernel(const __grid_constant__ CUtensorMap lane_map, const __grid_constant__ CUtensorMap col_map, const ProductArgs p) {
+    using S = Shape<CN, MODE>;
+    constexpr int kStages = S::stages, kBuffers = S::buffers, kGroup = CN / S::groups, kRead = kGroup < 16 || MODE == ONE ? 8 : 16;
     extern __shared__ uint8_t raw[];
-    uint8_t* const tiles = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(raw) + 1023) / 1024 * 1024);      // the swizzle's period
-    float* const user_scale = reinterpret_cast<float*>(tiles + kStages * kStageBytes);                               // [2][UN]
-    uint64_t* const full = reinterpret_cast<uint64_t*>(user_scale + 2 * UN), *const empty = full + kStages;
+    uint8_t* const stages = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(raw) + 1023) / 1024 * 1024);     // the swizzle's period
+    uint8_t* const transit = stages + kStages * S::stage_bytes;
+    float* const scales = reinterpret_cast<float*>(transit + S::transit);                                            // [kScaleSteps][columns', lanes']
+    uint64_t* const full = reinterpret_cast<uint64_t*>(scales + kScaleSteps * S::step_scales), *const empty = full + kStages;
     uint64_t* const ready = empty + kStages, *const spare = ready + kBuffers;                                        // accumulators: summed, read back
-    uint32_t* const tmem_slot = reinterpret_cast<uint32_t*>(spare + kBuffers);
+    uint64_t* const scaled = spare + kBuffers, *const used = scaled + kScaleSteps;                                   // scales: there, used
+    uint32_t* const tmem_slot = reinterpret_cast<uint32_t*>(used + kScaleSteps);
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     if (threadIdx.x == 0) {
         for (int s = 0; s < kStages; s++) { barrier_init(full + s, 1); barrier_init(empty + s, 1); }
-        for (int b = 0; b < kBuffers; b++) { barrier_init(ready + b, 1); barrier_init(spare + b, kEpilogueThreads / 32); }
+        for (int b = 0; b < kBuffers; b++) { barrier_init(ready + b, 1); barrier_init(spare + b, S::readers); }
+        for (int s = 0; s < kScaleSteps; s++) { barrier_init(scaled + s, 32); barrier_init(used + s, S::readers); }
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
     if (warp == 0) {
-        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_at(tmem_slot)), "n"(columns_for(UN)) : "memory");
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_at(tmem_slot)), "n"(S::tmem_columns) : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
     }
     fence_before();
     __syncthreads();
     fence_after();
     const uint32_t tmem = *tmem_slot;
+    // first rows of tile t
+    const auto user_of = [&](uint32_t t) { return t % p.user_tiles * (MODE == SQUARE ? kLanes : CN); };
+    const auto item_of = [&](uint32_t t) { return t / p.user_tiles * (MODE == SQUARE ? CN : kLanes); };
+    const auto lane_of = [&](uint32_t t) { return MODE == SQUARE ? user_of(t) : item_of(t); };
+    const auto col_of = [&](uint32_t t) { return MODE == SQUARE ? item_of(t) : user_of(t); };
 
-    // 384 threads are launched with 168 registers each; those that hold sums take what the others leave: 128 * 56 + 256 * 224
-    if (warp >= kEpilogueThreads / 32) {
-        asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
-        if (warp == kEpilogueThreads / 32 && lane == 0) {       // operands
-            uint32_t step = 0;
-            bool ok = true;
+    if (warp >= S::readers) {
+        // Where sums take registers, 384 threads are launched with 168 each; those that hold sums take what the others leave: 128 * 56 + 256 * 224
+        if (MODE != ONE) asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
+        uint32_t step = 0;
+        bool ok = true;
+        if (warp == S::readers && lane == 0) {                  // operands
             for (uint32_t t = blockIdx.x; ok && t < p.tiles; t += gridDim.x) {
-                const int item0 = (int)(t / p.user_tiles) * kItems, user0 = (int)(t % p.user_tiles) * UN;
-                for (uint32_t c = 0; c < p.col_blocks; c++, step++) {
+                const int lane0 = (int)lane_of(t), col0 = (int)col_of(t);
+                for (uint32_t c = 0; c < p.blocks; c++, step++) {
                     const int s = step % kStages;
                     if (step >= kStages && !(ok = barrier_wait(empty + s, (step / kStages + 1) & 1))) break;
-                    barrier_expect(full + s, kStageBytes);
-                    fetch_tile(&item_map, tiles + s * kStageBytes, full + s, (int)(c * kScaleBlock), item0);
-                    fetch_tile(&user_map, tiles + s * kStageBytes + kItemTileBytes, full + s, (int)(c * kScaleBlock), user0);
+                    barrier_expect(full + s, S::stage_bytes);
+                    fetch_tile(&lane_map, stages + s * S::stage_bytes, full + s, (int)(c * kScaleBlock), lane0);
+                    fetch_tile(&col_map, stages + s * S::stage_bytes + kLaneTileBytes, full + s, (int)(c * kScaleBlock), col0);
                 }
             }
             // copies in flight end before the block does
             for (uint32_t q = step > kStages ? step - kStages : 0; q < step; q++) ok &= barrier_wait(full + q % kStages, q / kStages & 1);
-            if (!ok && p.flags) atomicOr(p.flags, (uint32_t)MASCOT_FLAG_GAVE_UP);
         }
-        if (warp == kEpilogueThreads / 32 + 1 && lane == 0) {   // matrix instructions
+        if (warp == S::readers + 1 && lane == 0) {              // matrix instructions
             // accumulators fp32 (1 << 4), both operands e4m3 (0) and K-major (0), N / 8, M / 16
-            constexpr uint32_t idesc = 1u << 4 | (uint32_t)(UN / 8) << 17 | (uint32_t)(kItems / 16) << 24;
-            uint32_t step = 0;
-            bool ok = true;
+            constexpr uint32_t idesc = 1u << 4 | (uint32_t)(CN / 8) << 17 | (uint32_t)(kLanes / 16) << 24;
             for (uint32_t t = blockIdx.x; ok && t < p.tiles; t += gridDim.x)
-                for (uint32_t c = 0; c < p.col_blocks; c++, step++) {
+                for (uint32_t c = 0; c < p.blocks; c++, step++) {
                     const int s = step % kStages, b = step % kBuffers;
                     if (step >= kBuffers && !(ok = barrier_wait(spare + b, (step / kBuffers + 1) & 1))) break;
                     if (!(ok = barrier_wait(full + s, step / kStages & 1))) break;
                     fence_after();
-                    const uint64_t items = operand_desc(tiles + s * kStageBytes), users = operand_desc(tiles + s * kStageBytes + kItemTileBytes);
+                    const uint64_t lanes = operand_desc(stages + s * S::stage_bytes), cols = operand_desc(stages + s * S::stage_bytes + kLaneTileBytes);
 #pragma unroll
-                    for (int k = 0; k < 4; k++) multiply(tmem + b * UN, items + 2 * k, users + 2 * k, idesc, k > 0);     // 32 columns each
+                    for (int k = 0; k < 4; k++) multiply(tmem + b * CN, lanes + 2 * k, cols + 2 * k, idesc, k > 0);      // 32 columns each
                     commit(empty + s);
                     commit(ready + b);
                 }
-            if (!ok && p.flags) atomicOr(p.flags, (uint32_t)MASCOT_FLAG_GAVE_UP);
         }
-    } else {                                                    // scales, sums, scores
-        asm volatile("setmaxnreg.inc.sync.aligned.u32 224;");
-        const int half = warp / 4;
+        if (warp == S::readers + 2) {                           // scales, 0 for rows that are not there
+            for (uint32_t t = blockIdx.x; ok && t < p.tiles; t += gridDim.x) {
+                const uint32_t lane0 = lane_of(t), col0 = col_of(t);
+                for (uint32_t c = 0; c < p.blocks; c++, step++) {
+                    const int q = step % kScaleSteps;
+                    if (step >= kScaleSteps && !(ok = __all_sync(0xffffffffu, barrier_wait(used + q, (step / kScaleSteps + 1) & 1)))) break;
+                    float* const to = scales + q * S::step_scales;
+                    const float* const of_lanes = p.lane.scale + (size_t)c * p.lane.scales, *const of_cols = p.col.scale + (size_t)c * p.col.scales;
+                    const auto fetch = [&](float* at, const float* from, const Side& side, uint32_t row) {
+                        fetch_word(at, from + (min(row, side.rows - 1) >> side.shift), row < side.rows);
+                    };
+                    if (MODE == SQUARE) { if (lane < S::groups) fetch(to + lane, of_cols, p.col, col0 + lane * kGroup); }
+                    else {
+#pragma unroll
+                        for (int k = lane; k < CN; k += 32) fetch(to + k, of_cols, p.col, col0 + k);
+                    }
+#pragma unroll
+                    for (int k = lane; k < kLanes; k += 32) fetch(to + S::step_scales - kLanes + k, of_lanes, p.lane, lane0 + k);
+                    asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(smem_at(scaled + q)) : "memory");
+                }
+            }
+            asm volatile("cp.async.wait_all;" ::: "memory");
+        }
+        if (!ok && p.flags) atomicOr(p.flags, (uint32_t)MASCOT_FLAG_GAVE_UP);
+    } else {                                                    // sums and scores
+        if (MODE != ONE) asm volatile("setmaxnreg.inc.sync.aligned.u32 224;");
+        const int group = warp / 4;
         const uint32_t lanes = (uint32_t)(warp % 4) * 32;
-        const auto scales_of = [&](uint32_t t, uint32_t c, float& user, float& item) {      // this thread's share of a step's scales
-            user = item = 0.f;
-            if (t >= p.tiles) return;
-            const uint32_t item0 = t / p.user_tiles * kItems, u = t % p.user_tiles * UN + threadIdx.x, i = item0 + lanes + lane;
-            if (threadIdx.x < UN && u < p.m) user = __ldg(p.a_scale + (size_t)c * p.m + u);
-            if (SQUARE) item = __ldg(p.b_scale + (size_t)c * p.n_scales + item0 / kScaleBlock);
-            else if (i < p.n) item = __ldg(p.b_scale + (size_t)c * p.n_scales + i);
-        };
         uint32_t step = 0;
         bool ok = true;
-        float next_user, next_item;
-        scales_of(blockIdx.x, 0, next_user, next_item);
         for (uint32_t t = blockIdx.x; t < p.tiles; t += gridDim.x) {
-            float sum[kHalf] = {};
-            for (uint32_t c = 0; c < p.col_blocks; c++, step++) {
-                const int b = step % kBuffers;
-                const float item_scale = next_item;
-                float* const scale = user_scale + (step & 1) * UN;
-                if (threadIdx.x < UN) scale[threadIdx.x] = next_user;
-                if (c + 1 < p.col_blocks) scales_of(t, c + 1, next_user, next_item);
-                else scales_of(t + gridDim.x, 0, next_user, next_item);
-                asm volatile("bar.sync 1, %0;" ::"n"(kEpilogueThreads) : "memory");      // one a step: its buffer is used again two steps on
-                ok = __all_sync(0xffffffffu, ok && barrier_wait(ready + b, step / kBuffers & 1));
+            const uint32_t l = lane_of(t) + lanes, c0 = col_of(t) + group * kGroup;      // the warp's first lane and column
+            Out* const out = static_cast<Out*>(p.out) + l * p.lane_step + c0 * p.col_step;
+            const int rows = l < p.lane.rows ? (int)min(p.lane.rows - l, 32u) : 0, cols = c0 < p.col.rows ? (int)min(p.col.rows - c0, (uint32_t)kGroup) : 0;
+            uint64_t sum[MODE == ONE ? 1 : kGroup / 2] = {};    // two columns each
+            for (uint32_t c = 0; c < p.blocks; c++, step++) {
+                const int b = step % kBuffers, q = step % kScaleSteps;
+                const float* const scale = scales + q * S::step_scales;
+                const uint32_t from = tmem + (lanes << 16) + b * CN + group * kGroup;
+                ok = __all_sync(0xffffffffu, ok && barrier_wait(scaled + q, step / kScaleSteps & 1) && barrier_wait(ready + b, step / kBuffers & 1));
                 fence_after();
+                uint32_t part[2][kRead];
+                read_columns<kRead>(from, part[0]);
+                float lane_scale = scale[S::step_scales - kLanes + lanes + lane];
+                if (MODE == SQUARE) lane_scale *= scale[group];
+                if (!ok) lane_scale = __int_as_float(0x7fffffff);
+                const uint64_t lane_scales = pair_of(lane_scale, lane_scale);
+                Out* to = out + lane;                           // ONE
 #pragma unroll
-                for (int k0 = 0; k0 < kHalf; k0 += kRead) {
-                    float part[kRead];
-                    read_columns<kRead>(tmem + (lanes << 16) + b * UN + half * kHalf + k0, part);
-                    if (k0 + kRead == kHalf) {
+                for (int k0 = 0; k0 < kGroup; k0 += kRead) {
+                    uint32_t (&now)[kRead] = part[k0 / kRead & 1];
+                    wait_columns<kRead>(now);
+                    if (k0 + kRead < kGroup) read_columns<kRead>(from + k0 + kRead, part[(k0 / kRead + 1) & 1]);
+                    else {
                         fence_before();
                         __syncwarp();
                         if (lane == 0) barrier_arrive(spare + b);
                     }
 #pragma unroll
                     for (int k = 0; k < kRead; k += 4) {
-                        const float4 s = *reinterpret_cast<const float4*>(scale + half * kHalf + k0 + k);
-                        sum[k0 + k] = fmaf(part[k] * item_scale, s.x, sum[k0 + k]);
-                        sum[k0 + k + 1] = fmaf(part[k + 1] * item_scale, s.y, sum[k0 + k + 1]);
-                        sum[k0 + k + 2] = fmaf(part[k + 2] * item_scale, s.z, sum[k0 + k + 2]);
-                        sum[k0 + k + 3] = fmaf(part[k + 3] * item_scale, s.w, sum[k0 + k + 3]);
+                        const uint64_t x[2] = {pair_of(now[k], now[k + 1]), pair_of(now[k + 2], now[k + 3])};
+                        if constexpr (MODE == SQUARE) {
+                            sum[(k0 + k) / 2] = fma2(x[0], lane_scales, sum[(k0 + k) / 2]);
+                            sum[(k0 + k) / 2 + 1] = fma2(x[1], lane_scales, sum[(k0 + k) / 2 + 1]);
+                        } else {
+                            const ulonglong2 s = *reinterpret_cast<const ulonglong2*>(scale + group * kGroup + k0 + k);
+                            if constexpr (MODE == ROWS) {
+                                sum[(k0 + k) / 2] = fma2(mul2(x[0], lane_scales), s.x, sum[(k0 + k) / 2]);
+                                sum[(k0 + k) / 2 + 1] = fma2(mul2(x[1], lane_scales), s.y, sum[(k0 + k) / 2 + 1]);
+                            } else {
+                                const uint64_t y[2] = {mul2(mul2(x[0], lane_scales), s.x), mul2(mul2(x[1], lane_scales), s.y)};
+#pragma unroll
+                                for (int i = 0; i < 4; i++, to += p.col_step)
+                                    if (lane < rows && k0 + k + i < cols) *to = from_float<Out>(half_of(y[i / 2], i & 1));
+                            }
+                        }
                     }
                 }
+                __syncwarp();
+                if (lane == 0) barrier_arrive(used + q);
             }
-            const uint32_t i = t / p.user_tiles * kItems + lanes + lane, u0 = t % p.user_tiles * UN + half * kHalf;
-            if (i < p.n) {
-                Out* out = static_cast<Out*>(p.out) + (size_t)u0 * p.out_stride + i;
-                const int users = u0 < p.m ? (int)min(p.m - u0, (uint32_t)kHalf) : 0;
+            if constexpr (MODE == ROWS) {
+                if (lane < rows) {
+                    Out* to = out + lane;
 #pragma unroll
-                for (int k = 0; k < kHalf; k++, out += p.out_stride)
-                    if (k < users) *out = from_float<Out>(ok ? sum[k] : __int_as_float(0x7fffffff));
+                    for (int k = 0; k < kGroup; k++, to += p.col_step)
+                        if (k < cols) *to = from_float<Out>(half_of(sum[k / 2], k & 1));
+                }
             }
+            if constexpr (MODE == SQUARE) store_rows<Out, kGroup>(sum, transit + warp * 32 * kStagePitch, out, p.lane_step, rows, cols, lane);
         }
         if (!ok && lane == 0 && p.flags) atomicOr(p.flags, (uint32_t)MASCOT_FLAG_GAVE_UP);
         fence_before();
     }
     __syncthreads();
-    if (warp == 0) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "n"(columns_for(UN)) : "memory");
+    if (warp == 0) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "n"(S::tmem_columns) : "memory");
 }
 
 using EncodeTiled = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*, const cuuint32_t*, const cuuint32_t*,
@@ -250,37 +356,49 @@ int sm_count() {
     return cudaGetDevice(&dev) == cudaSuccess && cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev) == cudaSuccess ? n : 1;
 }
 
-template <int UN, typename Out, bool SQUARE>
-cudaError_t launch_product(const mascot_rows& a, const mascot_rows& b, ProductArgs p, int sms, cudaStream_t st) {
-    CUtensorMap items, users;
-    if (!tile_map(&items, b, kItems) || !tile_map(&users, a, UN)) return cudaErrorInvalidValue;
-    p.user_tiles = (p.m + UN - 1) / UN;
-    p.tiles = p.user_tiles * ((p.n + kItems - 1) / kItems);
-    const cudaError_t e = cudaFuncSetAttribute(product_kernel<UN, Out, SQUARE>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem_for(UN));
+template <int CN, typename Out, Mode MODE>
+cudaError_t launch_product(const mascot_rows& a, const mascot_rows& b, const ProductArgs& given, int sms, cudaStream_t st) {
+    using S = Shape<CN, MODE>;
+    ProductArgs p = given;                                      // lane side: items, column side: users
+    const uint32_t users = MODE == SQUARE ? kLanes : CN, items = MODE == SQUARE ? CN : kLanes;
+    if (MODE == SQUARE) { std::swap(p.lane, p.col); std::swap(p.lane_step, p.col_step); }
+    CUtensorMap lane_map, col_map;
+    if (!tile_map(&lane_map, MODE == SQUARE ? a : b, kLanes) || !tile_map(&col_map, MODE == SQUARE ? b : a, CN)) return cudaErrorInvalidValue;
+    p.user_tiles = (uint32_t)((a.rows + users - 1) / users);
+    p.tiles = p.user_tiles * (uint32_t)((b.rows + items - 1) / items);
+    const cudaError_t e = cudaFuncSetAttribute(product_kernel<CN, Out, MODE>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)S::smem);
     if (e != cudaSuccess) return e;
-    product_kernel<UN, Out, SQUARE><<<std::min<uint32_t>(p.tiles, sms), kProductThreads, smem_for(UN), st>>>(items, users, p);
+    product_kernel<CN, Out, MODE><<<std::min<uint32_t>(p.tiles, sms), S::threads, S::smem, st>>>(lane_map, col_map, p);
     return cudaGetLastError();
 }
 
 // Users of a tile: as many as there are, up to 256, but fewer where that leaves SMs without a tile.
-int users_of_tile(uint32_t m, uint32_t n, int sms) {
+int users_of_tile(uint64_t m, uint64_t n, int sms) {
     int users = 16;
-    while (users < 256 && (uint32_t)users < m) users *= 2;
-    const uint32_t item_tiles = (n + kItems - 1) / kItems;
-    while (users > 32 && (uint64_t)item_tiles * ((m + users - 1) / users) < (uint32_t)sms) users /= 2;
+    while (users < 256 && (uint64_t)users < m) users *= 2;
+    while (users > 32 && (n + kLanes - 1) / kLanes * ((m + users - 1) / users) < (uint64_t)sms) users /= 2;
     return users;
 }
 
-template <typename Out, bool SQUARE>
+template <typename Out, Mode MODE>
+cudaError_t launch_users(const mascot_rows& a, const mascot_rows& b, const ProductArgs& p, int sms, cudaStream_t st) {
+    switch (users_of_tile(a.rows, b.rows, sms)) {
+        case 16: return launch_product<16, Out, MODE>(a, b, p, sms, st);
+        case 32: return launch_product<32, Out, MODE>(a, b, p, sms, st);
+        case 64: return launch_product<64, Out, MODE>(a, b, p, sms, st);
+        case 128: return launch_product<128, Out, MODE>(a, b, p, sms, st);
+        default: return launch_product<256, Out, MODE>(a, b, p, sms, st);
+    }
+}
+
+template <typename Out>
 cudaError_t launch_tiles(const mascot_rows& a, const mascot_rows& b, const ProductArgs& p, cudaStream_t st) {
     const int sms = sm_count();
-    switch (users_of_tile(p.m, p.n, sms)) {
-        case 16: return launch_product<16, Out, SQUARE>(a, b, p, sms, st);
-        case 32: return launch_product<32, Out, SQUARE>(a, b, p, sms, st);
-        case 64: return launch_product<64, Out, SQUARE>(a, b, p, sms, st);
-        case 128: return launch_product<128, Out, SQUARE>(a, b, p, sms, st);
-        default: return launch_product<256, Out, SQUARE>(a, b, p, sms, st);
-    }
+    if (p.blocks == 1) return launch_users<Out, ONE>(a, b, p, sms, st);
+    // lanes for users pay where there are enough for all of them; half a tile of items where whole ones leave SMs without a tile
+    if (p.lane.shift && a.rows > kLanes)
+        return (a.rows + kLanes - 1) / kLanes * ((b.rows + 255) / 256) >= (uint64_t)sms ? launch_product<256, Out, SQUARE>(a, b, p, sms, st) : launch_product<128, Out, SQUARE>(a, b, p, sms, st);
+    return launch_users<Out, ROWS>(a, b, p, sms, st);
 }
 
 }  // namespace
@@ -292,7 +410,7 @@ extern "C" int mascot_rows_product(const mascot_rows* a, const float* a_scale, c
                                    const mascot_rows* out, uint32_t* flags, void* stream) {
     ROW_CHECK(check_rows("a", a, true));
     ROW_CHECK(check_rows("b", b, true));
-    if (((a->rows + 15) / 16) * ((b->rows + kItems - 1) / kItems) > 0x3fffffffull) return fail(nullptr, MASCOT_ERR_UNSUPPORTED, "too many scores for one call: split a or b");
+    if (((a->rows + 15) / 16) * ((b->rows + kLanes - 1) / kLanes) > 0x3fffffffull) return fail(nullptr, MASCOT_ERR_UNSUPPORTED, "too many scores for one call: split a or b");
     if (!out) return fail(nullptr, MASCOT_ERR_BAD_ARG, "out: null pointer");
     if (out->rows != a->rows || out->width != b->rows) return fail(nullptr, MASCOT_ERR_BAD_ARG, "out: must have a row for each of a, and a column for each of b");
     if (a->width != b->width) return fail(nullptr, MASCOT_ERR_BAD_ARG, "a and b must have one width");
@@ -319,11 +437,13 @@ extern "C" int mascot_rows_product(const mascot_rows* a, const float* a_scale, c
     ROW_CHECK(check_memory("out", out->data));
     ROW_CHECK(check_memory("flags", flags));
     if (!encode_tiled()) return fail(nullptr, MASCOT_ERR_UNSUPPORTED, "the driver has no cuTensorMapEncodeTiled");
-    const ProductArgs p{a_scale, b_scale, out->data, out->stride, (uint32_t)a->rows, (uint32_t)b->rows, col_blocks, n_scales, 0, 0, flags};
-    const cudaError_t e = with_type(out->type, [&](auto* o) {
-        using Out = std::remove_pointer_t<decltype(o)>;
-        return b_block_rows == 1 ? launch_tiles<Out, false>(*a, *b, p, static_cast<cudaStream_t>(stream)) : launch_tiles<Out, true>(*a, *b, p, static_cast<cudaStream_t>(stream));
-    });
+    ProductArgs p = {};
+    p.lane = Side{b_scale, (uint32_t)b->rows, n_scales, b_block_rows == 1 ? 0u : 7u};
+    p.col = Side{a_scale, (uint32_t)a->rows, (uint32_t)a->rows, 0};
+    p.out = out->data; p.lane_step = 1; p.col_step = out->stride;
+    p.blocks = col_blocks;
+    p.flags = flags;
+    const cudaError_t e = with_type(out->type, [&](auto* o) { return launch_tiles<std::remove_pointer_t<decltype(o)>>(*a, *b, p, static_cast<cudaStream_t>(stream)); });
     CU(nullptr, e);
     return MASCOT_OK;
 }
