@@ -592,12 +592,12 @@ int mascot_rows_gradient(const mascot_rows* grad, const mascot_ids* ids, float s
     int which = 0;
     if (j.n) CU(nullptr, sort_entries(j, s, &which, st));
     const bool aligned = aligned_rows(*grad, 4) && aligned_rows(*out, 4);
-    const cudaError_t e = with_type(grad->type, [&](auto* t) {
+    const cudaError_t launched = with_type(grad->type, [&](auto* t) {
         return with_type(out->type, [&](auto* o) {
             return sum_entries<std::remove_pointer_t<decltype(t)>, std::remove_pointer_t<decltype(o)>, false>(j, s, which, aligned, st);
         });
     });
-    CU(nullptr, e);
+    CU(nullptr, launched);
     return MASCOT_OK;
 }
 
@@ -657,12 +657,12 @@ int mascot_pair_gradient(const mascot_rows* P, const mascot_rows* Q, const masco
     int which = 0;
     if (j.n) CU(nullptr, sort_entries(j, s, &which, st));
     const bool aligned = aligned_rows(*P, 4) && aligned_rows(*Q, 4) && aligned_rows(*dP, 4) && aligned_rows(*dQ, 4);
-    const cudaError_t e = with_type(P->type, [&](auto* t) {
+    const cudaError_t launched = with_type(P->type, [&](auto* t) {
         return with_type(dP->type, [&](auto* o) {
             return sum_entries<std::remove_pointer_t<decltype(t)>, std::remove_pointer_t<decltype(o)>, true>(j, s, which, aligned, st);
         });
     });
-    CU(nullptr, e);
+    CU(nullptr, launched);
     return MASCOT_OK;
 }
 

@@ -390,13 +390,13 @@ int mascot_rows_lookup(const mascot_rows* table, const float* table_scale, uint3
     LookupArgs a{table->data, table_scale, out->data, table->stride, out->stride, ids->count, ids_of(*ids), (uint32_t)table->rows, table->width,
                  (uint32_t)row_blocks, block_rows == kScaleBlock ? 7u : 0u, scale, flags};
     const cudaStream_t st = static_cast<cudaStream_t>(stream);
-    const cudaError_t e = with_type(out->type, [&](auto* o) {
+    const cudaError_t launched = with_type(out->type, [&](auto* o) {
         using Out = std::remove_pointer_t<decltype(o)>;
         const bool aligned = aligned_rows(*table, 16 / sizeof(Out)) && aligned_rows(*out, 16 / sizeof(Out));
         if (e4m3) return launch_lookup<E4m3, Out>(a, aligned, st);
         return with_type(table->type, [&](auto* t) { return launch_lookup<std::remove_pointer_t<decltype(t)>, Out>(a, aligned, st); });
     });
-    CU(nullptr, e);
+    CU(nullptr, launched);
     return MASCOT_OK;
 }
 
@@ -434,11 +434,11 @@ int mascot_pair_loss(const mascot_rows* P, const mascot_rows* Q, const mascot_id
     for (const auto& x : out) ROW_CHECK(check_memory(x.what, x.p));
     const PairArgs a{P->data, Q->data, P->stride, Q->stride, n, ids_of(*users), ids_of(*preferred), ids_of(*other), (uint32_t)P->rows, (uint32_t)Q->rows,
                      P->width, beta, smoothing, reference, weight, loss, margin, coef, flags};
-    const cudaError_t e = with_type(P->type, [&](auto* t) {
+    const cudaError_t launched = with_type(P->type, [&](auto* t) {
         using T = std::remove_pointer_t<decltype(t)>;
         return launch_pair_loss<T>(a, aligned_rows(*P, 16 / sizeof(T)) && aligned_rows(*Q, 16 / sizeof(T)), static_cast<cudaStream_t>(stream));
     });
-    CU(nullptr, e);
+    CU(nullptr, launched);
     return MASCOT_OK;
 }
 
@@ -465,7 +465,7 @@ int mascot_rows_quantize(const mascot_rows* x, uint32_t block_rows, const mascot
     const QuantArgs a{x->data, static_cast<uint8_t*>(q->data), scale, x->stride, q->stride, (uint32_t)x->rows, x->width, padded, row_blocks};
     const cudaStream_t st = static_cast<cudaStream_t>(stream);
     const bool aligned = aligned_rows(*x, 4) && aligned_rows(q_written, 4);
-    const cudaError_t e = with_type(x->type, [&](auto* t) {
+    const cudaError_t launched = with_type(x->type, [&](auto* t) {
         using T = std::remove_pointer_t<decltype(t)>;
         if (block_rows == 1) {
             const size_t blocks = ((size_t)a.rows * col_blocks + kQuantBlock / 32 - 1) / (kQuantBlock / 32);
@@ -480,7 +480,7 @@ int mascot_rows_quantize(const mascot_rows* x, uint32_t block_rows, const mascot
         }
         return cudaGetLastError();
     });
-    CU(nullptr, e);
+    CU(nullptr, launched);
     return MASCOT_OK;
 }
 

@@ -8,8 +8,9 @@
 // operands by TMA, one issues the matrix instructions, one fetches scales, the others read back, scale and store: warp w the
 // lanes 32 (w % 4) on, and columns of the group w / 4.  Rows of a (users) are the inner index of the tiles, so that rows
 // of b (items) are fetched from HBM once and from L2 after that.  What differs is which side the lanes are (Mode):
-//   ONE     rows of 128 columns and less: items.  What a warp reads back of an accumulator's column is 32 consecutive scores of
-//           a user, stored as they come, whatever the alignment of `out`.  Nothing is summed up, so registers allow 16 such warps.
+//   ONE     rows of 128 columns and less: items.  What is written bounds it.  Four warps read 8 columns of all lanes at a time, meet
+//           over shared memory and store whole rows of 128 scores, in pieces as wide as the row's address allows (32 scores a
+//           warp, straight from the accumulator, took 1.4 times as long).  Nothing is summed up, so registers allow 16 such warps.
 //   ROWS    longer rows, a scale for each row of b, or few users: items too.  A column's scale is a broadcast from shared memory,
 //           whose 128 bytes to a warp bound the step at 4 CN cycles, twice what the matrix instructions take.
 //   SQUARE  longer rows, a scale for 128 rows of b: users.  The scale of a lane and half of the columns is one number, kept in a
@@ -28,18 +29,20 @@ constexpr int kLanes = 128;                          // lanes of tensor memory
 constexpr int kLaneTileBytes = kLanes * kScaleBlock;
 constexpr int kScaleSteps = 8;                       // steps whose scales are under way or in use: a step may be shorter than a fetch from HBM
 constexpr int kStagePitch = 80;                      // bytes of a row's piece of 64 on its way through shared memory (SQUARE)
-constexpr long long kPatience = 1ll << 33;           // cycles (four seconds) that a wait may take
+constexpr uint32_t kNap = 10'000'000;                // ns; a wait gives up after kTries of them (at least: a try may end early)
+constexpr int kTries = 4000;
 
 template <int CN, Mode MODE> struct Shape {
-    static constexpr int stages = CN == 256 ? 4 : CN == 128 ? 6 : 8;
+    static constexpr int stages = CN == 256 ? (MODE == ONE ? 3 : 4) : CN == 128 ? (MODE == ONE ? 4 : 6) : MODE == ONE && CN == 64 ? 6 : 8;
     static constexpr int buffers = CN == 256 ? 2 : 4;                        // accumulators in tensor memory
     static constexpr int tmem_columns = CN * buffers;                        // powers of two, 64 to 512
     static constexpr int groups = MODE == ONE && CN >= 64 ? 4 : 2;           // of four warps that read back, CN / groups columns each
     static constexpr int readers = 4 * groups, threads = 32 * readers + 128;
     static constexpr int stage_bytes = kLaneTileBytes + CN * kScaleBlock;
     static constexpr int step_scales = kLanes + (MODE == SQUARE ? 4 : CN);
-    static constexpr int transit = MODE == SQUARE ? readers * 32 * kStagePitch : 0;
+    static constexpr int transit = MODE == SQUARE ? readers * 32 * kStagePitch : MODE == ONE ? groups * 2 * (CN / groups < 16 ? 8 : 16) * kLanes * 4 : 0;
     static constexpr size_t smem = 1024 + (size_t)stages * stage_bytes + transit + kScaleSteps * step_scales * 4 + 8 * (2 * stages + 2 * buffers + 2 * kScaleSteps) + 16;
+    static_assert(smem <= 227 * 1024, "shared memory of a block");
 };
 
 // One side of the product: the lanes' or the columns' rows.
@@ -66,17 +69,16 @@ __device__ __forceinline__ void barrier_arrive(uint64_t* b) {
 __device__ __forceinline__ void barrier_expect(uint64_t* b, uint32_t bytes) {
     asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(smem_at(b)), "r"(bytes) : "memory");
 }
-// Waits for the phase of that parity to end, but not for ever.
+// Waits for the phase of that parity to end, but not for ever: each try sleeps up to kNap ns.
 __device__ __forceinline__ bool barrier_wait(uint64_t* b, uint32_t parity) {
     const uint32_t at = smem_at(b);
-    long long begin = 0;
-    for (int round = 0;; round++) {
+#pragma unroll 1
+    for (int tries = 0; tries < kTries; tries++) {
         uint32_t done;
-        asm volatile("{ .reg .pred p; mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2; selp.u32 %0, 1, 0, p; }" : "=r"(done) : "r"(at), "r"(parity) : "memory");
+        asm volatile("{ .reg .pred p; mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, %3; selp.u32 %0, 1, 0, p; }" : "=r"(done) : "r"(at), "r"(parity), "r"(kNap) : "memory");
         if (done) return true;
-        if (round == 0) begin = clock64();
-        else if (clock64() - begin > kPatience) return false;
     }
+    return false;
 }
 
 // Box of 128 columns by the map's rows at (column, row) into shared memory; what lies outside the matrix is zero.
@@ -131,6 +133,37 @@ __device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) { u
 
 __device__ __forceinline__ float half_of(uint64_t pair, int which) { return __uint_as_float((uint32_t)(pair >> 32 * which)); }
 
+// Stores N columns of the warp's lanes, two to an element of v, at the offsets `at` from an address that is the same for the warp.
+template <typename Out, int N>
+__device__ __forceinline__ void store_columns(uint8_t* base, const uint32_t* at, const uint64_t* v, bool there, int cols) {
+    if (cols >= N) {
+#pragma unroll
+        for (int k = 0; k < N; k++) if (there) *reinterpret_cast<Out*>(base + at[k]) = from_float<Out>(half_of(v[k / 2], k & 1));
+    } else {
+#pragma unroll
+        for (int k = 0; k < N; k++) if (there && k < cols) *reinterpret_cast<Out*>(base + at[k]) = from_float<Out>(half_of(v[k / 2], k & 1));
+    }
+}
+
+// Stores R rows of 128 scores, fp32 in shared memory, each times its scale: a warp, WIDE neighbours a lane.
+template <typename Out, int R, int WIDE>
+__device__ __forceinline__ void store_whole(uint8_t* to, size_t pitch, const float* from, const float* scale, int lane) {
+    float s[R];
+#pragma unroll
+    for (int r = 0; r < R; r++) s[r] = scale[r];
+#pragma unroll
+    for (int r = 0; r < R; r++, to += pitch) {
+#pragma unroll
+        for (int k = 0; k < 4 / WIDE; k++) {
+            const Piece<float, WIDE> x = reinterpret_cast<const Piece<float, WIDE>*>(from + r * kLanes)[lane + 32 * k];
+            Piece<Out, WIDE> y;
+#pragma unroll
+            for (int i = 0; i < WIDE; i++) y.v[i] = from_float<Out>(x.v[i] * s[r]);
+            reinterpret_cast<Piece<Out, WIDE>*>(to)[lane + 32 * k] = y;
+        }
+    }
+}
+
 // Stores the warp's 32 rows of NC scores, two to an element of v, along the rows: 64 bytes of each row at a time go through `transit`.
 // `out`: the first row's first score; rows and cols: how many there are of them.
 template <typename Out, int NC>
@@ -170,16 +203,16 @@ __device__ __forceinline__ void store_rows(const uint64_t (&v)[NC / 2], uint8_t*
 template <int CN, typename Out, Mode MODE>
 __global__ void __launch_bounds__(Shape<CN, MODE>::threads, 1) product_kernel(const __grid_constant__ CUtensorMap lane_map, const __grid_constant__ CUtensorMap col_map, const ProductArgs p) {
     using S = Shape<CN, MODE>;
-    constexpr int kStages = S::stages, kBuffers = S::buffers, kGroup = CN / S::groups, kRead = kGroup < 16 || MODE == ONE ? 8 : 16;
+    constexpr int kStages = S::stages, kBuffers = S::buffers, kGroup = CN / S::groups, kRead = kGroup < 16 ? 8 : 16;
     extern __shared__ uint8_t raw[];
-    uint8_t* const stages = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(raw) + 1023) / 1024 * 1024);     // the swizzle's period
+    uint8_t* const stages = raw + (1024 - smem_at(raw) % 1024) % 1024;                                               // the swizzle's period
     uint8_t* const transit = stages + kStages * S::stage_bytes;
     float* const scales = reinterpret_cast<float*>(transit + S::transit);                                            // [kScaleSteps][columns', lanes']
     uint64_t* const full = reinterpret_cast<uint64_t*>(scales + kScaleSteps * S::step_scales), *const empty = full + kStages;
     uint64_t* const ready = empty + kStages, *const spare = ready + kBuffers;                                        // accumulators: summed, read back
     uint64_t* const scaled = spare + kBuffers, *const used = scaled + kScaleSteps;                                   // scales: there, used
     uint32_t* const tmem_slot = reinterpret_cast<uint32_t*>(used + kScaleSteps);
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;     // the same for the warp, and known to be
     if (threadIdx.x == 0) {
         for (int s = 0; s < kStages; s++) { barrier_init(full + s, 1); barrier_init(empty + s, 1); }
         for (int b = 0; b < kBuffers; b++) { barrier_init(ready + b, 1); barrier_init(spare + b, S::readers); }
@@ -263,11 +296,23 @@ __global__ void __launch_bounds__(Shape<CN, MODE>::threads, 1) product_kernel(co
         if (MODE != ONE) asm volatile("setmaxnreg.inc.sync.aligned.u32 224;");
         const int group = warp / 4;
         const uint32_t lanes = (uint32_t)(warp % 4) * 32;
+        // where a lane's scores of kRead columns go, from the first one: bytes below 2^32, since steps are below 2^26 elements
+        uint32_t at[MODE == ROWS ? kRead : 1];
+        if (MODE == ROWS) {
+#pragma unroll
+            for (int k = 0; k < kRead; k++) at[k] = (uint32_t)((lane + k * p.col_step) * sizeof(Out));
+        }
+        // ONE: the chunk's half of the group's part of `transit`, and neighbours that a store may take at once
+        const size_t pitch = p.col_step * sizeof(Out);
+        const uint32_t odd = (uint32_t)(reinterpret_cast<uintptr_t>(p.out) | pitch) % 16;
+        const int wide = odd % (4 * sizeof(Out)) == 0 ? 4 : odd % (2 * sizeof(Out)) == 0 ? 2 : 1;
+        float* chunk = reinterpret_cast<float*>(transit) + group * 2 * kRead * kLanes;
+        bool turn = false;
         uint32_t step = 0;
         bool ok = true;
         for (uint32_t t = blockIdx.x; t < p.tiles; t += gridDim.x) {
             const uint32_t l = lane_of(t) + lanes, c0 = col_of(t) + group * kGroup;      // the warp's first lane and column
-            Out* const out = static_cast<Out*>(p.out) + l * p.lane_step + c0 * p.col_step;
+            uint8_t* const out = static_cast<uint8_t*>(p.out) + (l * p.lane_step + c0 * p.col_step) * sizeof(Out);
             const int rows = l < p.lane.rows ? (int)min(p.lane.rows - l, 32u) : 0, cols = c0 < p.col.rows ? (int)min(p.col.rows - c0, (uint32_t)kGroup) : 0;
             uint64_t sum[MODE == ONE ? 1 : kGroup / 2] = {};    // two columns each
             for (uint32_t c = 0; c < p.blocks; c++, step++) {
@@ -276,39 +321,66 @@ __global__ void __launch_bounds__(Shape<CN, MODE>::threads, 1) product_kernel(co
                 const uint32_t from = tmem + (lanes << 16) + b * CN + group * kGroup;
                 ok = __all_sync(0xffffffffu, ok && barrier_wait(scaled + q, step / kScaleSteps & 1) && barrier_wait(ready + b, step / kBuffers & 1));
                 fence_after();
-                uint32_t part[2][kRead];
-                read_columns<kRead>(from, part[0]);
                 float lane_scale = scale[S::step_scales - kLanes + lanes + lane];
                 if (MODE == SQUARE) lane_scale *= scale[group];
                 if (!ok) lane_scale = __int_as_float(0x7fffffff);
                 const uint64_t lane_scales = pair_of(lane_scale, lane_scale);
-                Out* to = out + lane;                           // ONE
+                const auto release = [&]() {                    // the accumulator has been read
+                    fence_before();
+                    __syncwarp();
+                    if (lane == 0) barrier_arrive(spare + b);
+                };
+                if constexpr (MODE == ONE) {
+                    constexpr int kRows = kRead / 4;            // of a chunk, for each of the four warps
+                    const int items = (int)min(p.lane.rows - (l - lanes), (uint32_t)kLanes), row0 = warp % 4 * kRows;
+                    uint8_t* row = out - lanes * sizeof(Out) + row0 * pitch;
+                    const float* of_rows = scale + group * kGroup + row0;
+                    uint32_t part[kRead];
+                    read_columns<kRead>(from, part);
+#pragma unroll 1
+                    for (int left = cols - row0, k0 = 0; k0 < kGroup; k0 += kRead, left -= kRead, row += kRead * pitch, of_rows += kRead) {
+                        float* const to = chunk + lanes + lane;
+                        wait_columns<kRead>(part);
 #pragma unroll
-                for (int k0 = 0; k0 < kGroup; k0 += kRead) {
-                    uint32_t (&now)[kRead] = part[k0 / kRead & 1];
-                    wait_columns<kRead>(now);
-                    if (k0 + kRead < kGroup) read_columns<kRead>(from + k0 + kRead, part[(k0 / kRead + 1) & 1]);
-                    else {
-                        fence_before();
-                        __syncwarp();
-                        if (lane == 0) barrier_arrive(spare + b);
-                    }
-#pragma unroll
-                    for (int k = 0; k < kRead; k += 4) {
-                        const uint64_t x[2] = {pair_of(now[k], now[k + 1]), pair_of(now[k + 2], now[k + 3])};
-                        if constexpr (MODE == SQUARE) {
-                            sum[(k0 + k) / 2] = fma2(x[0], lane_scales, sum[(k0 + k) / 2]);
-                            sum[(k0 + k) / 2 + 1] = fma2(x[1], lane_scales, sum[(k0 + k) / 2 + 1]);
+                        for (int k = 0; k < kRead; k += 2) {
+                            const uint64_t x = mul2(pair_of(part[k], part[k + 1]), lane_scales);
+                            to[k * kLanes] = half_of(x, 0);
+                            to[(k + 1) * kLanes] = half_of(x, 1);
+                        }
+                        if (k0 + kRead < kGroup) read_columns<kRead>(from + k0 + kRead, part);
+                        else release();
+                        asm volatile("bar.sync %0, 128;" ::"r"(1 + group) : "memory");     // one a chunk: its half of `transit` is written again two chunks on
+                        const float* const rows_at = chunk + row0 * kLanes;
+                        if (items == kLanes && left >= kRows) {
+                            if (wide == 4) store_whole<Out, kRows, 4>(row, pitch, rows_at, of_rows, lane);
+                            else if (sizeof(Out) == 2 && wide == 2) store_whole<Out, kRows, 2>(row, pitch, rows_at, of_rows, lane);
+                            else store_whole<Out, kRows, 1>(row, pitch, rows_at, of_rows, lane);
                         } else {
-                            const ulonglong2 s = *reinterpret_cast<const ulonglong2*>(scale + group * kGroup + k0 + k);
-                            if constexpr (MODE == ROWS) {
+                            for (int r = 0; r < min(kRows, left); r++)
+                                for (int i = lane; i < items; i += 32) reinterpret_cast<Out*>(row + r * pitch)[i] = from_float<Out>(rows_at[r * kLanes + i] * of_rows[r]);
+                        }
+                        chunk = turn ? chunk - kRead * kLanes : chunk + kRead * kLanes;
+                        turn = !turn;
+                    }
+                } else {
+                    uint32_t part[2][kRead];
+                    read_columns<kRead>(from, part[0]);
+#pragma unroll
+                    for (int k0 = 0; k0 < kGroup; k0 += kRead) {
+                        uint32_t (&now)[kRead] = part[k0 / kRead & 1];
+                        wait_columns<kRead>(now);
+                        if (k0 + kRead < kGroup) read_columns<kRead>(from + k0 + kRead, part[(k0 / kRead + 1) & 1]);
+                        else release();
+#pragma unroll
+                        for (int k = 0; k < kRead; k += 4) {
+                            const uint64_t x[2] = {pair_of(now[k], now[k + 1]), pair_of(now[k + 2], now[k + 3])};
+                            if constexpr (MODE == SQUARE) {
+                                sum[(k0 + k) / 2] = fma2(x[0], lane_scales, sum[(k0 + k) / 2]);
+                                sum[(k0 + k) / 2 + 1] = fma2(x[1], lane_scales, sum[(k0 + k) / 2 + 1]);
+                            } else {
+                                const ulonglong2 s = *reinterpret_cast<const ulonglong2*>(scale + group * kGroup + k0 + k);
                                 sum[(k0 + k) / 2] = fma2(mul2(x[0], lane_scales), s.x, sum[(k0 + k) / 2]);
                                 sum[(k0 + k) / 2 + 1] = fma2(mul2(x[1], lane_scales), s.y, sum[(k0 + k) / 2 + 1]);
-                            } else {
-                                const uint64_t y[2] = {mul2(mul2(x[0], lane_scales), s.x), mul2(mul2(x[1], lane_scales), s.y)};
-#pragma unroll
-                                for (int i = 0; i < 4; i++, to += p.col_step)
-                                    if (lane < rows && k0 + k + i < cols) *to = from_float<Out>(half_of(y[i / 2], i & 1));
                             }
                         }
                     }
@@ -317,14 +389,13 @@ __global__ void __launch_bounds__(Shape<CN, MODE>::threads, 1) product_kernel(co
                 if (lane == 0) barrier_arrive(used + q);
             }
             if constexpr (MODE == ROWS) {
-                if (lane < rows) {
-                    Out* to = out + lane;
 #pragma unroll
-                    for (int k = 0; k < kGroup; k++, to += p.col_step)
-                        if (k < cols) *to = from_float<Out>(half_of(sum[k / 2], k & 1));
+                for (int k = 0; k < kGroup; k += 4) {
+                    const uint64_t y[2] = {sum[k / 2], sum[k / 2 + 1]};
+                    store_columns<Out, 4>(out + k / kRead * kRead * p.col_step * sizeof(Out), at + k % kRead, y, lane < rows, cols - k);
                 }
             }
-            if constexpr (MODE == SQUARE) store_rows<Out, kGroup>(sum, transit + warp * 32 * kStagePitch, out, p.lane_step, rows, cols, lane);
+            if constexpr (MODE == SQUARE) store_rows<Out, kGroup>(sum, transit + warp * 32 * kStagePitch, reinterpret_cast<Out*>(out), p.lane_step, rows, cols, lane);
         }
         if (!ok && lane == 0 && p.flags) atomicOr(p.flags, (uint32_t)MASCOT_FLAG_GAVE_UP);
         fence_before();
@@ -417,7 +488,7 @@ extern "C" int mascot_rows_product(const mascot_rows* a, const float* a_scale, c
     if (b_block_rows != 1 && b_block_rows != kScaleBlock) return fail(nullptr, MASCOT_ERR_BAD_ARG, "b_block_rows must be 1 or 128");
     if (is_empty(*a) || is_empty(*b)) return MASCOT_OK;
     if (out->type > MASCOT_BF16) return fail(nullptr, MASCOT_ERR_BAD_ARG, "out: must be MASCOT_F32, MASCOT_F16 or MASCOT_BF16");
-    if (out->stride < out->width || out->stride > (1ull << 31)) return fail(nullptr, MASCOT_ERR_BAD_ARG, "out: stride must be from the width to 2^31");
+    if (out->stride < out->width || out->stride >= (1ull << 26)) return fail(nullptr, MASCOT_ERR_BAD_ARG, "out: stride must be from the width to 2^26");
     if (!out->data || !a_scale || !b_scale) return fail(nullptr, MASCOT_ERR_BAD_ARG, "null pointer");
     if (reinterpret_cast<uintptr_t>(out->data) % type_bytes(out->type) || reinterpret_cast<uintptr_t>(a_scale) % 4 || reinterpret_cast<uintptr_t>(b_scale) % 4)
         return fail(nullptr, MASCOT_ERR_BAD_ARG, "an address is not a multiple of the element's size");
@@ -443,7 +514,7 @@ extern "C" int mascot_rows_product(const mascot_rows* a, const float* a_scale, c
     p.out = out->data; p.lane_step = 1; p.col_step = out->stride;
     p.blocks = col_blocks;
     p.flags = flags;
-    const cudaError_t e = with_type(out->type, [&](auto* o) { return launch_tiles<std::remove_pointer_t<decltype(o)>>(*a, *b, p, static_cast<cudaStream_t>(stream)); });
-    CU(nullptr, e);
+    const cudaError_t launched = with_type(out->type, [&](auto* o) { return launch_tiles<std::remove_pointer_t<decltype(o)>>(*a, *b, p, static_cast<cudaStream_t>(stream)); });
+    CU(nullptr, launched);
     return MASCOT_OK;
 }

@@ -461,7 +461,7 @@ def test_product_widths(mascot, width, block_rows, dst):
     check_product(mascot, 3, 260, width, block_rows, dst)
 
 
-@pytest.mark.parametrize("m,n,width", [(1, 100_003, 128), (1000, 20_011, 64), (4096, 5000, 128), (513, 2049, 1024)])
+@pytest.mark.parametrize("m,n,width", [(1, 100_003, 128), (20, 20_001, 128), (50, 20_001, 300), (100, 20_001, 64), (120, 20_001, 520), (1000, 20_011, 64), (4096, 5000, 128), (513, 2049, 1024), (900, 12_345, 384)])
 def test_product_of_many_tiles(mascot, m, n, width):
     check_product(mascot, m, n, width, 1, torch.float32)
     check_product(mascot, m, n, width, 128, torch.float16, any_scale=False)
