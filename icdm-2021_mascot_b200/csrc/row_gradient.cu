@@ -13,18 +13,20 @@
 //            goes on in the next chunk or comes from the one before, the chunk's part is left in the workspace.
 //   combine  adds these parts up in the order of the chunks, and clears rows that no entry names.
 #include <algorithm>
+#include <initializer_list>
 
+#include "launch_cache.h"
 #include "row_ops.h"
 
 namespace mascot {
 namespace {
 
-constexpr int kSortBlock = 256, kSortItems = 16, kTile = kSortBlock * kSortItems;     // entries of a block of the sort
+constexpr int kSortBlock = 512, kSortItems = 16, kTile = kSortBlock * kSortItems, kSortWarps = kSortBlock / 32;     // entries of a block of the sort
 constexpr int kMaxDigitBits = 10, kMaxBins = 1 << kMaxDigitBits;
 constexpr int kScanTiles = 32;                  // up to so many tiles the scatter kernel adds their counts up itself
-constexpr int kSmallBlock = 1024, kSmallItems = 12;
+constexpr int kSmallBlock = 1024, kSmallItems = 12, kSmallWarps = kSmallBlock / 32;
 constexpr uint32_t kSmall = kSmallBlock * kSmallItems;
-constexpr int kSmallDigitBits = 8;
+constexpr int kSmallDigitBits = 8, kSmallBins = 1 << kSmallDigitBits;
 constexpr int kReduceBlock = 256, kCombineBlock = 1024;
 constexpr uint32_t kLongSpan = 64;              // chunks of one row that a warp still adds up alone
 
@@ -48,7 +50,9 @@ struct Job {
 };
 
 struct Space {                                  // the workspace, see carve()
-    uint32_t *key[2], *val[2], *counts, *totals;
+    uint32_t *key, *counts, *totals;            // rows of the entries as they come; [tiles][bins]; [bins]
+    uint2* entry[2];                            // (row, entry)
+    uint4* pair;                                // user, preferred, other, bits of coef
     float *head, *tail;                         // [chunks][pitch]
     uint8_t* touched;                           // a byte per row
     uint32_t pitch, chunks, tiles;
@@ -56,14 +60,15 @@ struct Space {                                  // the workspace, see carve()
 
 // ---- sort --------------------------------------------------------------------------------------------------
 
-// Row of entry e, or `total`.
-__device__ __forceinline__ uint32_t entry_key(const Job& j, uint32_t e, bool& bad) {
+// Row of entry e, or `total`.  Pairs: the entry of the user also leaves the pair's rows where the sums find them.
+__device__ __forceinline__ uint32_t entry_key(const Job& j, const Space& s, uint32_t e, bool& bad) {
     if (j.kinds == 1) {
         const uint32_t r = row_of(j.ids[0], e, j.rows[0], bad);
         return r == kNoRow ? j.total : r;
     }
-    const uint32_t kind = e / j.per, b = e - kind * j.per;
+    const uint32_t kind = e >= 2 * j.per ? 2 : e >= j.per ? 1 : 0, b = e - kind * j.per;
     const uint32_t u = row_of(j.ids[0], b, j.rows[0], bad), p = row_of(j.ids[1], b, j.rows[1], bad), o = row_of(j.ids[2], b, j.rows[1], bad);
+    if (kind == 0) s.pair[b] = make_uint4(u, p, o, __float_as_uint(__ldg(j.coef + b)));
     if (u == kNoRow || p == kNoRow || o == kNoRow) return j.total;
     return kind == 0 ? u : j.rows[0] + (kind == 1 ? p : o);
 }
@@ -74,10 +79,14 @@ __device__ __forceinline__ void clear_touched(uint8_t* touched, uint32_t rows, s
 
 // Stable ranks of a warp's keys among the keys with the same digit that the warp has met so far; `count` is the
 // warp's own row of counters, zero at first.
-__device__ __forceinline__ uint32_t warp_rank(uint32_t digit, bool there, uint16_t* count, uint32_t lane) {
-    const uint32_t peers = __match_any_sync(0xffffffffu, there ? digit : 0xffffffffu);
-    uint32_t before = 0;
+__device__ __forceinline__ uint32_t warp_rank(uint32_t digit, bool there, int bits, uint16_t* count, uint32_t lane) {
+    uint32_t peers = __ballot_sync(0xffffffffu, there);
+    for (int b = 0; b < bits; b++) {
+        const uint32_t set = __ballot_sync(0xffffffffu, digit >> b & 1);
+        peers &= digit >> b & 1 ? set : ~set;
+    }
     const uint32_t below = __popc(peers & ((1u << lane) - 1u));
+    uint32_t before = 0;
     if (there) before = count[digit];
     __syncwarp();
     if (there && below == 0) count[digit] = (uint16_t)(before + __popc(peers));
@@ -85,12 +94,24 @@ __device__ __forceinline__ uint32_t warp_rank(uint32_t digit, bool there, uint16
     return before + below;
 }
 
-// Exclusive scan over `bins` values in shared memory by a whole block, in place; bins at most 4 * blockDim.x.
+// Counters of `warps` warps, [warp][bins], become offsets of the warps within a bin, for two bins (2 b, 2 b + 1) at once; their sums come back.
+__device__ __forceinline__ uint32_t warp_offsets(uint16_t* count, int warps, int bins, int b) {
+    uint32_t sum = 0;                                           // two halves that never carry: at most 12288 entries
+    for (int w = 0; w < warps; w++) {
+        uint32_t* const c = reinterpret_cast<uint32_t*>(count + w * bins) + b;
+        const uint32_t x = *c;
+        *c = sum;
+        sum += x;
+    }
+    return sum;
+}
+
+// Exclusive scan over `bins` values in shared memory by a whole block, in place; bins at most 2 * blockDim.x.
 __device__ __forceinline__ void block_scan(uint32_t* v, int bins, uint32_t* warp_sums) {
     const int t = threadIdx.x, lane = t & 31, warp = t >> 5, warps = blockDim.x >> 5;
-    uint32_t x[4], sum = 0;
+    uint32_t x[2], sum = 0;
 #pragma unroll
-    for (int k = 0; k < 4; k++) { const int b = 4 * t + k; x[k] = b < bins ? v[b] : 0u; sum += x[k]; }
+    for (int k = 0; k < 2; k++) { const int b = 2 * t + k; x[k] = b < bins ? v[b] : 0u; sum += x[k]; }
     uint32_t inc = sum;
 #pragma unroll
     for (int d = 1; d < 32; d <<= 1) { const uint32_t y = __shfl_up_sync(0xffffffffu, inc, d); if (lane >= d) inc += y; }
@@ -106,155 +127,165 @@ __device__ __forceinline__ void block_scan(uint32_t* v, int bins, uint32_t* warp
     __syncthreads();
     uint32_t run = warp_sums[warp] + inc - sum;
 #pragma unroll
-    for (int k = 0; k < 4; k++) { const int b = 4 * t + k; if (b < bins) v[b] = run; run += x[k]; }
+    for (int k = 0; k < 2; k++) { const int b = 2 * t + k; if (b < bins) v[b] = run; run += x[k]; }
     __syncthreads();
 }
 
-// One block, everything in shared memory: keys and values twice, counters of 32 warps.  What bounds it is the latency of a
-// pass (about 1.5 us of ranking); a sort over many blocks costs three launches a digit.
+constexpr size_t kSmallSmem = 8 * (size_t)kSmall + 2 * (size_t)kSmallWarps * kSmallBins + 4 * kSmallBins + 4 * 32;
+
+// One block: entries stay in registers while they are ranked and go through shared memory to their next place.  A sort over
+// many blocks costs two launches a digit at least.
 __global__ void __launch_bounds__(kSmallBlock) small_sort_kernel(const Job j, const Space s, int passes, int bits) {
-    extern __shared__ uint32_t mem[];
-    uint32_t* key[2] = {mem, mem + kSmall};
-    uint32_t* val[2] = {mem + 2 * kSmall, mem + 3 * kSmall};
-    uint16_t* const count = reinterpret_cast<uint16_t*>(mem + 4 * kSmall);
-    uint32_t* const bins_at = mem + 4 * kSmall + 32 * (1 << kSmallDigitBits) / 2;
-    uint32_t* const warp_sums = bins_at + (1 << kSmallDigitBits);
+    extern __shared__ uint2 at[];
+    uint16_t* const count = reinterpret_cast<uint16_t*>(at + kSmall);
+    uint32_t* const start = reinterpret_cast<uint32_t*>(count + kSmallWarps * kSmallBins), *const warp_sums = start + kSmallBins;
     const int t = threadIdx.x, lane = t & 31, warp = t >> 5, bins = 1 << bits;
     if (!j.accumulate) clear_touched(s.touched, j.total, t, kSmallBlock);
+    const uint32_t rounds = (j.n + kSmallBlock - 1) / kSmallBlock, first = warp * rounds * 32 + lane;      // a warp's entries, in order
     bool bad = false;
-    for (uint32_t e = t; e < j.n; e += kSmallBlock) { key[0][e] = entry_key(j, e, bad); val[0][e] = e; }
+    uint2 e[kSmallItems];
+#pragma unroll
+    for (int k = 0; k < kSmallItems; k++) {
+        const uint32_t i = first + k * 32;
+        e[k] = make_uint2(0, i);
+        if (k < rounds && i < j.n) e[k].x = entry_key(j, s, i, bad);
+    }
     if (bad && j.flags) atomicOr(j.flags, (uint32_t)MASCOT_FLAG_BAD_ID);
-    const uint32_t per_warp = ((j.n + 1023) / 1024) * 32, first = warp * per_warp;       // a warp's entries, in order
     uint16_t* const mine = count + (warp << bits);
-    int from = 0;
-    for (int p = 0; p < passes; p++, from ^= 1) {
-        for (int b = lane; b < bins; b += 32) mine[b] = 0;
-        __syncthreads();
+    for (int p = 0; p < passes; p++) {
+        for (int b = lane; b < bins / 2; b += 32) reinterpret_cast<uint32_t*>(mine)[b] = 0;
+        __syncwarp();
         uint32_t rank[kSmallItems];
 #pragma unroll
-        for (int k = 0; k < kSmallItems; k++) {
-            if (k * 32u >= per_warp) break;
-            const uint32_t e = first + k * 32 + lane;
-            const bool there = e < j.n;
-            const uint32_t d = there ? key[from][e] >> (p * bits) & (bins - 1) : 0u;
-            rank[k] = warp_rank(d, there, mine, lane);
+        for (int k = 0; k < kSmallItems; k++)
+            if (k < rounds) rank[k] = warp_rank(e[k].x >> (p * bits) & (bins - 1), first + k * 32 < j.n, bits, mine, lane);
+        __syncthreads();
+        for (int b = t; b < bins / 2; b += kSmallBlock) {
+            const uint32_t sums = warp_offsets(count, kSmallWarps, bins, b);
+            start[2 * b] = sums & 0xffff;
+            start[2 * b + 1] = sums >> 16;
         }
         __syncthreads();
-        for (int b = t; b < bins; b += kSmallBlock) {           // counters become offsets of the warps within a bin
-            uint32_t sum = 0;
-            for (int w = 0; w < 32; w++) { uint16_t* const c = count + (w << bits) + b; const uint32_t x = *c; *c = (uint16_t)sum; sum += x; }
-            bins_at[b] = sum;
-        }
-        __syncthreads();
-        block_scan(bins_at, bins, warp_sums);
+        block_scan(start, bins, warp_sums);
 #pragma unroll
-        for (int k = 0; k < kSmallItems; k++) {
-            if (k * 32u >= per_warp) break;
-            const uint32_t e = first + k * 32 + lane;
-            if (e < j.n) {
-                const uint32_t x = key[from][e], d = x >> (p * bits) & (bins - 1), at = bins_at[d] + mine[d] + rank[k];
-                key[from ^ 1][at] = x;
-                val[from ^ 1][at] = val[from][e];
-            }
-        }
+        for (int k = 0; k < kSmallItems; k++)
+            if (k < rounds && first + k * 32 < j.n) { const uint32_t d = e[k].x >> (p * bits) & (bins - 1); at[start[d] + mine[d] + rank[k]] = e[k]; }
         __syncthreads();
+        if (p + 1 < passes) {
+#pragma unroll
+            for (int k = 0; k < kSmallItems; k++) if (k < rounds && first + k * 32 < j.n) e[k] = at[first + k * 32];
+            // `at` is written again only behind the next pass's barriers
+        }
     }
-    for (uint32_t e = t; e < j.n; e += kSmallBlock) { s.key[0][e] = key[from][e]; s.val[0][e] = val[from][e]; }
+    for (uint32_t i = t; i < j.n; i += kSmallBlock) s.entry[0][i] = at[i];
 }
 
-// Counts of the digits of a tile, [bin][tile].  The first pass makes the keys, and keeps them.
+// Counts of the digits of a tile, [tile][bin].  The first pass makes the keys, and keeps them.
 template <bool FIRST>
 __global__ void __launch_bounds__(kSortBlock) count_kernel(const Job j, const Space s, int from, int shift, int bits) {
     __shared__ uint32_t hist[kMaxBins];
     const int bins = 1 << bits;
     for (int b = threadIdx.x; b < bins; b += kSortBlock) hist[b] = 0;
     if (FIRST && !j.accumulate) clear_touched(s.touched, j.total, (size_t)blockIdx.x * kSortBlock + threadIdx.x, (size_t)gridDim.x * kSortBlock);
-    __syncthreads();
     bool bad = false;
-#pragma unroll 4
+    uint32_t key[kSortItems];
+#pragma unroll
     for (int k = 0; k < kSortItems; k++) {
         const uint32_t e = blockIdx.x * kTile + k * kSortBlock + threadIdx.x;
-        if (e >= j.n) break;
-        uint32_t key;
-        if (FIRST) { key = entry_key(j, e, bad); s.key[0][e] = key; }
-        else key = s.key[from][e];
-        atomicAdd(&hist[key >> shift & (bins - 1)], 1u);
+        if (e < j.n) key[k] = FIRST ? entry_key(j, s, e, bad) : s.entry[from][e].x;
     }
     if (FIRST && bad && j.flags) atomicOr(j.flags, (uint32_t)MASCOT_FLAG_BAD_ID);
     __syncthreads();
-    for (int b = threadIdx.x; b < bins; b += kSortBlock) s.counts[(size_t)b * s.tiles + blockIdx.x] = hist[b];
-}
-
-// A warp per bin: counts of the tiles become offsets within the bin, the sums go to totals.
-__global__ void __launch_bounds__(256) scan_kernel(const Space s, int bins) {
-    const int bin = (blockIdx.x * 256 + threadIdx.x) >> 5, lane = threadIdx.x & 31;
-    if (bin >= bins) return;
-    uint32_t* const c = s.counts + (size_t)bin * s.tiles;
-    uint32_t run = 0;
-    for (uint32_t t0 = 0; t0 < s.tiles; t0 += 128) {
-        uint32_t x[4], sum = 0;
 #pragma unroll
-        for (int k = 0; k < 4; k++) { const uint32_t t = t0 + 4 * lane + k; x[k] = t < s.tiles ? c[t] : 0u; sum += x[k]; }
-        uint32_t inc = sum;
-#pragma unroll
-        for (int d = 1; d < 32; d <<= 1) { const uint32_t y = __shfl_up_sync(0xffffffffu, inc, d); if (lane >= d) inc += y; }
-        uint32_t at = run + inc - sum;
-#pragma unroll
-        for (int k = 0; k < 4; k++) { const uint32_t t = t0 + 4 * lane + k; if (t < s.tiles) c[t] = at; at += x[k]; }
-        run += __shfl_sync(0xffffffffu, inc, 31);
+    for (int k = 0; k < kSortItems; k++) {
+        const uint32_t e = blockIdx.x * kTile + k * kSortBlock + threadIdx.x;
+        if (e < j.n) {
+            if (FIRST) s.key[e] = key[k];
+            atomicAdd(&hist[key[k] >> shift & (bins - 1)], 1u);
+        }
     }
-    if (lane == 0) s.totals[bin] = run;
+    __syncthreads();
+    for (int b = threadIdx.x; b < bins; b += kSortBlock) s.counts[(size_t)blockIdx.x * bins + b] = hist[b];
 }
 
-// Moves a tile's entries to their places.  Ranks within a warp by matching digits, in the order of the entries; warps and tiles by
-// their counts.
+// A block for 32 bins, a warp for a run of tiles: counts of the tiles become offsets within the bin, the sums go to totals.
+__global__ void __launch_bounds__(1024) scan_kernel(const Space s, int bins) {
+    __shared__ uint32_t sums[32][32];
+    const uint32_t lane = threadIdx.x & 31, warp = threadIdx.x >> 5, bin = blockIdx.x * 32 + lane;
+    const uint32_t per = (s.tiles + 31) / 32, t0 = min(s.tiles, warp * per), t1 = min(s.tiles, t0 + per);
+    uint32_t sum = 0;
+    if (bin < bins) {
+#pragma unroll 8
+        for (uint32_t t = t0; t < t1; t++) sum += s.counts[(size_t)t * bins + bin];
+    }
+    sums[warp][lane] = sum;
+    __syncthreads();
+    uint32_t run = 0;
+    for (uint32_t w = 0; w < 32; w++) { const uint32_t x = sums[w][lane]; if (w < warp) run += x; else if (w == 31) break; }
+    if (bin >= bins) return;
+#pragma unroll 8
+    for (uint32_t t = t0; t < t1; t++) {
+        const uint32_t x = s.counts[(size_t)t * bins + bin];
+        s.counts[(size_t)t * bins + bin] = run;
+        run += x;
+    }
+    if (warp == 31) s.totals[bin] = run;
+}
+
+// Moves a tile's entries to their places: ranked by warps in the order of the entries, put in order in shared memory, and written from
+// there, so that the entries of a bin leave as one run.
 template <bool FIRST>
 __global__ void __launch_bounds__(kSortBlock) scatter_kernel(const Job j, const Space s, int from, int shift, int bits, bool scanned) {
-    extern __shared__ uint32_t mem[];                           // offsets of the bins, then the warps' counters
-    __shared__ uint32_t warp_sums[kSortBlock / 32];
+    extern __shared__ uint2 at[];                               // entries in their order; the warps' counters; the bins' offsets
+    __shared__ uint32_t warp_sums[32];
     const int t = threadIdx.x, lane = t & 31, warp = t >> 5, bins = 1 << bits;
-    uint32_t* const base = mem;
-    uint16_t* const count = reinterpret_cast<uint16_t*>(mem + bins), *const mine = count + (warp << bits);
-    for (int b = t; b < bins * (kSortBlock / 32) / 2; b += kSortBlock) reinterpret_cast<uint32_t*>(count)[b] = 0;
+    uint16_t* const count = reinterpret_cast<uint16_t*>(at + kTile), *const mine = count + (warp << bits);
+    uint32_t* const start = reinterpret_cast<uint32_t*>(count + (kSortWarps << bits)), *const base = start + bins;
+    for (int b = lane; b < bins / 2; b += 32) reinterpret_cast<uint32_t*>(mine)[b] = 0;
+    const uint32_t first = blockIdx.x * kTile + warp * (32 * kSortItems) + lane;
+    uint2 e[kSortItems];
+#pragma unroll
+    for (int k = 0; k < kSortItems; k++) {
+        const uint32_t i = first + k * 32;
+        e[k] = make_uint2(0, i);
+        if (i < j.n) { if (FIRST) e[k].x = s.key[i]; else e[k] = s.entry[from][i]; }
+    }
     uint32_t within[kMaxBins / kSortBlock];                     // entries of the bin in the tiles before
 #pragma unroll
     for (int k = 0; k < kMaxBins / kSortBlock; k++) {
         const int b = t + k * kSortBlock;
         within[k] = 0;
         if (b < bins) {
-            const uint32_t* const c = s.counts + (size_t)b * s.tiles;
             uint32_t sum = 0;
-            if (scanned) { within[k] = c[blockIdx.x]; sum = s.totals[b]; }
-            else for (uint32_t q = 0; q < s.tiles; q++) { if (q == blockIdx.x) within[k] = sum; sum += c[q]; }
+            if (scanned) { within[k] = s.counts[(size_t)blockIdx.x * bins + b]; sum = s.totals[b]; }
+            else {
+#pragma unroll 8
+                for (uint32_t q = 0; q < s.tiles; q++) { if (q == blockIdx.x) within[k] = sum; sum += s.counts[(size_t)q * bins + b]; }
+            }
             base[b] = sum;
         }
     }
+    __syncwarp();
+    uint32_t rank[kSortItems];
+#pragma unroll
+    for (int k = 0; k < kSortItems; k++) rank[k] = warp_rank(e[k].x >> shift & (bins - 1), first + k * 32 < j.n, bits, mine, lane);
     __syncthreads();
+    for (int b = t; b < bins / 2; b += kSortBlock) {
+        const uint32_t sums = warp_offsets(count, kSortWarps, bins, b);
+        start[2 * b] = sums & 0xffff;
+        start[2 * b + 1] = sums >> 16;
+    }
     block_scan(base, bins, warp_sums);
+    block_scan(start, bins, warp_sums);
 #pragma unroll
-    for (int k = 0; k < kMaxBins / kSortBlock; k++) { const int b = t + k * kSortBlock; if (b < bins) base[b] += within[k]; }
-    const uint32_t first = blockIdx.x * kTile + warp * (32 * kSortItems);
-    uint32_t key[kSortItems], rank[kSortItems];
+    for (int k = 0; k < kMaxBins / kSortBlock; k++) { const int b = t + k * kSortBlock; if (b < bins) base[b] += within[k] - start[b]; }
 #pragma unroll
-    for (int k = 0; k < kSortItems; k++) { const uint32_t e = first + k * 32 + lane; key[k] = e < j.n ? s.key[from][e] : 0u; }
-#pragma unroll
-    for (int k = 0; k < kSortItems; k++) rank[k] = warp_rank(key[k] >> shift & (bins - 1), first + k * 32 + lane < j.n, mine, lane);
+    for (int k = 0; k < kSortItems; k++)
+        if (first + k * 32 < j.n) { const uint32_t d = e[k].x >> shift & (bins - 1); at[start[d] + mine[d] + rank[k]] = e[k]; }
     __syncthreads();
-    for (int b = t; b < bins; b += kSortBlock) {
-        uint32_t sum = 0;
-#pragma unroll
-        for (int w = 0; w < kSortBlock / 32; w++) { uint16_t* const c = count + (w << bits) + b; const uint32_t x = *c; *c = (uint16_t)sum; sum += x; }
-    }
-    __syncthreads();
-#pragma unroll
-    for (int k = 0; k < kSortItems; k++) {
-        const uint32_t e = first + k * 32 + lane;
-        if (e < j.n) {
-            const uint32_t d = key[k] >> shift & (bins - 1), at = base[d] + mine[d] + rank[k];
-            s.key[from ^ 1][at] = key[k];
-            s.val[from ^ 1][at] = FIRST ? e : s.val[from][e];
-        }
-    }
+    const uint32_t here = min((uint32_t)kTile, j.n - blockIdx.x * kTile);
+#pragma unroll 4
+    for (uint32_t i = t; i < here; i += kSortBlock) { const uint2 x = at[i]; s.entry[from ^ 1][i + base[x.x >> shift & (bins - 1)]] = x; }
 }
 
 // ---- sums --------------------------------------------------------------------------------------------------
@@ -275,90 +306,86 @@ __device__ __forceinline__ void write_row(const Job& j, uint32_t row, uint32_t c
     store_piece<Out, N>(at, r);
 }
 
-// An entry's value: c * (row a - row b), without b where that is null, and plain where there is no coefficient.
-template <typename T> struct Value { const T *a, *b; float c; };
-template <typename T, bool PAIRS>
-__device__ __forceinline__ Value<T> value_of(const Job& j, uint32_t e, uint32_t col) {
-    Value<T> v{nullptr, nullptr, 1.f};
-    if (!PAIRS) { v.a = static_cast<const T*>(j.src[0]) + (size_t)e * j.src_stride[0] + col; return v; }
-    const uint32_t kind = e >= 2 * j.per ? 2 : e >= j.per ? 1 : 0, b = e - kind * j.per;
-    bool bad = false;
-    v.c = __ldg(j.coef + b);
-    if (kind == 0) {
-        const uint32_t p = row_of(j.ids[1], b, j.rows[1], bad), o = row_of(j.ids[2], b, j.rows[1], bad);
-        v.a = static_cast<const T*>(j.src[1]) + p * j.src_stride[1] + col;
-        v.b = static_cast<const T*>(j.src[1]) + o * j.src_stride[1] + col;
-    } else {
-        const uint32_t u = row_of(j.ids[0], b, j.rows[0], bad);
-        v.a = static_cast<const T*>(j.src[0]) + u * j.src_stride[0] + col;
-        if (kind == 2) v.c = -v.c;
-    }
-    if (v.c == 0.f) v.a = nullptr;                              // whatever the rows hold
-    return v;
-}
-
-constexpr int kBatch = 4;                       // entries whose rows a team has in flight
-
+// A team's lanes take a group of entries each, one round trip for all of them, and hand them round; the rows of BATCH
+// entries are in flight at once.  What bounds it is those rows: random ones, from HBM or L2.
 template <typename T, typename Out, int N, bool PAIRS>
-__global__ void __launch_bounds__(kReduceBlock) reduce_kernel(const Job j, const Space s, const uint32_t* key, const uint32_t* val, int team_log2) {
-    const uint32_t chunk = (blockIdx.x * kReduceBlock + threadIdx.x) >> team_log2, tl = threadIdx.x & ((1u << team_log2) - 1);
-    const uint32_t col = ((blockIdx.y << team_log2) + tl) * N;
-    if (chunk >= s.chunks || col >= j.width) return;
-    const uint32_t begin = chunk << j.chunk_log2, end = min(j.n, begin + (1u << j.chunk_log2));
-    const uint32_t before = begin ? __ldg(key + begin - 1) : kNoRow, after = end < j.n ? __ldg(key + end) : kNoRow;
-    uint32_t row = __ldg(key + begin);
+__global__ void __launch_bounds__(kReduceBlock) reduce_kernel(const Job j, const Space s, const uint2* entry, int team_log2) {
+    constexpr int BATCH = PAIRS ? 4 : 8;
+    const uint32_t team = 1u << team_log2, tl = threadIdx.x & (team - 1);
+    const uint32_t chunk = (blockIdx.x * kReduceBlock + threadIdx.x) >> team_log2, col = ((blockIdx.y << team_log2) + tl) * N;
+    const bool writes = chunk < s.chunks && col < j.width;
+    const uint32_t begin = min(j.n, chunk << j.chunk_log2), end = min(j.n, begin + (1u << j.chunk_log2));
+    const uint32_t before = chunk < s.chunks && begin ? __ldg(&entry[begin - 1].x) : kNoRow, after = end < j.n ? __ldg(&entry[end].x) : kNoRow;
+    const T* const src0 = static_cast<const T*>(j.src[0]) + col, *const src1 = static_cast<const T*>(j.src[1]) + col;
+    uint32_t row = kNoRow;
     float sum[N] = {};
-    const auto flush = [&](uint32_t r) {
-        if (r >= j.total) return;
-        if (r == before || r == after) {                       // part of a row that other chunks share
-            float* const part = (r == before ? s.head : s.tail) + (size_t)chunk * s.pitch + col;
+    const auto flush = [&]() {
+        if (row >= j.total || !writes) return;
+        if (row == before || row == after) {                   // part of a row that other chunks share
+            float* const part = (row == before ? s.head : s.tail) + (size_t)chunk * s.pitch + col;
 #pragma unroll
             for (int k = 0; k < N; k++) part[k] = sum[k];
-        } else write_row<Out, N>(j, r, col, sum);
-        if (r != before && !j.accumulate && col == 0) s.touched[r] = 1;
+        } else write_row<Out, N>(j, row, col, sum);
+        if (row != before && !j.accumulate && col == 0) s.touched[row] = 1;
     };
-    for (uint32_t e0 = begin; e0 < end && row < j.total; e0 += kBatch) {
-        const uint4 k4 = __ldg(reinterpret_cast<const uint4*>(key + e0)), v4 = __ldg(reinterpret_cast<const uint4*>(val + e0));
-        const uint32_t keys[kBatch] = {k4.x, k4.y, k4.z, k4.w}, vals[kBatch] = {v4.x, v4.y, v4.z, v4.w};
-        Value<T> v[kBatch];
-        Piece<T, N> a[kBatch], b[kBatch];
-#pragma unroll
-        for (int k = 0; k < kBatch; k++) {
-            v[k] = Value<T>{nullptr, nullptr, 0.f};
-            if (e0 + k < end && keys[k] < j.total) v[k] = value_of<T, PAIRS>(j, vals[k], col);
+    for (uint32_t g = begin; __any_sync(0xffffffffu, g < end); g += team) {
+        uint2 mine = make_uint2(j.total, 0);
+        if (g + tl < end) mine = __ldg(entry + g + tl);
+        uint32_t my_a = mine.y, my_b = kNoRow;
+        float my_c = 1.f;
+        if (PAIRS && mine.x < j.total) {
+            const uint32_t kind = mine.y >= 2 * j.per ? 2 : mine.y >= j.per ? 1 : 0;
+            const uint4 p = __ldg(s.pair + (mine.y - kind * j.per));
+            my_c = kind == 2 ? -__uint_as_float(p.w) : __uint_as_float(p.w);
+            my_a = kind ? p.x : p.y;
+            if (kind == 0) my_b = p.z;
         }
+        for (uint32_t k0 = 0; k0 < team; k0 += BATCH) {
+            if (!__any_sync(0xffffffffu, g + k0 < end)) break;
+            uint32_t key[BATCH], b_row[BATCH];
+            float c[BATCH];
+            Piece<T, N> a[BATCH], b[BATCH];
 #pragma unroll
-        for (int k = 0; k < kBatch; k++) {
-            if (v[k].a) a[k] = load_piece<T, N>(v[k].a);
-            if (PAIRS && v[k].b && v[k].a) b[k] = load_piece<T, N>(v[k].b);
-        }
-#pragma unroll
-        for (int k = 0; k < kBatch; k++) {
-            if (e0 + k >= end) break;
-            if (keys[k] != row) {
-                flush(row);
-                row = keys[k];
-#pragma unroll
-                for (int x = 0; x < N; x++) sum[x] = 0.f;
+            for (int k = 0; k < BATCH; k++) {
+                key[k] = __shfl_sync(0xffffffffu, mine.x, k0 + k, team);
+                const uint32_t a_row = __shfl_sync(0xffffffffu, my_a, k0 + k, team);
+                c[k] = PAIRS ? __shfl_sync(0xffffffffu, my_c, k0 + k, team) : 1.f;
+                b_row[k] = PAIRS ? __shfl_sync(0xffffffffu, my_b, k0 + k, team) : kNoRow;
+                if (key[k] >= j.total || !writes) c[k] = 0.f;   // coef 0: whatever the rows hold
+                if (c[k] != 0.f) {
+                    a[k] = load_piece<T, N>(!PAIRS || b_row[k] == kNoRow ? src0 + a_row * j.src_stride[0] : src1 + a_row * j.src_stride[1]);
+                    if (PAIRS && b_row[k] != kNoRow) b[k] = load_piece<T, N>(src1 + b_row[k] * j.src_stride[1]);
+                }
             }
-            if (v[k].a) {
 #pragma unroll
-                for (int x = 0; x < N; x++) {
-                    if (!PAIRS) sum[x] += as_float(a[k].v[x]);
-                    else sum[x] = fmaf(v[k].c, v[k].b ? as_float(a[k].v[x]) - as_float(b[k].v[x]) : as_float(a[k].v[x]), sum[x]);
+            for (int k = 0; k < BATCH; k++) {
+                if (key[k] != row) {
+                    flush();
+                    row = key[k];
+#pragma unroll
+                    for (int x = 0; x < N; x++) sum[x] = 0.f;
+                }
+                if (c[k] != 0.f) {
+#pragma unroll
+                    for (int x = 0; x < N; x++) {
+                        if (!PAIRS) sum[x] += as_float(a[k].v[x]);
+                        else sum[x] = fmaf(c[k], b_row[k] != kNoRow ? as_float(a[k].v[x]) - as_float(b[k].v[x]) : as_float(a[k].v[x]), sum[x]);
+                    }
                 }
             }
         }
     }
-    flush(row);
+    flush();
 }
 
-// The first position behind the entries of `row`, searched from `at`, which is one of them.
-__device__ __forceinline__ uint32_t row_end(const uint32_t* key, uint32_t at, uint32_t n, uint32_t row) {
-    uint32_t lo = at, hi = n;                                   // key[lo] == row, key[hi] > row
+// The first position behind the entries of `row`, searched by a warp from `at`, which is one of them: 32 places at a time.
+__device__ __forceinline__ uint32_t row_end(const uint2* entry, uint32_t at, uint32_t n, uint32_t row, uint32_t lane) {
+    uint32_t lo = at, hi = n;                                   // the entry at lo is one, that at hi is none
     while (hi - lo > 1) {
-        const uint32_t mid = lo + (hi - lo) / 2;
-        if (__ldg(key + mid) == row) lo = mid; else hi = mid;
+        const uint32_t step = (hi - lo + 31) / 32, mid = lo + lane * step;      // lane 0: lo
+        const uint32_t in = __popc(__ballot_sync(0xffffffffu, mid < hi && __ldg(&entry[mid].x) == row));      // the first `in` places
+        hi = min(hi, lo + in * step);
+        lo += (in - 1) * step;
     }
     return hi;
 }
@@ -367,7 +394,7 @@ __device__ __forceinline__ uint32_t row_end(const uint32_t* key, uint32_t at, ui
 // more than kLongSpan chunks is added up by all warps of the block, a slice each: only one row a block can be that long, since it
 // covers all chunks of the block behind its first.  The other blocks clear the rows that no entry names, a warp for 32 of them.
 template <typename Out, int N>
-__global__ void __launch_bounds__(kCombineBlock) combine_kernel(const Job j, const Space s, const uint32_t* key, uint32_t combine_blocks) {
+__global__ void __launch_bounds__(kCombineBlock) combine_kernel(const Job j, const Space s, const uint2* entry, uint32_t combine_blocks) {
     const uint32_t lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     if (blockIdx.x >= combine_blocks) {
         const uint32_t row0 = (blockIdx.x - combine_blocks) * kCombineBlock + warp * 32;
@@ -396,9 +423,14 @@ __global__ void __launch_bounds__(kCombineBlock) combine_kernel(const Job j, con
     if (chunk < s.chunks) {
         const uint32_t begin = chunk << j.chunk_log2, end = min(j.n, begin + (1u << j.chunk_log2));
         if (end < j.n) {
-            row = __ldg(key + end - 1);
-            const bool mine = row < j.total && __ldg(key + end) == row && (begin == 0 || __ldg(key + begin - 1) != row);
-            if (mine) count = ((row_end(key, end, j.n, row) - 1) >> j.chunk_log2) - chunk;
+            row = __ldg(&entry[end - 1].x);
+            const uint32_t next = __ldg(&entry[end].x), before = begin ? __ldg(&entry[begin - 1].x) : kNoRow;
+            if (row < j.total && next == row && before != row) {
+                // most rows end in the next 32 chunks: lane q looks at the end of chunk q + 1 behind this one
+                const uint64_t last = ((uint64_t)(chunk + 2 + lane) << j.chunk_log2) - 1;
+                const uint32_t through = __ballot_sync(0xffffffffu, last + 1 < j.n && __ldg(&entry[last].x) == row && __ldg(&entry[last + 1].x) == row);
+                count = through != 0xffffffffu ? __ffs(~through) : ((row_end(entry, end, j.n, row, lane) - 1) >> j.chunk_log2) - chunk;
+            }
         }
     }
     if (count > kLongSpan && lane == 0) { long_chunk = chunk; long_count = count; long_row = row; }
@@ -407,7 +439,7 @@ __global__ void __launch_bounds__(kCombineBlock) combine_kernel(const Job j, con
             float sum[N];
 #pragma unroll
             for (int k = 0; k < N; k++) sum[k] = s.tail[(size_t)chunk * s.pitch + c + k];
-#pragma unroll 4
+#pragma unroll 8
             for (uint32_t q = 1; q <= count; q++) {
                 const float* const part = s.head + (size_t)(chunk + q) * s.pitch + c;
 #pragma unroll
@@ -451,24 +483,24 @@ __global__ void __launch_bounds__(kCombineBlock) combine_kernel(const Job j, con
 // ---- host ---------------------------------------------------------------------------------------------------
 
 // Entries of a chunk: enough chunks to fill the GPU, and no more parts than that needs.
-int chunk_log2(uint64_t n) { return n < (1u << 17) ? 4 : n < (1u << 20) ? 5 : n < (1u << 22) ? 6 : 7; }
+int chunk_log2(uint64_t n) { return n < (1u << 17) ? 4 : n < (1u << 19) ? 5 : n < (1u << 21) ? 6 : 7; }
 int bits_for(uint64_t keys) { int b = 1; while (b < 32 && (1ull << b) < keys) b++; return b; }      // of the largest key, keys - 1
 
-size_t carve(uint64_t n, uint64_t total, uint32_t width, char* base, Space* s) {
-    const auto up = [](size_t x) { return (x + 255) / 256 * 256; };
+size_t carve(uint64_t n, uint64_t total, uint32_t width, bool pairs, char* base, Space* s) {
     size_t at = 0;
-    const auto take = [&](size_t bytes) { char* const p = base ? base + at : nullptr; at += up(bytes); return p; };
+    const auto take = [&](size_t bytes) { char* const p = base ? base + at : nullptr; at += (bytes + 255) / 256 * 256; return p; };
     Space sp = {};
     if (n) {
         sp.tiles = (uint32_t)((n + kTile - 1) / kTile);
         sp.chunks = (uint32_t)((n + (1u << chunk_log2(n)) - 1) >> chunk_log2(n));
         sp.pitch = (width + 3) / 4 * 4;
-        for (int k = 0; k < 2; k++) {
-            sp.key[k] = reinterpret_cast<uint32_t*>(take(4 * n));
-            sp.val[k] = reinterpret_cast<uint32_t*>(take(4 * n));
-        }
-        sp.counts = reinterpret_cast<uint32_t*>(take(4 * (size_t)sp.tiles * kMaxBins));
-        sp.totals = reinterpret_cast<uint32_t*>(take(4 * kMaxBins));
+        const bool small = n <= kSmall;
+        sp.entry[0] = reinterpret_cast<uint2*>(take(8 * n));
+        sp.entry[1] = reinterpret_cast<uint2*>(take(small ? 0 : 8 * n));
+        sp.key = reinterpret_cast<uint32_t*>(take(small ? 0 : 4 * n));
+        sp.counts = reinterpret_cast<uint32_t*>(take(small ? 0 : 4 * (size_t)sp.tiles * kMaxBins));
+        sp.totals = reinterpret_cast<uint32_t*>(take(small ? 0 : 4 * kMaxBins));
+        sp.pair = reinterpret_cast<uint4*>(take(pairs ? 16 * (n / 3) : 0));
         sp.head = reinterpret_cast<float*>(take(4 * (size_t)sp.chunks * sp.pitch));
         sp.tail = reinterpret_cast<float*>(take(4 * (size_t)sp.chunks * sp.pitch));
         sp.touched = reinterpret_cast<uint8_t*>(take(total));
@@ -477,54 +509,75 @@ size_t carve(uint64_t n, uint64_t total, uint32_t width, char* base, Space* s) {
     return at;
 }
 
+// Raises a kernel's limit of dynamic shared memory, once for a device.
+template <class Kernel>
+cudaError_t allow_smem(Kernel kernel, size_t bytes, LaunchCache& cache) {
+    int dev = 0, fit = 0;
+    const cudaError_t e = cudaGetDevice(&dev);
+    if (e != cudaSuccess) return e;
+    return (cudaError_t)cache.lookup(dev, 0, 0, bytes, [&](size_t most) { return (int)cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)most); },
+                                     [](int, size_t, int*) { return 0; }, &fit);
+}
+
+constexpr size_t scatter_smem(int bins) { return 8 * (size_t)kTile + 2 * (size_t)bins * kSortWarps + 8 * (size_t)bins; }
+
 // Sorts the entries; *which tells which of the two buffers holds them.
 cudaError_t sort_entries(const Job& j, const Space& s, int* which, cudaStream_t st) {
+    static LaunchCache small_cache, first_cache, next_cache;
     const int key_bits = bits_for((uint64_t)j.total + 1);
     if (j.n <= kSmall) {
         const int passes = (key_bits + kSmallDigitBits - 1) / kSmallDigitBits, bits = (key_bits + passes - 1) / passes;
-        constexpr size_t smem = 4 * 4 * (size_t)kSmall + 32 * 2 * (1 << kSmallDigitBits) + 4 * (1 << kSmallDigitBits) + 4 * 32;
-        const cudaError_t e = cudaFuncSetAttribute(small_sort_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+        const cudaError_t e = allow_smem(small_sort_kernel, kSmallSmem, small_cache);
         if (e != cudaSuccess) return e;
-        small_sort_kernel<<<1, kSmallBlock, smem, st>>>(j, s, passes, bits);
+        small_sort_kernel<<<1, kSmallBlock, kSmallSmem, st>>>(j, s, passes, bits);
         *which = 0;
         return cudaGetLastError();
     }
     const int passes = (key_bits + kMaxDigitBits - 1) / kMaxDigitBits, bits = (key_bits + passes - 1) / passes, bins = 1 << bits;
     const bool scanned = s.tiles > kScanTiles;
-    const size_t smem = 4 * (size_t)bins + 2 * (size_t)bins * (kSortBlock / 32);
+    cudaError_t e = allow_smem(scatter_kernel<true>, scatter_smem(kMaxBins), first_cache);
+    if (e == cudaSuccess) e = allow_smem(scatter_kernel<false>, scatter_smem(kMaxBins), next_cache);
+    if (e != cudaSuccess) return e;
     for (int p = 0; p < passes; p++) {
-        if (p == 0) count_kernel<true><<<s.tiles, kSortBlock, 0, st>>>(j, s, 0, 0, bits);
-        else count_kernel<false><<<s.tiles, kSortBlock, 0, st>>>(j, s, p & 1, p * bits, bits);
-        if (scanned) scan_kernel<<<(bins + 7) / 8, 256, 0, st>>>(s, bins);
-        if (p == 0) scatter_kernel<true><<<s.tiles, kSortBlock, smem, st>>>(j, s, 0, 0, bits, scanned);
-        else scatter_kernel<false><<<s.tiles, kSortBlock, smem, st>>>(j, s, p & 1, p * bits, bits, scanned);
+        const int from = p & 1;                                 // the first pass takes its entries from `key` and leaves them in entry[1]
+        if (p == 0) count_kernel<true><<<s.tiles, kSortBlock, 0, st>>>(j, s, from, 0, bits);
+        else count_kernel<false><<<s.tiles, kSortBlock, 0, st>>>(j, s, from, p * bits, bits);
+        if (scanned) scan_kernel<<<(bins + 31) / 32, 1024, 0, st>>>(s, bins);
+        if (p == 0) scatter_kernel<true><<<s.tiles, kSortBlock, scatter_smem(bins), st>>>(j, s, from, 0, bits, scanned);
+        else scatter_kernel<false><<<s.tiles, kSortBlock, scatter_smem(bins), st>>>(j, s, from, p * bits, bits, scanned);
     }
     *which = passes & 1;
     return cudaGetLastError();
 }
 
-template <typename T, typename Out, bool PAIRS>
-cudaError_t sum_entries(const Job& j, const Space& s, int which, bool aligned, cudaStream_t st) {
-    const uint32_t n_per = aligned ? 4 : 1, pieces = (j.width + n_per - 1) / n_per;
-    int log2 = 0;
+template <typename T, typename Out, int N, bool PAIRS>
+cudaError_t sum_pieces(const Job& j, const Space& s, int which, cudaStream_t st) {
+    const uint32_t pieces = (j.width + N - 1) / N;
+    int log2 = 3;
     while (log2 < 5 && (1u << log2) < pieces) log2++;
     const uint32_t teams_per_block = kReduceBlock >> log2;
     const dim3 grid((s.chunks + teams_per_block - 1) / teams_per_block, (pieces + (1u << log2) - 1) >> log2);
     const uint32_t combine_blocks = s.chunks > 1 ? (s.chunks + kCombineBlock / 32 - 1) / (kCombineBlock / 32) : 0;
     const uint32_t clear_blocks = j.accumulate ? 0 : (uint32_t)(((uint64_t)j.total + kCombineBlock - 1) / kCombineBlock);
-    if (j.n) {
-        if (aligned) reduce_kernel<T, Out, 4, PAIRS><<<grid, kReduceBlock, 0, st>>>(j, s, s.key[which], s.val[which], log2);
-        else reduce_kernel<T, Out, 1, PAIRS><<<grid, kReduceBlock, 0, st>>>(j, s, s.key[which], s.val[which], log2);
-    }
-    if (combine_blocks + clear_blocks) {
-        if (aligned) combine_kernel<Out, 4><<<combine_blocks + clear_blocks, kCombineBlock, 0, st>>>(j, s, s.key[which], combine_blocks);
-        else combine_kernel<Out, 1><<<combine_blocks + clear_blocks, kCombineBlock, 0, st>>>(j, s, s.key[which], combine_blocks);
-    }
+    if (j.n) reduce_kernel<T, Out, N, PAIRS><<<grid, kReduceBlock, 0, st>>>(j, s, s.entry[which], log2);
+    if (combine_blocks + clear_blocks) combine_kernel<Out, (N < 4 ? N : 4)><<<combine_blocks + clear_blocks, kCombineBlock, 0, st>>>(j, s, s.entry[which], combine_blocks);
     return cudaGetLastError();
 }
 
-int check_workspace(uint64_t n, uint64_t total, uint32_t width, void* workspace, uint64_t bytes) {
-    const size_t need = carve(n, total, width, nullptr, nullptr);
+// `pieces`: elements that all rows may be moved in.
+template <typename T, typename Out, bool PAIRS>
+cudaError_t sum_entries(const Job& j, const Space& s, int which, uint32_t pieces, cudaStream_t st) {
+    if (sizeof(T) == 2 && pieces == 8) return sum_pieces<T, Out, (sizeof(T) == 2 ? 8 : 4), PAIRS>(j, s, which, st);
+    return pieces >= 4 ? sum_pieces<T, Out, 4, PAIRS>(j, s, which, st) : sum_pieces<T, Out, 1, PAIRS>(j, s, which, st);
+}
+uint32_t pieces_of(std::initializer_list<const mascot_rows*> all) {
+    uint32_t n = 8;
+    for (const mascot_rows* m : all) n = aligned_rows(*m, n) ? n : aligned_rows(*m, 4) ? 4 : 1;
+    return n;
+}
+
+int check_workspace(uint64_t n, uint64_t total, uint32_t width, bool pairs, void* workspace, uint64_t bytes) {
+    const size_t need = carve(n, total, width, pairs, nullptr, nullptr);
     if (need == 0) return MASCOT_OK;
     if (!workspace || bytes < need) return fail(nullptr, MASCOT_ERR_BAD_ARG, "workspace: smaller than the *_workspace call says");
     if (reinterpret_cast<uintptr_t>(workspace) % 16) return fail(nullptr, MASCOT_ERR_BAD_ARG, "workspace: must be 16-byte aligned");
@@ -540,14 +593,14 @@ extern "C" {
 
 int mascot_rows_gradient_workspace(uint64_t count, uint64_t rows, uint32_t width, uint64_t* bytes) {
     if (!bytes || count >= kMaxRows || rows >= kMaxRows || width == 0 || width > kMaxWidth) return fail(nullptr, MASCOT_ERR_BAD_ARG, "null pointer or size out of range");
-    *bytes = carve(count, rows, width, nullptr, nullptr);
+    *bytes = carve(count, rows, width, false, nullptr, nullptr);
     return MASCOT_OK;
 }
 
 int mascot_pair_gradient_workspace(uint64_t count, uint64_t n_users, uint64_t n_items, uint32_t width, uint64_t* bytes) {
     if (!bytes || count >= kMaxRows || n_users >= kMaxRows || n_items >= kMaxRows || width == 0 || width > kMaxWidth || 3 * count >= kMaxRows || n_users + n_items >= kMaxRows)
         return fail(nullptr, MASCOT_ERR_BAD_ARG, "null pointer or size out of range");
-    *bytes = carve(3 * count, n_users + n_items, width, nullptr, nullptr);
+    *bytes = carve(3 * count, n_users + n_items, width, true, nullptr, nullptr);
     return MASCOT_OK;
 }
 
@@ -558,7 +611,7 @@ int mascot_rows_gradient(const mascot_rows* grad, const mascot_ids* ids, float s
     ROW_CHECK(check_rows("out", out, false));
     if (grad->width != out->width) return fail(nullptr, MASCOT_ERR_BAD_ARG, "out: width is not the gradient's");
     if (grad->rows != ids->count) return fail(nullptr, MASCOT_ERR_BAD_ARG, "grad: must have a row for each id");
-    ROW_CHECK(check_workspace(ids->count, out->rows, out->width, workspace, workspace_bytes));
+    ROW_CHECK(check_workspace(ids->count, out->rows, out->width, false, workspace, workspace_bytes));
     const size_t id_bytes = ids->count * ids->bits / 8;
     ROW_CHECK(check_distinct("grad", grad, "out", out));
     ROW_CHECK(check_distinct("ids", ids->data, id_bytes, "out", out));
@@ -587,14 +640,14 @@ int mascot_rows_gradient(const mascot_rows* grad, const mascot_ids* ids, float s
     j.chunk_log2 = chunk_log2(j.n);
     j.scale = scale; j.accumulate = accumulate != 0; j.flags = flags;
     Space s;
-    carve(j.n, j.total, j.width, static_cast<char*>(workspace), &s);
+    carve(j.n, j.total, j.width, false, static_cast<char*>(workspace), &s);
     const cudaStream_t st = static_cast<cudaStream_t>(stream);
     int which = 0;
     if (j.n) CU(nullptr, sort_entries(j, s, &which, st));
-    const bool aligned = aligned_rows(*grad, 4) && aligned_rows(*out, 4);
+    const uint32_t pieces = pieces_of({grad, out});
     const cudaError_t launched = with_type(grad->type, [&](auto* t) {
         return with_type(out->type, [&](auto* o) {
-            return sum_entries<std::remove_pointer_t<decltype(t)>, std::remove_pointer_t<decltype(o)>, false>(j, s, which, aligned, st);
+            return sum_entries<std::remove_pointer_t<decltype(t)>, std::remove_pointer_t<decltype(o)>, false>(j, s, which, pieces, st);
         });
     });
     CU(nullptr, launched);
@@ -616,7 +669,7 @@ int mascot_pair_gradient(const mascot_rows* P, const mascot_rows* Q, const masco
     if (3 * n >= kMaxRows || total >= kMaxRows) return fail(nullptr, MASCOT_ERR_BAD_ARG, "three times the pairs, and the rows of both tables, must be below 2^31 - 1");
     if (n && !coef) return fail(nullptr, MASCOT_ERR_BAD_ARG, "coef: null pointer");
     if (reinterpret_cast<uintptr_t>(coef) % 4) return fail(nullptr, MASCOT_ERR_BAD_ARG, "coef: address is not a multiple of the element's size");
-    ROW_CHECK(check_workspace(3 * n, total, P->width, workspace, workspace_bytes));
+    ROW_CHECK(check_workspace(3 * n, total, P->width, true, workspace, workspace_bytes));
     ROW_CHECK(check_distinct("dP", dP, "dQ", dQ));
     for (const auto* out : {dP, dQ}) {
         const char* const name = out == dP ? "dP" : "dQ";
@@ -652,14 +705,14 @@ int mascot_pair_gradient(const mascot_rows* P, const mascot_rows* Q, const masco
     j.chunk_log2 = chunk_log2(j.n);
     j.scale = scale; j.accumulate = accumulate != 0; j.flags = flags;
     Space s;
-    carve(j.n, j.total, j.width, static_cast<char*>(workspace), &s);
+    carve(j.n, j.total, j.width, true, static_cast<char*>(workspace), &s);
     const cudaStream_t st = static_cast<cudaStream_t>(stream);
     int which = 0;
     if (j.n) CU(nullptr, sort_entries(j, s, &which, st));
-    const bool aligned = aligned_rows(*P, 4) && aligned_rows(*Q, 4) && aligned_rows(*dP, 4) && aligned_rows(*dQ, 4);
+    const uint32_t pieces = pieces_of({P, Q, dP, dQ});
     const cudaError_t launched = with_type(P->type, [&](auto* t) {
         return with_type(dP->type, [&](auto* o) {
-            return sum_entries<std::remove_pointer_t<decltype(t)>, std::remove_pointer_t<decltype(o)>, true>(j, s, which, aligned, st);
+            return sum_entries<std::remove_pointer_t<decltype(t)>, std::remove_pointer_t<decltype(o)>, true>(j, s, which, pieces, st);
         });
     });
     CU(nullptr, launched);
