@@ -9,8 +9,8 @@
 //            the items' rows counted behind the users'.  Up to kSmall entries one block does all passes in shared
 //            memory; more take count / scan / scatter kernels for each digit.
 //   reduce   the sorted entries are cut into chunks of equal length, a team of lanes for each, so that a popular row is
-//            shared by many teams and many unpopular ones by one.  A row that lies within a chunk is written at once; of one that
-//            goes on in the next chunk or comes from the one before, the chunk's part is left in the workspace.
+//            shared by many teams and many unpopular ones by one.  A row that ends less than a quarter of a chunk behind a chunk's
+//            end is finished by that chunk's team; of one that goes on further, each chunk's part is left in the workspace.
 //   combine  adds these parts up in the order of the chunks, and clears rows that no entry names.
 #include <algorithm>
 #include <initializer_list>
@@ -21,19 +21,19 @@
 namespace mascot {
 namespace {
 
-constexpr int kSortBlock = 512, kSortItems = 16, kTile = kSortBlock * kSortItems, kSortWarps = kSortBlock / 32;     // entries of a block of the sort
-constexpr int kMaxDigitBits = 10, kMaxBins = 1 << kMaxDigitBits;
-constexpr int kScanTiles = 32;                  // up to so many tiles the scatter kernel adds their counts up itself
-constexpr int kSmallBlock = 1024, kSmallItems = 12, kSmallWarps = kSmallBlock / 32;
+constexpr int kSortBlock = 512, kSortWarps = kSortBlock / 32;
+constexpr int kFewItems = 4, kManyItems = 16;   // entries of a thread of the sort: a tile is 2048 or 8192
+constexpr uint32_t kManyFrom = 1u << 20;        // entries from which tiles are large: there are enough of them for all SMs then
+constexpr int kMaxBins = 1024;                  // digits of 8 or 10 bits
+constexpr uint32_t kScanTiles = 16;             // up to so many tiles the scatter kernel adds their counts up itself
+constexpr int kSmallBlock = 512, kSmallItems = 8, kSmallWarps = kSmallBlock / 32, kSmallBits = 8, kSmallBins = 1 << kSmallBits;
 constexpr uint32_t kSmall = kSmallBlock * kSmallItems;
-constexpr int kSmallDigitBits = 8, kSmallBins = 1 << kSmallDigitBits;
-constexpr int kReduceBlock = 256, kCombineBlock = 1024;
-constexpr uint32_t kLongSpan = 64;              // chunks of one row that a warp still adds up alone
+constexpr int kReduceBlock = 256, kCombineBlock = 512, kCombineBlocksPerSm = 4;
 
 // What is summed: where entries come from and what their values are.
 struct Job {
     Ids ids[3];                                 // lookup: one; pairs: users, preferred, other
-    uint32_t per;                               // ids of one kind: entry e is id e % per of kind e / per
+    uint32_t per;                               // ids of one kind; entry e of pairs is id e / 3 of kind e % 3, so that a tile of entries is one of pairs
     uint32_t kinds;                             // 1: lookup, 3: pairs
     uint32_t n;                                 // entries: kinds * per
     uint32_t rows[2];                           // of the table; of both tables
@@ -54,34 +54,49 @@ struct Space {                                  // the workspace, see carve()
     uint2* entry[2];                            // (row, entry)
     uint4* pair;                                // user, preferred, other, bits of coef
     float *head, *tail;                         // [chunks][pitch]
+    uint32_t *owners, *n_owners;                // chunks where a row begins whose parts are added up
     uint8_t* touched;                           // a byte per row
     uint32_t pitch, chunks, tiles;
 };
 
 // ---- sort --------------------------------------------------------------------------------------------------
 
-// Row of entry e, or `total`.  Pairs: the entry of the user also leaves the pair's rows where the sums find them.
-__device__ __forceinline__ uint32_t entry_key(const Job& j, const Space& s, uint32_t e, bool& bad) {
+// Rows, or `total`, of COUNT entries `step` apart, as far as there are so many; all loads are under way at once.  Pairs: the entry of the
+// user also leaves the pair where the sums find it.
+template <int COUNT>
+__device__ __forceinline__ void entry_keys(const Job& j, const Space& s, uint32_t first, uint32_t step, uint32_t (&key)[COUNT], bool& bad) {
+    uint32_t at[COUNT];
+#pragma unroll
+    for (int k = 0; k < COUNT; k++) at[k] = min(first + k * step, j.n - 1) / j.kinds;
     if (j.kinds == 1) {
-        const uint32_t r = row_of(j.ids[0], e, j.rows[0], bad);
-        return r == kNoRow ? j.total : r;
+        RawId id[COUNT];
+        load_ids<COUNT>(j.ids[0], at, id);
+#pragma unroll
+        for (int k = 0; k < COUNT; k++) {
+            const uint32_t r = row_of(id[k], j.ids[0], j.rows[0], bad);
+            key[k] = r == kNoRow ? j.total : r;
+        }
+        return;
     }
-    const uint32_t kind = e >= 2 * j.per ? 2 : e >= j.per ? 1 : 0, b = e - kind * j.per;
-    const uint32_t u = row_of(j.ids[0], b, j.rows[0], bad), p = row_of(j.ids[1], b, j.rows[1], bad), o = row_of(j.ids[2], b, j.rows[1], bad);
-    if (kind == 0) s.pair[b] = make_uint4(u, p, o, __float_as_uint(__ldg(j.coef + b)));
-    if (u == kNoRow || p == kNoRow || o == kNoRow) return j.total;
-    return kind == 0 ? u : j.rows[0] + (kind == 1 ? p : o);
-}
-
-__device__ __forceinline__ void clear_touched(uint8_t* touched, uint32_t rows, size_t first, size_t step) {
-    for (size_t w = first; w < ((size_t)rows + 15) / 16; w += step) reinterpret_cast<uint4*>(touched)[w] = make_uint4(0, 0, 0, 0);
+    RawId u[COUNT], p[COUNT], o[COUNT];
+    load_ids<COUNT>(j.ids[0], at, u);
+    load_ids<COUNT>(j.ids[1], at, p);
+    load_ids<COUNT>(j.ids[2], at, o);
+#pragma unroll
+    for (int k = 0; k < COUNT; k++) {
+        const uint32_t e = first + k * step, b = e / 3, kind = e - 3 * b;
+        const uint32_t ur = row_of(u[k], j.ids[0], j.rows[0], bad), pr = row_of(p[k], j.ids[1], j.rows[1], bad), orow = row_of(o[k], j.ids[2], j.rows[1], bad);
+        if (e < j.n && kind == 0) s.pair[b] = make_uint4(ur, pr, orow, __float_as_uint(__ldg(j.coef + b)));
+        key[k] = ur == kNoRow || pr == kNoRow || orow == kNoRow ? j.total : kind == 0 ? ur : j.rows[0] + (kind == 1 ? pr : orow);
+    }
 }
 
 // Stable ranks of a warp's keys among the keys with the same digit that the warp has met so far; `count` is the
 // warp's own row of counters, zero at first.
-__device__ __forceinline__ uint32_t warp_rank(uint32_t digit, bool there, int bits, uint16_t* count, uint32_t lane) {
+template <int BITS> __device__ __forceinline__ uint32_t warp_rank(uint32_t digit, bool there, uint16_t* count, uint32_t lane) {
     uint32_t peers = __ballot_sync(0xffffffffu, there);
-    for (int b = 0; b < bits; b++) {
+#pragma unroll
+    for (int b = 0; b < BITS; b++) {
         const uint32_t set = __ballot_sync(0xffffffffu, digit >> b & 1);
         peers &= digit >> b & 1 ? set : ~set;
     }
@@ -131,49 +146,50 @@ __device__ __forceinline__ void block_scan(uint32_t* v, int bins, uint32_t* warp
     __syncthreads();
 }
 
-constexpr size_t kSmallSmem = 8 * (size_t)kSmall + 2 * (size_t)kSmallWarps * kSmallBins + 4 * kSmallBins + 4 * 32;
+__device__ __forceinline__ void begin_sums(const Job& j, const Space& s, size_t first, size_t step) {
+    if (first == 0) *s.n_owners = 0;
+    if (!j.accumulate) for (size_t w = first; w < ((size_t)j.total + 15) / 16; w += step) reinterpret_cast<uint4*>(s.touched)[w] = make_uint4(0, 0, 0, 0);
+}
 
 // One block: entries stay in registers while they are ranked and go through shared memory to their next place.  A sort over
 // many blocks costs two launches a digit at least.
-__global__ void __launch_bounds__(kSmallBlock) small_sort_kernel(const Job j, const Space s, int passes, int bits) {
-    extern __shared__ uint2 at[];
-    uint16_t* const count = reinterpret_cast<uint16_t*>(at + kSmall);
-    uint32_t* const start = reinterpret_cast<uint32_t*>(count + kSmallWarps * kSmallBins), *const warp_sums = start + kSmallBins;
-    const int t = threadIdx.x, lane = t & 31, warp = t >> 5, bins = 1 << bits;
-    if (!j.accumulate) clear_touched(s.touched, j.total, t, kSmallBlock);
+__global__ void __launch_bounds__(kSmallBlock) small_sort_kernel(const Job j, const Space s, int passes) {
+    __shared__ uint2 at[kSmall];
+    __shared__ __align__(16) uint16_t count[kSmallWarps * kSmallBins];
+    __shared__ uint32_t start[kSmallBins], warp_sums[32];
+    const int t = threadIdx.x, lane = t & 31, warp = t >> 5;
+    begin_sums(j, s, t, kSmallBlock);
     const uint32_t rounds = (j.n + kSmallBlock - 1) / kSmallBlock, first = warp * rounds * 32 + lane;      // a warp's entries, in order
     bool bad = false;
-    uint2 e[kSmallItems];
+    uint32_t key[kSmallItems], val[kSmallItems];
+    entry_keys<kSmallItems>(j, s, first, 32, key, bad);
 #pragma unroll
-    for (int k = 0; k < kSmallItems; k++) {
-        const uint32_t i = first + k * 32;
-        e[k] = make_uint2(0, i);
-        if (k < rounds && i < j.n) e[k].x = entry_key(j, s, i, bad);
-    }
+    for (int k = 0; k < kSmallItems; k++) val[k] = first + k * 32;
     if (bad && j.flags) atomicOr(j.flags, (uint32_t)MASCOT_FLAG_BAD_ID);
-    uint16_t* const mine = count + (warp << bits);
+    uint16_t* const mine = count + warp * kSmallBins;
     for (int p = 0; p < passes; p++) {
-        for (int b = lane; b < bins / 2; b += 32) reinterpret_cast<uint32_t*>(mine)[b] = 0;
+        const int shift = p * kSmallBits;
+        reinterpret_cast<uint4*>(mine)[lane] = make_uint4(0, 0, 0, 0);
         __syncwarp();
         uint32_t rank[kSmallItems];
 #pragma unroll
         for (int k = 0; k < kSmallItems; k++)
-            if (k < rounds) rank[k] = warp_rank(e[k].x >> (p * bits) & (bins - 1), first + k * 32 < j.n, bits, mine, lane);
+            if (k < rounds) rank[k] = warp_rank<kSmallBits>(key[k] >> shift & (kSmallBins - 1), first + k * 32 < j.n, mine, lane);
         __syncthreads();
-        for (int b = t; b < bins / 2; b += kSmallBlock) {
-            const uint32_t sums = warp_offsets(count, kSmallWarps, bins, b);
-            start[2 * b] = sums & 0xffff;
-            start[2 * b + 1] = sums >> 16;
+        if (t < kSmallBins / 2) {
+            const uint32_t sums = warp_offsets(count, kSmallWarps, kSmallBins, t);
+            start[2 * t] = sums & 0xffff;
+            start[2 * t + 1] = sums >> 16;
         }
         __syncthreads();
-        block_scan(start, bins, warp_sums);
+        block_scan(start, kSmallBins, warp_sums);
 #pragma unroll
         for (int k = 0; k < kSmallItems; k++)
-            if (k < rounds && first + k * 32 < j.n) { const uint32_t d = e[k].x >> (p * bits) & (bins - 1); at[start[d] + mine[d] + rank[k]] = e[k]; }
+            if (k < rounds && first + k * 32 < j.n) { const uint32_t d = key[k] >> shift & (kSmallBins - 1); at[start[d] + mine[d] + rank[k]] = make_uint2(key[k], val[k]); }
         __syncthreads();
         if (p + 1 < passes) {
 #pragma unroll
-            for (int k = 0; k < kSmallItems; k++) if (k < rounds && first + k * 32 < j.n) e[k] = at[first + k * 32];
+            for (int k = 0; k < kSmallItems; k++) if (k < rounds && first + k * 32 < j.n) { key[k] = at[first + k * 32].x; val[k] = at[first + k * 32].y; }
             // `at` is written again only behind the next pass's barriers
         }
     }
@@ -181,24 +197,32 @@ __global__ void __launch_bounds__(kSmallBlock) small_sort_kernel(const Job j, co
 }
 
 // Counts of the digits of a tile, [tile][bin].  The first pass makes the keys, and keeps them.
-template <bool FIRST>
-__global__ void __launch_bounds__(kSortBlock) count_kernel(const Job j, const Space s, int from, int shift, int bits) {
+template <bool FIRST, int ITEMS>
+__global__ void __launch_bounds__(kSortBlock) count_kernel(const Job j, const Space s, const uint2* entry, int shift, int bits) {
     __shared__ uint32_t hist[kMaxBins];
     const int bins = 1 << bits;
     for (int b = threadIdx.x; b < bins; b += kSortBlock) hist[b] = 0;
-    if (FIRST && !j.accumulate) clear_touched(s.touched, j.total, (size_t)blockIdx.x * kSortBlock + threadIdx.x, (size_t)gridDim.x * kSortBlock);
-    bool bad = false;
-    uint32_t key[kSortItems];
+    if (FIRST) begin_sums(j, s, (size_t)blockIdx.x * kSortBlock + threadIdx.x, (size_t)gridDim.x * kSortBlock);
+    const uint32_t first = blockIdx.x * (ITEMS * kSortBlock) + threadIdx.x;
+    uint32_t key[ITEMS];
+    if (FIRST) {
+        bool bad = false;
 #pragma unroll
-    for (int k = 0; k < kSortItems; k++) {
-        const uint32_t e = blockIdx.x * kTile + k * kSortBlock + threadIdx.x;
-        if (e < j.n) key[k] = FIRST ? entry_key(j, s, e, bad) : s.entry[from][e].x;
+        for (int k = 0; k < ITEMS; k += 4) {
+            uint32_t four[4];
+            entry_keys<4>(j, s, first + k * kSortBlock, kSortBlock, four, bad);
+#pragma unroll
+            for (int q = 0; q < 4; q++) key[k + q] = four[q];
+        }
+        if (bad && j.flags) atomicOr(j.flags, (uint32_t)MASCOT_FLAG_BAD_ID);
+    } else {
+#pragma unroll
+        for (int k = 0; k < ITEMS; k++) key[k] = entry[min(first + k * kSortBlock, j.n - 1)].x;
     }
-    if (FIRST && bad && j.flags) atomicOr(j.flags, (uint32_t)MASCOT_FLAG_BAD_ID);
     __syncthreads();
 #pragma unroll
-    for (int k = 0; k < kSortItems; k++) {
-        const uint32_t e = blockIdx.x * kTile + k * kSortBlock + threadIdx.x;
+    for (int k = 0; k < ITEMS; k++) {
+        const uint32_t e = first + k * kSortBlock;
         if (e < j.n) {
             if (FIRST) s.key[e] = key[k];
             atomicAdd(&hist[key[k] >> shift & (bins - 1)], 1u);
@@ -234,25 +258,22 @@ __global__ void __launch_bounds__(1024) scan_kernel(const Space s, int bins) {
 
 // Moves a tile's entries to their places: ranked by warps in the order of the entries, put in order in shared memory, and written from
 // there, so that the entries of a bin leave as one run.
-template <bool FIRST>
-__global__ void __launch_bounds__(kSortBlock) scatter_kernel(const Job j, const Space s, int from, int shift, int bits, bool scanned) {
+template <bool FIRST, int ITEMS, int BITS>
+__global__ void __launch_bounds__(kSortBlock, 2) scatter_kernel(const Space s, uint32_t n, const uint2* from, uint2* to, int shift, bool scanned) {
     extern __shared__ uint2 at[];                               // entries in their order; the warps' counters; the bins' offsets
     __shared__ uint32_t warp_sums[32];
-    const int t = threadIdx.x, lane = t & 31, warp = t >> 5, bins = 1 << bits;
-    uint16_t* const count = reinterpret_cast<uint16_t*>(at + kTile), *const mine = count + (warp << bits);
-    uint32_t* const start = reinterpret_cast<uint32_t*>(count + (kSortWarps << bits)), *const base = start + bins;
+    const int t = threadIdx.x, lane = t & 31, warp = t >> 5;
+    constexpr int bins = 1 << BITS, kTile = ITEMS * kSortBlock, kPer = (bins + kSortBlock - 1) / kSortBlock;
+    uint16_t* const count = reinterpret_cast<uint16_t*>(at + kTile), *const mine = count + (warp << BITS);
+    uint32_t* const start = reinterpret_cast<uint32_t*>(count + (kSortWarps << BITS)), *const base = start + bins;
     for (int b = lane; b < bins / 2; b += 32) reinterpret_cast<uint32_t*>(mine)[b] = 0;
-    const uint32_t first = blockIdx.x * kTile + warp * (32 * kSortItems) + lane;
-    uint2 e[kSortItems];
+    const uint32_t first = blockIdx.x * kTile + warp * (32 * ITEMS) + lane;
+    uint32_t key[ITEMS];
 #pragma unroll
-    for (int k = 0; k < kSortItems; k++) {
-        const uint32_t i = first + k * 32;
-        e[k] = make_uint2(0, i);
-        if (i < j.n) { if (FIRST) e[k].x = s.key[i]; else e[k] = s.entry[from][i]; }
-    }
-    uint32_t within[kMaxBins / kSortBlock];                     // entries of the bin in the tiles before
+    for (int k = 0; k < ITEMS; k++) { const uint32_t i = min(first + k * 32, n - 1); key[k] = FIRST ? s.key[i] : from[i].x; }
+    uint32_t within[kPer];                     // entries of the bin in the tiles before
 #pragma unroll
-    for (int k = 0; k < kMaxBins / kSortBlock; k++) {
+    for (int k = 0; k < kPer; k++) {
         const int b = t + k * kSortBlock;
         within[k] = 0;
         if (b < bins) {
@@ -266,9 +287,12 @@ __global__ void __launch_bounds__(kSortBlock) scatter_kernel(const Job j, const 
         }
     }
     __syncwarp();
-    uint32_t rank[kSortItems];
+    uint32_t rank[ITEMS / 2];                              // two to a word
 #pragma unroll
-    for (int k = 0; k < kSortItems; k++) rank[k] = warp_rank(e[k].x >> shift & (bins - 1), first + k * 32 < j.n, bits, mine, lane);
+    for (int k = 0; k < ITEMS; k++) {
+        const uint32_t r = warp_rank<BITS>(key[k] >> shift & (bins - 1), first + k * 32 < n, mine, lane);
+        if (k % 2 == 0) rank[k / 2] = r; else rank[k / 2] |= r << 16;
+    }
     __syncthreads();
     for (int b = t; b < bins / 2; b += kSortBlock) {
         const uint32_t sums = warp_offsets(count, kSortWarps, bins, b);
@@ -278,14 +302,16 @@ __global__ void __launch_bounds__(kSortBlock) scatter_kernel(const Job j, const 
     block_scan(base, bins, warp_sums);
     block_scan(start, bins, warp_sums);
 #pragma unroll
-    for (int k = 0; k < kMaxBins / kSortBlock; k++) { const int b = t + k * kSortBlock; if (b < bins) base[b] += within[k] - start[b]; }
+    for (int k = 0; k < kPer; k++) { const int b = t + k * kSortBlock; if (b < bins) base[b] += within[k] - start[b]; }
 #pragma unroll
-    for (int k = 0; k < kSortItems; k++)
-        if (first + k * 32 < j.n) { const uint32_t d = e[k].x >> shift & (bins - 1); at[start[d] + mine[d] + rank[k]] = e[k]; }
+    for (int k = 0; k < ITEMS; k++) {
+        const uint32_t i = first + k * 32, d = key[k] >> shift & (bins - 1);
+        if (i < n) at[start[d] + mine[d] + (rank[k / 2] >> 16 * (k % 2) & 0xffff)] = make_uint2(key[k], FIRST ? i : from[i].y);
+    }
     __syncthreads();
-    const uint32_t here = min((uint32_t)kTile, j.n - blockIdx.x * kTile);
+    const uint32_t here = min((uint32_t)kTile, n - blockIdx.x * kTile);
 #pragma unroll 4
-    for (uint32_t i = t; i < here; i += kSortBlock) { const uint2 x = at[i]; s.entry[from ^ 1][i + base[x.x >> shift & (bins - 1)]] = x; }
+    for (uint32_t i = t; i < here; i += kSortBlock) { const uint2 x = at[i]; to[i + base[x.x >> shift & (bins - 1)]] = x; }
 }
 
 // ---- sums --------------------------------------------------------------------------------------------------
@@ -306,73 +332,101 @@ __device__ __forceinline__ void write_row(const Job& j, uint32_t row, uint32_t c
     store_piece<Out, N>(at, r);
 }
 
-// A team's lanes take a group of entries each, one round trip for all of them, and hand them round; the rows of BATCH
-// entries are in flight at once.  What bounds it is those rows: random ones, from HBM or L2.
+// What an entry adds: c * (row a - row b), without b where that is kNoRow; nothing where a is.
+struct Term { uint32_t key, a, b; float c; };
+template <bool PAIRS> __device__ __forceinline__ Term term_of(const Job& j, uint2 entry, uint4 pair) {
+    Term t{entry.x, entry.y, kNoRow, 1.f};
+    if (PAIRS) {
+        const uint32_t kind = entry.y % 3;
+        t.a = kind ? pair.x : pair.y;
+        if (kind == 0) t.b = pair.z;
+        t.c = kind == 2 ? -__uint_as_float(pair.w) : __uint_as_float(pair.w);
+        if (t.c == 0.f) t.a = kNoRow;                           // whatever the rows hold
+    }
+    if (entry.x >= j.total) t.a = kNoRow;
+    return t;
+}
+
+// A team's lanes take a group of entries each, one round trip for all of them and the next group's at the same time, and hand their
+// rows round; the rows of BATCH entries are in flight at once.  What bounds it is instructions: for 16 bytes of a row, eight
+// conversions and eight additions for two-byte types, and as many more for what goes with an entry.  So what a lane can
+// work out for a group (where rows begin, which entries add nothing) it does, and the team reads it off ballots.
 template <typename T, typename Out, int N, bool PAIRS>
-__global__ void __launch_bounds__(kReduceBlock) reduce_kernel(const Job j, const Space s, const uint2* entry, int team_log2) {
-    constexpr int BATCH = PAIRS ? 4 : 8;
-    const uint32_t team = 1u << team_log2, tl = threadIdx.x & (team - 1);
+__global__ void __launch_bounds__(kReduceBlock, N == 8 && PAIRS ? 2 : 3) reduce_kernel(const Job j, const Space s, const uint2* entry, int team_log2) {
+    constexpr int BATCH = 4;
+    const uint32_t team = 1u << team_log2, lane = threadIdx.x & 31, tl = lane & (team - 1), team_at = lane & ~(team - 1);
+    const uint32_t team_mask = (team == 32 ? 0xffffffffu : (1u << team) - 1) << team_at;
     const uint32_t chunk = (blockIdx.x * kReduceBlock + threadIdx.x) >> team_log2, col = ((blockIdx.y << team_log2) + tl) * N;
+    const uint32_t size = 1u << j.chunk_log2, over = size / 4;
+    const uint32_t begin = min(j.n, chunk << j.chunk_log2), end = min(j.n, begin + size);
     const bool writes = chunk < s.chunks && col < j.width;
-    const uint32_t begin = min(j.n, chunk << j.chunk_log2), end = min(j.n, begin + (1u << j.chunk_log2));
-    const uint32_t before = chunk < s.chunks && begin ? __ldg(&entry[begin - 1].x) : kNoRow, after = end < j.n ? __ldg(&entry[end].x) : kNoRow;
+    // rows across the chunk's ends: finished by the chunk before where they end within `over` entries, else in parts
+    const auto row_at = [&](uint32_t i) { return i < j.n ? __ldg(&entry[i].x) : kNoRow; };
+    const uint32_t before = chunk < s.chunks && begin ? row_at(begin - 1) : kNoRow, last = end > begin ? row_at(end - 1) : kNoRow;
+    const bool in_parts = before != kNoRow && row_at(begin + over) == before, on_in_parts = end < j.n && row_at(end + over) == last;
+    const uint32_t until = on_in_parts || end == begin ? end : min(j.n, end + over);
     const T* const src0 = static_cast<const T*>(j.src[0]) + col, *const src1 = static_cast<const T*>(j.src[1]) + col;
-    uint32_t row = kNoRow;
+    uint32_t row = j.total;
     float sum[N] = {};
     const auto flush = [&]() {
         if (row >= j.total || !writes) return;
-        if (row == before || row == after) {                   // part of a row that other chunks share
-            float* const part = (row == before ? s.head : s.tail) + (size_t)chunk * s.pitch + col;
+        const bool from_before = in_parts && row == before;
+        if (from_before || (on_in_parts && row == last)) {
+            float* const part = (from_before ? s.head : s.tail) + (size_t)chunk * s.pitch + col;
 #pragma unroll
             for (int k = 0; k < N; k++) part[k] = sum[k];
+            if (!from_before && col == 0) s.owners[atomicAdd(s.n_owners, 1u)] = chunk;
         } else write_row<Out, N>(j, row, col, sum);
-        if (row != before && !j.accumulate && col == 0) s.touched[row] = 1;
+        if (!from_before && !j.accumulate && col == 0) s.touched[row] = 1;
     };
-    for (uint32_t g = begin; __any_sync(0xffffffffu, g < end); g += team) {
-        uint2 mine = make_uint2(j.total, 0);
-        if (g + tl < end) mine = __ldg(entry + g + tl);
-        uint32_t my_a = mine.y, my_b = kNoRow;
-        float my_c = 1.f;
-        if (PAIRS && mine.x < j.total) {
-            const uint32_t kind = mine.y >= 2 * j.per ? 2 : mine.y >= j.per ? 1 : 0;
-            const uint4 p = __ldg(s.pair + (mine.y - kind * j.per));
-            my_c = kind == 2 ? -__uint_as_float(p.w) : __uint_as_float(p.w);
-            my_a = kind ? p.x : p.y;
-            if (kind == 0) my_b = p.z;
-        }
+    const auto entry_at = [&](uint32_t i) {
+        uint2 e = make_uint2(j.total, 0);
+        if (i < until) e = __ldg(entry + i);
+        if (i >= end ? e.x != last : !in_parts && e.x == before) e.x = j.total;
+        return e;
+    };
+    const auto pair_of = [&](uint2 e) { return PAIRS && e.x < j.total ? __ldg(s.pair + e.y / 3) : make_uint4(0, 0, 0, 0); };
+    uint2 now = entry_at(begin + tl), next = entry_at(begin + team + tl);
+    uint4 pair = pair_of(now);
+    for (uint32_t g = begin; __any_sync(0xffffffffu, g < until); g += team) {
+        const Term mine = term_of<PAIRS>(j, now, pair);
+        const uint32_t left = __shfl_up_sync(0xffffffffu, mine.key, 1, team);
+        const uint32_t begins = __ballot_sync(0xffffffffu, mine.key != (tl ? left : row)) >> team_at, adds = __ballot_sync(0xffffffffu, mine.a != kNoRow) >> team_at;
+        const uint32_t twos = PAIRS ? __ballot_sync(0xffffffffu, mine.b != kNoRow) >> team_at : 0u;
+        now = next;
+        pair = pair_of(now);
+        next = entry_at(g + 2 * team + tl);
         for (uint32_t k0 = 0; k0 < team; k0 += BATCH) {
-            if (!__any_sync(0xffffffffu, g + k0 < end)) break;
-            uint32_t key[BATCH], b_row[BATCH];
+            if (!__any_sync(0xffffffffu, g + k0 < until)) break;
+            Piece<T, N> a[BATCH], b[PAIRS ? BATCH : 1];
             float c[BATCH];
-            Piece<T, N> a[BATCH], b[BATCH];
 #pragma unroll
             for (int k = 0; k < BATCH; k++) {
-                key[k] = __shfl_sync(0xffffffffu, mine.x, k0 + k, team);
-                const uint32_t a_row = __shfl_sync(0xffffffffu, my_a, k0 + k, team);
-                c[k] = PAIRS ? __shfl_sync(0xffffffffu, my_c, k0 + k, team) : 1.f;
-                b_row[k] = PAIRS ? __shfl_sync(0xffffffffu, my_b, k0 + k, team) : kNoRow;
-                if (key[k] >= j.total || !writes) c[k] = 0.f;   // coef 0: whatever the rows hold
-                if (c[k] != 0.f) {
-                    a[k] = load_piece<T, N>(!PAIRS || b_row[k] == kNoRow ? src0 + a_row * j.src_stride[0] : src1 + a_row * j.src_stride[1]);
-                    if (PAIRS && b_row[k] != kNoRow) b[k] = load_piece<T, N>(src1 + b_row[k] * j.src_stride[1]);
+                const uint32_t ra = __shfl_sync(0xffffffffu, mine.a, k0 + k, team), rb = PAIRS ? __shfl_sync(0xffffffffu, mine.b, k0 + k, team) : kNoRow;
+                c[k] = PAIRS ? __shfl_sync(0xffffffffu, mine.c, k0 + k, team) : 1.f;
+                const bool two = PAIRS && (twos >> (k0 + k) & 1);
+                if ((adds >> (k0 + k) & 1) && writes) {
+                    a[k] = load_piece<T, N>(two ? src1 + ra * j.src_stride[1] : src0 + ra * j.src_stride[0]);
+                    if (PAIRS && two) b[k] = load_piece<T, N>(src1 + rb * j.src_stride[1]);
                 }
             }
 #pragma unroll
             for (int k = 0; k < BATCH; k++) {
-                if (key[k] != row) {
+                if (begins >> (k0 + k) & 1) {
                     flush();
-                    row = key[k];
+                    row = __shfl_sync(team_mask, mine.key, k0 + k, team);
 #pragma unroll
                     for (int x = 0; x < N; x++) sum[x] = 0.f;
                 }
-                if (c[k] != 0.f) {
+                if (adds >> (k0 + k) & 1) {
 #pragma unroll
                     for (int x = 0; x < N; x++) {
                         if (!PAIRS) sum[x] += as_float(a[k].v[x]);
-                        else sum[x] = fmaf(c[k], b_row[k] != kNoRow ? as_float(a[k].v[x]) - as_float(b[k].v[x]) : as_float(a[k].v[x]), sum[x]);
+                        else sum[x] = fmaf(c[k], twos >> (k0 + k) & 1 ? as_float(a[k].v[x]) - as_float(b[k].v[x]) : as_float(a[k].v[x]), sum[x]);
                     }
                 }
             }
+            __syncwarp();
         }
     }
     flush();
@@ -390,11 +444,10 @@ __device__ __forceinline__ uint32_t row_end(const uint2* entry, uint32_t at, uin
     return hi;
 }
 
-// Blocks below `combine_blocks`: a warp per chunk adds up the row that begins in it and goes on behind it.  A row over
-// more than kLongSpan chunks is added up by all warps of the block, a slice each: only one row a block can be that long, since it
-// covers all chunks of the block behind its first.  The other blocks clear the rows that no entry names, a warp for 32 of them.
+// Blocks below `combine_blocks`: each takes rows whose parts are to be added up, its warps a slice of the parts each.  The other blocks
+// clear the rows that no entry names, a warp for 32 of them.
 template <typename Out, int N>
-__global__ void __launch_bounds__(kCombineBlock) combine_kernel(const Job j, const Space s, const uint2* entry, uint32_t combine_blocks) {
+__global__ void __launch_bounds__(kCombineBlock, kCombineBlocksPerSm) combine_kernel(const Job j, const Space s, const uint2* entry, uint32_t combine_blocks) {
     const uint32_t lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     if (blockIdx.x >= combine_blocks) {
         const uint32_t row0 = (blockIdx.x - combine_blocks) * kCombineBlock + warp * 32;
@@ -414,69 +467,42 @@ __global__ void __launch_bounds__(kCombineBlock) combine_kernel(const Job j, con
         }
         return;
     }
-    __shared__ float slice[kCombineBlock / 32][32 * N];
-    __shared__ uint32_t long_chunk, long_count, long_row;
-    if (threadIdx.x == 0) long_count = 0;
-    __syncthreads();
-    const uint32_t chunk = blockIdx.x * (kCombineBlock / 32) + warp;
-    uint32_t row = kNoRow, count = 0;                           // chunks that follow
-    if (chunk < s.chunks) {
-        const uint32_t begin = chunk << j.chunk_log2, end = min(j.n, begin + (1u << j.chunk_log2));
-        if (end < j.n) {
-            row = __ldg(&entry[end - 1].x);
-            const uint32_t next = __ldg(&entry[end].x), before = begin ? __ldg(&entry[begin - 1].x) : kNoRow;
-            if (row < j.total && next == row && before != row) {
-                // most rows end in the next 32 chunks: lane q looks at the end of chunk q + 1 behind this one
-                const uint64_t last = ((uint64_t)(chunk + 2 + lane) << j.chunk_log2) - 1;
-                const uint32_t through = __ballot_sync(0xffffffffu, last + 1 < j.n && __ldg(&entry[last].x) == row && __ldg(&entry[last + 1].x) == row);
-                count = through != 0xffffffffu ? __ffs(~through) : ((row_end(entry, end, j.n, row, lane) - 1) >> j.chunk_log2) - chunk;
-            }
-        }
-    }
-    if (count > kLongSpan && lane == 0) { long_chunk = chunk; long_count = count; long_row = row; }
-    if (count && count <= kLongSpan) {
-        for (uint32_t c = lane * N; c < j.width; c += 32 * N) {
-            float sum[N];
+    constexpr int kWarps = kCombineBlock / 32;
+    __shared__ float slice[kWarps][32 * N];
+    const uint32_t owners = *s.n_owners, size = 1u << j.chunk_log2;
+    for (uint32_t o = blockIdx.x; o < owners; o += combine_blocks) {
+        const uint32_t chunk = s.owners[o], first = (chunk + 1) << j.chunk_log2, row = __ldg(&entry[first].x);
+        // chunks that follow with a part of the row: all but one where it ends within a quarter, whose entries are in the part before
+        const uint32_t stop = row_end(entry, first, j.n, row, lane), whole = (stop - first) >> j.chunk_log2;
+        const uint32_t count = whole + (stop - first - whole * size > size / 4 ? 1 : 0);
+        const uint32_t per = (count + kWarps - 1) / kWarps, q0 = 1 + warp * per, q1 = min(count + 1, q0 + per);
+        for (uint32_t c0 = 0; c0 < j.width; c0 += 32 * N) {
+            const uint32_t c = c0 + lane * N;
+            float sum[N] = {};
+            if (c < j.width) {
+                if (warp == 0) {
 #pragma unroll
-            for (int k = 0; k < N; k++) sum[k] = s.tail[(size_t)chunk * s.pitch + c + k];
+                    for (int k = 0; k < N; k++) sum[k] = s.tail[(size_t)chunk * s.pitch + c + k];
+                }
 #pragma unroll 8
-            for (uint32_t q = 1; q <= count; q++) {
-                const float* const part = s.head + (size_t)(chunk + q) * s.pitch + c;
+                for (uint32_t q = q0; q < q1; q++) {
+                    const Piece<float, N> part = *reinterpret_cast<const Piece<float, N>*>(s.head + (size_t)(chunk + q) * s.pitch + c);
 #pragma unroll
-                for (int k = 0; k < N; k++) sum[k] += part[k];
+                    for (int k = 0; k < N; k++) sum[k] += part.v[k];
+                }
             }
-            write_row<Out, N>(j, row, c, sum);
-        }
-    }
-    __syncthreads();
-    const uint32_t all = long_count;
-    if (all == 0) return;
-    const uint32_t per = (all + kCombineBlock / 32 - 1) / (kCombineBlock / 32), q0 = 1 + warp * per, q1 = min(all + 1, q0 + per);
-    for (uint32_t c0 = 0; c0 < j.width; c0 += 32 * N) {
-        const uint32_t c = c0 + lane * N;
-        float sum[N] = {};
-        if (c < j.width) {
-            if (warp == 0) {
 #pragma unroll
-                for (int k = 0; k < N; k++) sum[k] = s.tail[(size_t)long_chunk * s.pitch + c + k];
+            for (int k = 0; k < N; k++) slice[warp][lane * N + k] = sum[k];
+            __syncthreads();
+            if (warp == 0 && c < j.width) {
+#pragma unroll
+                for (int w = 1; w < kWarps; w++)
+#pragma unroll
+                    for (int k = 0; k < N; k++) sum[k] += slice[w][lane * N + k];
+                write_row<Out, N>(j, row, c, sum);
             }
-#pragma unroll 8
-            for (uint32_t q = q0; q < q1; q++) {
-                const float* const part = s.head + (size_t)(long_chunk + q) * s.pitch + c;
-#pragma unroll
-                for (int k = 0; k < N; k++) sum[k] += part[k];
-            }
+            __syncthreads();
         }
-#pragma unroll
-        for (int k = 0; k < N; k++) slice[warp][lane * N + k] = sum[k];
-        __syncthreads();
-        if (warp == 0 && c < j.width) {
-            for (int w = 1; w < kCombineBlock / 32; w++)
-#pragma unroll
-                for (int k = 0; k < N; k++) sum[k] += slice[w][lane * N + k];
-            write_row<Out, N>(j, long_row, c, sum);
-        }
-        __syncthreads();
     }
 }
 
@@ -491,7 +517,8 @@ size_t carve(uint64_t n, uint64_t total, uint32_t width, bool pairs, char* base,
     const auto take = [&](size_t bytes) { char* const p = base ? base + at : nullptr; at += (bytes + 255) / 256 * 256; return p; };
     Space sp = {};
     if (n) {
-        sp.tiles = (uint32_t)((n + kTile - 1) / kTile);
+        const uint32_t tile = kSortBlock * (n < kManyFrom ? kFewItems : kManyItems);
+        sp.tiles = (uint32_t)((n + tile - 1) / tile);
         sp.chunks = (uint32_t)((n + (1u << chunk_log2(n)) - 1) >> chunk_log2(n));
         sp.pitch = (width + 3) / 4 * 4;
         const bool small = n <= kSmall;
@@ -503,6 +530,8 @@ size_t carve(uint64_t n, uint64_t total, uint32_t width, bool pairs, char* base,
         sp.pair = reinterpret_cast<uint4*>(take(pairs ? 16 * (n / 3) : 0));
         sp.head = reinterpret_cast<float*>(take(4 * (size_t)sp.chunks * sp.pitch));
         sp.tail = reinterpret_cast<float*>(take(4 * (size_t)sp.chunks * sp.pitch));
+        sp.owners = reinterpret_cast<uint32_t*>(take(4 * (size_t)sp.chunks));
+        sp.n_owners = reinterpret_cast<uint32_t*>(take(4));
         sp.touched = reinterpret_cast<uint8_t*>(take(total));
     }
     if (s) *s = sp;
@@ -519,35 +548,42 @@ cudaError_t allow_smem(Kernel kernel, size_t bytes, LaunchCache& cache) {
                                      [](int, size_t, int*) { return 0; }, &fit);
 }
 
-constexpr size_t scatter_smem(int bins) { return 8 * (size_t)kTile + 2 * (size_t)bins * kSortWarps + 8 * (size_t)bins; }
+// One digit of BITS bits: the first pass takes its entries from `key`.
+template <int ITEMS, int BITS>
+cudaError_t sort_digit(const Job& j, const Space& s, int pass, cudaStream_t st) {
+    static LaunchCache first_cache, next_cache;
+    constexpr int bins = 1 << BITS;
+    constexpr size_t smem = 8 * (size_t)ITEMS * kSortBlock + 2 * (size_t)bins * kSortWarps + 8 * (size_t)bins;
+    cudaError_t e = allow_smem(scatter_kernel<true, ITEMS, BITS>, smem, first_cache);
+    if (e == cudaSuccess) e = allow_smem(scatter_kernel<false, ITEMS, BITS>, smem, next_cache);
+    if (e != cudaSuccess) return e;
+    const bool scanned = s.tiles > kScanTiles;
+    uint2* const from = s.entry[pass & 1], *const to = s.entry[~pass & 1];
+    if (pass == 0) count_kernel<true, ITEMS><<<s.tiles, kSortBlock, 0, st>>>(j, s, nullptr, 0, BITS);
+    else count_kernel<false, ITEMS><<<s.tiles, kSortBlock, 0, st>>>(j, s, from, pass * BITS, BITS);
+    if (scanned) scan_kernel<<<bins / 32, 1024, 0, st>>>(s, bins);
+    if (pass == 0) scatter_kernel<true, ITEMS, BITS><<<s.tiles, kSortBlock, smem, st>>>(s, j.n, nullptr, to, 0, scanned);
+    else scatter_kernel<false, ITEMS, BITS><<<s.tiles, kSortBlock, smem, st>>>(s, j.n, from, to, pass * BITS, scanned);
+    return cudaGetLastError();
+}
 
 // Sorts the entries; *which tells which of the two buffers holds them.
 cudaError_t sort_entries(const Job& j, const Space& s, int* which, cudaStream_t st) {
-    static LaunchCache small_cache, first_cache, next_cache;
     const int key_bits = bits_for((uint64_t)j.total + 1);
     if (j.n <= kSmall) {
-        const int passes = (key_bits + kSmallDigitBits - 1) / kSmallDigitBits, bits = (key_bits + passes - 1) / passes;
-        const cudaError_t e = allow_smem(small_sort_kernel, kSmallSmem, small_cache);
-        if (e != cudaSuccess) return e;
-        small_sort_kernel<<<1, kSmallBlock, kSmallSmem, st>>>(j, s, passes, bits);
+        small_sort_kernel<<<1, kSmallBlock, 0, st>>>(j, s, (key_bits + kSmallBits - 1) / kSmallBits);
         *which = 0;
         return cudaGetLastError();
     }
-    const int passes = (key_bits + kMaxDigitBits - 1) / kMaxDigitBits, bits = (key_bits + passes - 1) / passes, bins = 1 << bits;
-    const bool scanned = s.tiles > kScanTiles;
-    cudaError_t e = allow_smem(scatter_kernel<true>, scatter_smem(kMaxBins), first_cache);
-    if (e == cudaSuccess) e = allow_smem(scatter_kernel<false>, scatter_smem(kMaxBins), next_cache);
-    if (e != cudaSuccess) return e;
+    const bool ten = (key_bits + 9) / 10 < (key_bits + 7) / 8, many = j.n >= kManyFrom;      // wider digits where they save a pass
+    const int passes = ten ? (key_bits + 9) / 10 : (key_bits + 7) / 8;
     for (int p = 0; p < passes; p++) {
-        const int from = p & 1;                                 // the first pass takes its entries from `key` and leaves them in entry[1]
-        if (p == 0) count_kernel<true><<<s.tiles, kSortBlock, 0, st>>>(j, s, from, 0, bits);
-        else count_kernel<false><<<s.tiles, kSortBlock, 0, st>>>(j, s, from, p * bits, bits);
-        if (scanned) scan_kernel<<<(bins + 31) / 32, 1024, 0, st>>>(s, bins);
-        if (p == 0) scatter_kernel<true><<<s.tiles, kSortBlock, scatter_smem(bins), st>>>(j, s, from, 0, bits, scanned);
-        else scatter_kernel<false><<<s.tiles, kSortBlock, scatter_smem(bins), st>>>(j, s, from, p * bits, bits, scanned);
+        const cudaError_t e = many ? (ten ? sort_digit<kManyItems, 10>(j, s, p, st) : sort_digit<kManyItems, 8>(j, s, p, st))
+                                   : (ten ? sort_digit<kFewItems, 10>(j, s, p, st) : sort_digit<kFewItems, 8>(j, s, p, st));
+        if (e != cudaSuccess) return e;
     }
     *which = passes & 1;
-    return cudaGetLastError();
+    return cudaSuccess;
 }
 
 template <typename T, typename Out, int N, bool PAIRS>
@@ -557,7 +593,7 @@ cudaError_t sum_pieces(const Job& j, const Space& s, int which, cudaStream_t st)
     while (log2 < 5 && (1u << log2) < pieces) log2++;
     const uint32_t teams_per_block = kReduceBlock >> log2;
     const dim3 grid((s.chunks + teams_per_block - 1) / teams_per_block, (pieces + (1u << log2) - 1) >> log2);
-    const uint32_t combine_blocks = s.chunks > 1 ? (s.chunks + kCombineBlock / 32 - 1) / (kCombineBlock / 32) : 0;
+    const uint32_t combine_blocks = s.chunks > 1 ? std::min<uint32_t>(s.chunks - 1, kCombineBlocksPerSm * current_sms()) : 0;
     const uint32_t clear_blocks = j.accumulate ? 0 : (uint32_t)(((uint64_t)j.total + kCombineBlock - 1) / kCombineBlock);
     if (j.n) reduce_kernel<T, Out, N, PAIRS><<<grid, kReduceBlock, 0, st>>>(j, s, s.entry[which], log2);
     if (combine_blocks + clear_blocks) combine_kernel<Out, (N < 4 ? N : 4)><<<combine_blocks + clear_blocks, kCombineBlock, 0, st>>>(j, s, s.entry[which], combine_blocks);

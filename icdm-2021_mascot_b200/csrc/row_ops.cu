@@ -80,6 +80,11 @@ int check_device() {
     return fail(nullptr, MASCOT_ERR_NO_DEVICE, "no usable CUDA device; libmascot has no CPU path");
 }
 
+int current_sms() {
+    int dev = 0, n = 0;
+    return cudaGetDevice(&dev) == cudaSuccess && cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev) == cudaSuccess ? n : 1;
+}
+
 int check_memory(const char* what, const void* p) {
     if (!p) return MASCOT_OK;
     cudaPointerAttributes at;
@@ -116,7 +121,7 @@ __global__ void __launch_bounds__(kLookupBlock) lookup_kernel(const LookupArgs a
     uint32_t row[kLookupRows];
     bool bad = false;
 #pragma unroll
-    for (int k = 0; k < kLookupRows; k++) row[k] = first + k < a.n ? row_of(a.ids, first + k, a.rows, bad) : kNoRow;
+    for (int k = 0; k < kLookupRows; k++) row[k] = first + k < a.n ? row_of(a.ids, (uint32_t)(first + k), a.rows, bad) : kNoRow;
     if (bad && tl == 0 && a.flags) atomicOr(a.flags, (uint32_t)MASCOT_FLAG_BAD_ID);
     for (uint32_t c = tl * N; c < a.width; c += N << team_log2) {
         Piece<In, N> in[kLookupRows];
@@ -158,9 +163,9 @@ cudaError_t launch_lookup(const LookupArgs& a, bool aligned, cudaStream_t st) {
 }
 
 // ---- preference loss -------------------------------------------------------------------------------------------
-// A pair is three rows and a dot product: bound by fetching rows, and by the latency of two dependent loads where there are
-// few pairs.  A team has the rows of kPairs pairs in flight; its lanes sum products in fp32 and then work out one
-// pair each.
+// A pair is three rows and a dot product: bound by fetching rows, and by the instructions around them.  A team of lanes takes a
+// run of pairs: each lane finds the rows of one of them and hands them round, the rows of kPairs pairs are in flight at once, and
+// in the end each lane works out the loss of its own pair.
 constexpr int kPairBlock = 256, kPairs = 4;
 
 struct PairArgs {
@@ -175,75 +180,81 @@ struct PairArgs {
 };
 
 template <typename T, int N>
-__global__ void __launch_bounds__(kPairBlock) pair_loss_kernel(const PairArgs a, int team_log2) {
-    const int team = 1 << team_log2, tl = threadIdx.x & (team - 1);
-    const size_t first = (((size_t)blockIdx.x * kPairBlock + threadIdx.x) >> team_log2) * kPairs;
-    uint32_t u[kPairs], i[kPairs], j[kPairs];
+__global__ void __launch_bounds__(kPairBlock, 2) pair_loss_kernel(const PairArgs a, int team_log2, uint32_t run) {
+    const uint32_t team = 1u << team_log2, lane = threadIdx.x & 31, tl = lane & (team - 1);
+    const size_t first = (((size_t)blockIdx.x * kPairBlock + threadIdx.x) >> team_log2) * run, at = first + tl;      // this lane's pair
+    const bool in_run = tl < run && at < a.n;
+    uint32_t u = kNoRow, i = kNoRow, j = kNoRow;
     bool bad = false;
+    if (in_run) {
+        u = row_of(a.u, (uint32_t)at, a.n_users, bad);
+        i = row_of(a.i, (uint32_t)at, a.n_items, bad);
+        j = row_of(a.j, (uint32_t)at, a.n_items, bad);
+        if (i == kNoRow || j == kNoRow) u = kNoRow;
+    }
+    if (bad && a.flags) atomicOr(a.flags, (uint32_t)MASCOT_FLAG_BAD_ID);
+    const float reference = in_run && a.reference ? __ldg(a.reference + at) : 0.f, w = in_run && a.weight ? __ldg(a.weight + at) : 1.f;
+    const uint32_t there = __ballot_sync(0xffffffffu, u != kNoRow) >> (lane & ~(team - 1));
+    const T* const P = static_cast<const T*>(a.P), *const Q = static_cast<const T*>(a.Q);
+    float margin = 0.f;
+    for (uint32_t k0 = 0; k0 < run; k0 += kPairs) {
+        float m[kPairs] = {};
+        uint32_t uk[kPairs], ik[kPairs], jk[kPairs];
 #pragma unroll
-    for (int k = 0; k < kPairs; k++) {
-        u[k] = i[k] = j[k] = kNoRow;
-        if (first + k < a.n) {
-            u[k] = row_of(a.u, first + k, a.n_users, bad);
-            i[k] = row_of(a.i, first + k, a.n_items, bad);
-            j[k] = row_of(a.j, first + k, a.n_items, bad);
-            if (i[k] == kNoRow || j[k] == kNoRow) u[k] = kNoRow;
+        for (int k = 0; k < kPairs; k++) {
+            uk[k] = __shfl_sync(0xffffffffu, u, k0 + k, team);
+            ik[k] = __shfl_sync(0xffffffffu, i, k0 + k, team);
+            jk[k] = __shfl_sync(0xffffffffu, j, k0 + k, team);
         }
-    }
-    if (bad && tl == 0 && a.flags) atomicOr(a.flags, (uint32_t)MASCOT_FLAG_BAD_ID);
-    float m[kPairs] = {};
-    for (uint32_t c = tl * N; c < a.width; c += N << team_log2) {
-        Piece<T, N> p[kPairs], qi[kPairs], qj[kPairs];
+        for (uint32_t c = tl * N; c < a.width; c += N << team_log2) {
+            Piece<T, N> p[kPairs], qi[kPairs], qj[kPairs];
 #pragma unroll
-        for (int k = 0; k < kPairs; k++)
-            if (u[k] != kNoRow) {
-                p[k] = load_piece<T, N>(static_cast<const T*>(a.P) + u[k] * a.p_stride + c);
-                qi[k] = load_piece<T, N>(static_cast<const T*>(a.Q) + i[k] * a.q_stride + c);
-                qj[k] = load_piece<T, N>(static_cast<const T*>(a.Q) + j[k] * a.q_stride + c);
-            }
+            for (int k = 0; k < kPairs; k++)
+                if (k0 + k < team && (there >> (k0 + k) & 1)) {
+                    p[k] = load_piece<T, N>(P + uk[k] * a.p_stride + c);
+                    qi[k] = load_piece<T, N>(Q + ik[k] * a.q_stride + c);
+                    qj[k] = load_piece<T, N>(Q + jk[k] * a.q_stride + c);
+                }
 #pragma unroll
-        for (int k = 0; k < kPairs; k++)
-            if (u[k] != kNoRow) {
+            for (int k = 0; k < kPairs; k++)
+                if (k0 + k < team && (there >> (k0 + k) & 1)) {
 #pragma unroll
-                for (int x = 0; x < N; x++) m[k] = fmaf(as_float(p[k].v[x]), as_float(qi[k].v[x]) - as_float(qj[k].v[x]), m[k]);
-            }
-    }
-    for (int d = team >> 1; d >= 1; d >>= 1) {
-#pragma unroll
-        for (int k = 0; k < kPairs; k++) m[k] += __shfl_xor_sync(0xffffffffu, m[k], d);
-    }
-    // lane k of the team: pair k (a team of one or two lanes goes round)
-    for (int k = tl; k < kPairs; k += team) {
-        const size_t at = first + k;
-        if (at >= a.n) break;
-        const float mk = k == 0 ? m[0] : k == 1 ? m[1] : k == 2 ? m[2] : m[3];
-        const bool there = (k == 0 ? u[0] : k == 1 ? u[1] : k == 2 ? u[2] : u[3]) != kNoRow;
-        float loss = 0.f, coef = 0.f;
-        if (there) {
-            const float z = a.beta * (a.reference ? mk - __ldg(a.reference + at) : mk), w = a.weight ? __ldg(a.weight + at) : 1.f;
-            // log(1 + exp(x)) = max(x, 0) + log(1 + exp(-|x|)); 1 - sigmoid(|z|) = e / (1 + e) keeps its digits where sigmoid is near 1
-            const float e = expf(-fabsf(z)), soft = log1pf(e), tail = e / (1.f + e), eps = a.smoothing, part = z >= 0.f ? eps : 1.f - eps;
-            if (w != 0.f) {
-                loss = w * (part == 0.f ? soft : fmaf(part, fabsf(z), soft));      // no 0 * infinity
-                coef = w * a.beta * (z >= 0.f ? eps - tail : tail - (1.f - eps));
-            }
+                    for (int x = 0; x < N; x++) m[k] = fmaf(as_float(p[k].v[x]), as_float(qi[k].v[x]) - as_float(qj[k].v[x]), m[k]);
+                }
         }
-        if (a.margin) a.margin[at] = there ? mk : 0.f;
-        if (a.loss) a.loss[at] = loss;
-        if (a.coef) a.coef[at] = coef;
+        for (uint32_t d = team >> 1; d >= 1; d >>= 1) {
+#pragma unroll
+            for (int k = 0; k < kPairs; k++) m[k] += __shfl_xor_sync(0xffffffffu, m[k], d);
+        }
+#pragma unroll
+        for (int k = 0; k < kPairs; k++) margin = tl == k0 + k ? m[k] : margin;
     }
+    if (!in_run) return;
+    float loss = 0.f, coef = 0.f;
+    if (u != kNoRow && w != 0.f) {
+        // log(1 + exp(x)) = max(x, 0) + log(1 + exp(-|x|)); 1 - sigmoid(|z|) = e / (1 + e) keeps its digits where sigmoid is near 1
+        const float z = a.beta * (margin - reference), e = expf(-fabsf(z)), soft = log1pf(e), tail = e / (1.f + e), eps = a.smoothing, part = z >= 0.f ? eps : 1.f - eps;
+        loss = w * (part == 0.f ? soft : fmaf(part, fabsf(z), soft));      // no 0 * infinity
+        coef = w * a.beta * (z >= 0.f ? eps - tail : tail - (1.f - eps));
+    }
+    if (a.margin) a.margin[at] = margin;
+    if (a.loss) a.loss[at] = loss;
+    if (a.coef) a.coef[at] = coef;
 }
 
 template <typename T>
 cudaError_t launch_pair_loss(const PairArgs& a, bool aligned, cudaStream_t st) {
     constexpr int N = 16 / sizeof(T);
     const uint32_t pieces = aligned ? a.width / N : a.width;
-    int log2 = 0;
+    int log2 = 2;
     while (log2 < 5 && (1u << log2) < pieces) log2++;
-    const size_t teams = (a.n + kPairs - 1) / kPairs;
-    const unsigned grid = (unsigned)((teams + (kPairBlock >> log2) - 1) / (kPairBlock >> log2));
-    if (aligned) pair_loss_kernel<T, N><<<grid, kPairBlock, 0, st>>>(a, log2);
-    else pair_loss_kernel<T, 1><<<grid, kPairBlock, 0, st>>>(a, log2);
+    // pairs of a team: as many as it has lanes where there are enough of them, one batch where there are few
+    const size_t teams = (size_t)current_sms() * 2 * (kPairBlock >> log2);
+    const uint32_t run = (uint32_t)std::min<size_t>(1u << log2, std::max<size_t>(kPairs, a.n / teams / kPairs * kPairs));
+    const size_t runs = (a.n + run - 1) / run;
+    const unsigned grid = (unsigned)((runs + (kPairBlock >> log2) - 1) / (kPairBlock >> log2));
+    if (aligned) pair_loss_kernel<T, N><<<grid, kPairBlock, 0, st>>>(a, log2, run);
+    else pair_loss_kernel<T, 1><<<grid, kPairBlock, 0, st>>>(a, log2, run);
     return cudaGetLastError();
 }
 

@@ -26,6 +26,7 @@ int check_distinct(const char* what_a, const void* a, size_t bytes_a, const char
 int check_distinct(const char* what_a, const void* a, size_t bytes_a, const char* what_b, const void* b, size_t bytes_b);
 int check_device();                                                     // there is one (a launch refuses a stream of another one itself)
 int check_memory(const char* what, const void* p);                       // device memory of the current device
+int current_sms();                                                          // of the current device
 
 #define ROW_CHECK(call) do { const int rc_ = (call); if (rc_ != MASCOT_OK) return rc_; } while (0)
 
@@ -44,12 +45,28 @@ inline Ids ids_of(const mascot_ids& ids) { return Ids{ids.data, ids.bits == 64};
 #ifdef __CUDACC__
 constexpr uint32_t kNoRow = 0xffffffffu;
 
-// The row that id `at` names in a table of `rows` rows, or kNoRow; `bad` collects ids that are neither rows nor -1.
-__device__ __forceinline__ uint32_t row_of(const Ids& ids, size_t at, uint32_t rows, bool& bad) {
-    const long long id = ids.wide ? __ldg(static_cast<const long long*>(ids.data) + at) : (long long)__ldg(static_cast<const int*>(ids.data) + at);
-    if (id >= 0 && id < (long long)rows) return (uint32_t)id;
-    bad |= id != -1;
+// Ids as they come, COUNT of them at once: all loads are under way together, whatever the ids' width.
+struct RawId { uint32_t low, high; };
+template <int COUNT> __device__ __forceinline__ void load_ids(const Ids& ids, const uint32_t (&at)[COUNT], RawId (&id)[COUNT]) {
+    if (ids.wide) {
+#pragma unroll
+        for (int k = 0; k < COUNT; k++) { const uint2 w = __ldg(static_cast<const uint2*>(ids.data) + at[k]); id[k] = {w.x, w.y}; }
+    } else {
+#pragma unroll
+        for (int k = 0; k < COUNT; k++) id[k] = {__ldg(static_cast<const uint32_t*>(ids.data) + at[k]), 0xffffffffu};
+    }
+}
+// The row that it names in a table of `rows` rows, or kNoRow; `bad` collects ids that are neither rows nor -1.
+__device__ __forceinline__ uint32_t row_of(RawId id, const Ids& ids, uint32_t rows, bool& bad) {
+    if (id.low < rows && (!ids.wide || id.high == 0)) return id.low;
+    bad |= (id.low & id.high) != 0xffffffffu;
     return kNoRow;
+}
+__device__ __forceinline__ uint32_t row_of(const Ids& ids, uint32_t at, uint32_t rows, bool& bad) {
+    const uint32_t one[1] = {at};
+    RawId id[1];
+    load_ids<1>(ids, one, id);
+    return row_of(id[0], ids, rows, bad);
 }
 
 template <typename T> __device__ __forceinline__ float as_float(T x);

@@ -422,11 +422,6 @@ bool tile_map(CUtensorMap* map, const mascot_rows& m, uint32_t box_rows) {
                           CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
-int sm_count() {
-    int dev = 0, n = 0;
-    return cudaGetDevice(&dev) == cudaSuccess && cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev) == cudaSuccess ? n : 1;
-}
-
 template <int CN, typename Out, Mode MODE>
 cudaError_t launch_product(const mascot_rows& a, const mascot_rows& b, const ProductArgs& given, int sms, cudaStream_t st) {
     using S = Shape<CN, MODE>;
@@ -464,7 +459,7 @@ cudaError_t launch_users(const mascot_rows& a, const mascot_rows& b, const Produ
 
 template <typename Out>
 cudaError_t launch_tiles(const mascot_rows& a, const mascot_rows& b, const ProductArgs& p, cudaStream_t st) {
-    const int sms = sm_count();
+    const int sms = current_sms();
     if (p.blocks == 1) return launch_users<Out, ONE>(a, b, p, sms, st);
     // lanes for users pay where there are enough for all of them; half a tile of items where whole ones leave SMs without a tile
     if (p.lane.shift && a.rows > kLanes)
