@@ -28,7 +28,7 @@ constexpr int kMaxBins = 1024;                  // digits of 8 or 10 bits
 constexpr uint32_t kScanTiles = 16;             // up to so many tiles the scatter kernel adds their counts up itself
 constexpr int kSmallBlock = 512, kSmallItems = 8, kSmallWarps = kSmallBlock / 32, kSmallBits = 8, kSmallBins = 1 << kSmallBits;
 constexpr uint32_t kSmall = kSmallBlock * kSmallItems;
-constexpr int kReduceBlock = 256, kCombineBlock = 512, kCombineBlocksPerSm = 4;
+constexpr int kReduceBlock = 256, kCombineBlock = 512;
 
 // What is summed: where entries come from and what their values are.
 struct Job {
@@ -347,14 +347,28 @@ template <bool PAIRS> __device__ __forceinline__ Term term_of(const Job& j, uint
     return t;
 }
 
-// A team's lanes take a group of entries each, one round trip for all of them and the next group's at the same time, and hand their
-// rows round; the rows of BATCH entries are in flight at once.  What bounds it is instructions: for 16 bytes of a row, eight
-// conversions and eight additions for two-byte types, and as many more for what goes with an entry.  So what a lane can
-// work out for a group (where rows begin, which entries add nothing) it does, and the team reads it off ballots.
+// 4, 8 or 16 bytes on their way to shared memory; rows of a table stay in L1 (popular ones come again), gradient rows do not.
+template <int BYTES, bool KEEP> __device__ __forceinline__ void fetch_piece(uint32_t to, const void* from) {
+    if constexpr (BYTES == 16 && !KEEP) asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(to), "l"(from) : "memory");
+    else asm volatile("cp.async.ca.shared.global [%0], [%1], %2;" ::"r"(to), "l"(from), "n"(BYTES) : "memory");
+}
+
+// A team's lanes take a group of entries each and hand their rows round; what a lane can work out for a group (where rows begin, which
+// entries add nothing) it does, and the team reads it off ballots.  What bounds it is the rows, random ones from HBM or
+// L2, so AHEAD of them are under way for each team: every lane copies its pieces into shared memory of its own, which needs
+// no registers and no meeting of threads (rows in registers: 4 in flight, 286 us for 4M rows of 256 bytes against 1.25 GB / 6.5 TB/s = 190).
+// Single elements (N = 1) are loaded where they are added.
+template <typename T, int N, bool PAIRS> struct Ring {
+    static constexpr int piece = sizeof(T) * N, ahead = PAIRS ? 8 : 16, sides = PAIRS ? 2 : 1;      // rows of an entry
+    static constexpr size_t smem = N > 1 ? (size_t)ahead * sides * kReduceBlock * piece : 0;
+};
+
 template <typename T, typename Out, int N, bool PAIRS>
-__global__ void __launch_bounds__(kReduceBlock, N == 8 && PAIRS ? 2 : 3) reduce_kernel(const Job j, const Space s, const uint2* entry, int team_log2) {
+__global__ void __launch_bounds__(kReduceBlock, 3) reduce_kernel(const Job j, const Space s, const uint2* entry, int team_log2) {
+    using R = Ring<T, N, PAIRS>;
     constexpr int BATCH = 4;
-    const uint32_t team = 1u << team_log2, lane = threadIdx.x & 31, tl = lane & (team - 1), team_at = lane & ~(team - 1);
+    extern __shared__ __align__(16) uint8_t ring[];             // [ahead][sides][threads]
+    const uint32_t team = 1u << team_log2, lane = threadIdx.x & 31, tl = lane & (team - 1), team_at = lane & ~(team - 1), ahead = min(team, (uint32_t)R::ahead);
     const uint32_t team_mask = (team == 32 ? 0xffffffffu : (1u << team) - 1) << team_at;
     const uint32_t chunk = (blockIdx.x * kReduceBlock + threadIdx.x) >> team_log2, col = ((blockIdx.y << team_log2) + tl) * N;
     const uint32_t size = 1u << j.chunk_log2, over = size / 4;
@@ -366,6 +380,9 @@ __global__ void __launch_bounds__(kReduceBlock, N == 8 && PAIRS ? 2 : 3) reduce_
     const bool in_parts = before != kNoRow && row_at(begin + over) == before, on_in_parts = end < j.n && row_at(end + over) == last;
     const uint32_t until = on_in_parts || end == begin ? end : min(j.n, end + over);
     const T* const src0 = static_cast<const T*>(j.src[0]) + col, *const src1 = static_cast<const T*>(j.src[1]) + col;
+    const size_t stride0 = j.src_stride[0], stride1 = j.src_stride[1];
+    const uint8_t* const mine_at = ring + threadIdx.x * R::piece;
+    const uint32_t mine_to = (uint32_t)__cvta_generic_to_shared(mine_at);
     uint32_t row = j.total;
     float sum[N] = {};
     const auto flush = [&]() {
@@ -386,48 +403,84 @@ __global__ void __launch_bounds__(kReduceBlock, N == 8 && PAIRS ? 2 : 3) reduce_
         return e;
     };
     const auto pair_of = [&](uint2 e) { return PAIRS && e.x < j.total ? __ldg(s.pair + e.y / 3) : make_uint4(0, 0, 0, 0); };
-    uint2 now = entry_at(begin + tl), next = entry_at(begin + team + tl);
-    uint4 pair = pair_of(now);
+    const auto ballot = [&](bool b) { return __ballot_sync(0xffffffffu, b) >> team_at; };
+    // rows of the entries k .. k + 3 of a group
+    const auto fetch = [&](const Term& t, uint32_t adds, uint32_t twos, uint32_t k0) {
+#pragma unroll
+        for (int k = 0; k < BATCH; k++) {
+            const uint32_t ra = __shfl_sync(0xffffffffu, t.a, k0 + k, team), rb = PAIRS ? __shfl_sync(0xffffffffu, t.b, k0 + k, team) : kNoRow;
+            if ((adds >> (k0 + k) & 1) && writes) {
+                const uint32_t to = mine_to + ((k0 + k) & (ahead - 1)) * (R::sides * kReduceBlock * R::piece);
+                const bool two = PAIRS && (twos >> (k0 + k) & 1);
+                fetch_piece<R::piece, PAIRS>(to, two ? src1 + ra * stride1 : src0 + ra * stride0);
+                if (PAIRS && two) fetch_piece<R::piece, PAIRS>(to + kReduceBlock * R::piece, src1 + rb * stride1);
+            }
+        }
+        asm volatile("cp.async.commit_group;" ::: "memory");
+    };
+    uint2 after = entry_at(begin + 2 * team + tl);
+    const uint2 e0 = entry_at(begin + tl), e1 = entry_at(begin + team + tl);
+    Term now = term_of<PAIRS>(j, e0, pair_of(e0)), next = term_of<PAIRS>(j, e1, pair_of(e1));
+    uint4 pair = pair_of(after);
+    uint32_t adds = ballot(now.a != kNoRow), twos = PAIRS ? ballot(now.b != kNoRow) : 0u;
+    if constexpr (N > 1) for (uint32_t k0 = 0; k0 < ahead; k0 += BATCH) fetch(now, adds, twos, k0);
     for (uint32_t g = begin; __any_sync(0xffffffffu, g < until); g += team) {
-        const Term mine = term_of<PAIRS>(j, now, pair);
-        const uint32_t left = __shfl_up_sync(0xffffffffu, mine.key, 1, team);
-        const uint32_t begins = __ballot_sync(0xffffffffu, mine.key != (tl ? left : row)) >> team_at, adds = __ballot_sync(0xffffffffu, mine.a != kNoRow) >> team_at;
-        const uint32_t twos = PAIRS ? __ballot_sync(0xffffffffu, mine.b != kNoRow) >> team_at : 0u;
-        now = next;
-        pair = pair_of(now);
-        next = entry_at(g + 2 * team + tl);
+        const uint32_t left = __shfl_up_sync(0xffffffffu, now.key, 1, team), begins = ballot(now.key != (tl ? left : row));
+        const uint32_t next_adds = ballot(next.a != kNoRow), next_twos = PAIRS ? ballot(next.b != kNoRow) : 0u;
         for (uint32_t k0 = 0; k0 < team; k0 += BATCH) {
             if (!__any_sync(0xffffffffu, g + k0 < until)) break;
             Piece<T, N> a[BATCH], b[PAIRS ? BATCH : 1];
             float c[BATCH];
+            if constexpr (N > 1) {
+                if (ahead == 16) asm volatile("cp.async.wait_group 3;" ::: "memory");
+                else asm volatile("cp.async.wait_group 1;" ::: "memory");
+            }
 #pragma unroll
             for (int k = 0; k < BATCH; k++) {
-                const uint32_t ra = __shfl_sync(0xffffffffu, mine.a, k0 + k, team), rb = PAIRS ? __shfl_sync(0xffffffffu, mine.b, k0 + k, team) : kNoRow;
-                c[k] = PAIRS ? __shfl_sync(0xffffffffu, mine.c, k0 + k, team) : 1.f;
-                const bool two = PAIRS && (twos >> (k0 + k) & 1);
-                if ((adds >> (k0 + k) & 1) && writes) {
-                    a[k] = load_piece<T, N>(two ? src1 + ra * j.src_stride[1] : src0 + ra * j.src_stride[0]);
-                    if (PAIRS && two) b[k] = load_piece<T, N>(src1 + rb * j.src_stride[1]);
+                c[k] = PAIRS ? __shfl_sync(0xffffffffu, now.c, k0 + k, team) : 1.f;
+                if constexpr (N > 1) {
+                    const uint8_t* const at = mine_at + ((k0 + k) & (ahead - 1)) * (R::sides * kReduceBlock * R::piece);
+                    a[k] = *reinterpret_cast<const Piece<T, N>*>(at);
+                    if (PAIRS) b[k] = *reinterpret_cast<const Piece<T, N>*>(at + kReduceBlock * R::piece);
+                } else {
+                    const uint32_t ra = __shfl_sync(0xffffffffu, now.a, k0 + k, team), rb = PAIRS ? __shfl_sync(0xffffffffu, now.b, k0 + k, team) : kNoRow;
+                    const bool two = PAIRS && (twos >> (k0 + k) & 1);
+                    if ((adds >> (k0 + k) & 1) && writes) {
+                        a[k] = load_piece<T, N>(two ? src1 + ra * stride1 : src0 + ra * stride0);
+                        if (PAIRS && two) b[k] = load_piece<T, N>(src1 + rb * stride1);
+                    }
                 }
             }
 #pragma unroll
             for (int k = 0; k < BATCH; k++) {
                 if (begins >> (k0 + k) & 1) {
                     flush();
-                    row = __shfl_sync(team_mask, mine.key, k0 + k, team);
+                    row = __shfl_sync(team_mask, now.key, k0 + k, team);
 #pragma unroll
                     for (int x = 0; x < N; x++) sum[x] = 0.f;
                 }
                 if (adds >> (k0 + k) & 1) {
+                    const bool two = PAIRS && (twos >> (k0 + k) & 1);
 #pragma unroll
                     for (int x = 0; x < N; x++) {
                         if (!PAIRS) sum[x] += as_float(a[k].v[x]);
-                        else sum[x] = fmaf(c[k], twos >> (k0 + k) & 1 ? as_float(a[k].v[x]) - as_float(b[k].v[x]) : as_float(a[k].v[x]), sum[x]);
+                        else sum[x] = fmaf(c[k], two ? as_float(a[k].v[x]) - as_float(b[k].v[x]) : as_float(a[k].v[x]), sum[x]);
                     }
                 }
             }
             __syncwarp();
+            if constexpr (N > 1) {                              // into the places that have just been read
+                const uint32_t k1 = k0 + ahead;
+                if (k1 < team) fetch(now, adds, twos, k1);
+                else fetch(next, next_adds, next_twos, k1 - team);
+            }
         }
+        now = next;
+        adds = next_adds;
+        twos = next_twos;
+        next = term_of<PAIRS>(j, after, pair);
+        after = entry_at(g + 3 * team + tl);
+        pair = pair_of(after);
     }
     flush();
 }
@@ -444,10 +497,20 @@ __device__ __forceinline__ uint32_t row_end(const uint2* entry, uint32_t at, uin
     return hi;
 }
 
-// Blocks below `combine_blocks`: each takes rows whose parts are to be added up, its warps a slice of the parts each.  The other blocks
-// clear the rows that no entry names, a warp for 32 of them.
+// Blocks below `combine_blocks` add up the parts of the rows that the owners name: a warp each, and all warps of the block a slice
+// each where a row has more parts than the block has warps.  The other blocks clear the rows that no entry names, a warp for 32 of them.
+template <int N> __device__ __forceinline__ void add_parts(const Space& s, uint32_t first, uint32_t end, uint32_t col, float (&sum)[N]) {
+#pragma unroll 16
+    for (uint32_t q = first; q < end; q++) {
+        const Piece<float, N> part = *reinterpret_cast<const Piece<float, N>*>(s.head + (size_t)q * s.pitch + col);
+#pragma unroll
+        for (int k = 0; k < N; k++) sum[k] += part.v[k];
+    }
+}
+
 template <typename Out, int N>
-__global__ void __launch_bounds__(kCombineBlock, kCombineBlocksPerSm) combine_kernel(const Job j, const Space s, const uint2* entry, uint32_t combine_blocks) {
+__global__ void __launch_bounds__(kCombineBlock, 2) combine_kernel(const Job j, const Space s, const uint2* entry, uint32_t combine_blocks) {
+    constexpr uint32_t kWarps = kCombineBlock / 32;
     const uint32_t lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     if (blockIdx.x >= combine_blocks) {
         const uint32_t row0 = (blockIdx.x - combine_blocks) * kCombineBlock + warp * 32;
@@ -467,42 +530,61 @@ __global__ void __launch_bounds__(kCombineBlock, kCombineBlocksPerSm) combine_ke
         }
         return;
     }
-    constexpr int kWarps = kCombineBlock / 32;
     __shared__ float slice[kWarps][32 * N];
+    __shared__ uint32_t long_chunk[kWarps], long_count[kWarps], long_row[kWarps], n_long;
     const uint32_t owners = *s.n_owners, size = 1u << j.chunk_log2;
-    for (uint32_t o = blockIdx.x; o < owners; o += combine_blocks) {
-        const uint32_t chunk = s.owners[o], first = (chunk + 1) << j.chunk_log2, row = __ldg(&entry[first].x);
-        // chunks that follow with a part of the row: all but one where it ends within a quarter, whose entries are in the part before
-        const uint32_t stop = row_end(entry, first, j.n, row, lane), whole = (stop - first) >> j.chunk_log2;
-        const uint32_t count = whole + (stop - first - whole * size > size / 4 ? 1 : 0);
-        const uint32_t per = (count + kWarps - 1) / kWarps, q0 = 1 + warp * per, q1 = min(count + 1, q0 + per);
-        for (uint32_t c0 = 0; c0 < j.width; c0 += 32 * N) {
-            const uint32_t c = c0 + lane * N;
-            float sum[N] = {};
-            if (c < j.width) {
-                if (warp == 0) {
+    for (uint32_t o0 = blockIdx.x * kWarps; o0 < owners; o0 += combine_blocks * kWarps) {
+        if (threadIdx.x == 0) n_long = 0;
+        __syncthreads();
+        if (o0 + warp < owners) {
+            const uint32_t chunk = s.owners[o0 + warp], first = (chunk + 1) << j.chunk_log2, row = __ldg(&entry[first].x);
+            // Chunks that follow with a part of the row.  Most rows end soon: lane q looks whether the row goes on in parts behind q chunks more.
+            const uint64_t at = (uint64_t)first + (uint64_t)lane * size + size / 4;
+            const uint32_t through = __ballot_sync(0xffffffffu, at < j.n && __ldg(&entry[at].x) == row);
+            uint32_t count = __popc(through);
+            if (through == 0xffffffffu) {                       // all but one where it ends within a quarter of a chunk: those entries are in the part before
+                const uint32_t stop = row_end(entry, first, j.n, row, lane), whole = (stop - first) >> j.chunk_log2;
+                count = whole + (stop - first - whole * size > size / 4 ? 1 : 0);
+            }
+            if (count > kWarps) {
+                if (lane == 0) { const uint32_t at_long = atomicAdd(&n_long, 1u); long_chunk[at_long] = chunk; long_count[at_long] = count; long_row[at_long] = row; }
+            } else {
+                for (uint32_t c = lane * N; c < j.width; c += 32 * N) {
+                    float sum[N];
 #pragma unroll
                     for (int k = 0; k < N; k++) sum[k] = s.tail[(size_t)chunk * s.pitch + c + k];
-                }
-#pragma unroll 8
-                for (uint32_t q = q0; q < q1; q++) {
-                    const Piece<float, N> part = *reinterpret_cast<const Piece<float, N>*>(s.head + (size_t)(chunk + q) * s.pitch + c);
-#pragma unroll
-                    for (int k = 0; k < N; k++) sum[k] += part.v[k];
+                    add_parts<N>(s, chunk + 1, chunk + 1 + count, c, sum);
+                    write_row<Out, N>(j, row, c, sum);
                 }
             }
-#pragma unroll
-            for (int k = 0; k < N; k++) slice[warp][lane * N + k] = sum[k];
-            __syncthreads();
-            if (warp == 0 && c < j.width) {
-#pragma unroll
-                for (int w = 1; w < kWarps; w++)
-#pragma unroll
-                    for (int k = 0; k < N; k++) sum[k] += slice[w][lane * N + k];
-                write_row<Out, N>(j, row, c, sum);
-            }
-            __syncthreads();
         }
+        __syncthreads();
+        for (uint32_t l = 0; l < n_long; l++) {
+            const uint32_t chunk = long_chunk[l], count = long_count[l], per = (count + kWarps - 1) / kWarps, q0 = min(count, warp * per), q1 = min(count, q0 + per);
+            for (uint32_t c0 = 0; c0 < j.width; c0 += 32 * N) {
+                const uint32_t c = c0 + lane * N;
+                float sum[N] = {};
+                if (c < j.width) {
+                    if (warp == 0) {
+#pragma unroll
+                        for (int k = 0; k < N; k++) sum[k] = s.tail[(size_t)chunk * s.pitch + c + k];
+                    }
+                    add_parts<N>(s, chunk + 1 + q0, chunk + 1 + q1, c, sum);
+                }
+#pragma unroll
+                for (int k = 0; k < N; k++) slice[warp][lane * N + k] = sum[k];
+                __syncthreads();
+                if (warp == 0 && c < j.width) {
+#pragma unroll
+                    for (int w = 1; w < (int)kWarps; w++)
+#pragma unroll
+                        for (int k = 0; k < N; k++) sum[k] += slice[w][lane * N + k];
+                    write_row<Out, N>(j, long_row[l], c, sum);
+                }
+                __syncthreads();
+            }
+        }
+        __syncthreads();
     }
 }
 
@@ -593,9 +675,15 @@ cudaError_t sum_pieces(const Job& j, const Space& s, int which, cudaStream_t st)
     while (log2 < 5 && (1u << log2) < pieces) log2++;
     const uint32_t teams_per_block = kReduceBlock >> log2;
     const dim3 grid((s.chunks + teams_per_block - 1) / teams_per_block, (pieces + (1u << log2) - 1) >> log2);
-    const uint32_t combine_blocks = s.chunks > 1 ? std::min<uint32_t>(s.chunks - 1, kCombineBlocksPerSm * current_sms()) : 0;
+    const uint32_t combine_blocks = s.chunks > 1 ? std::min<uint32_t>((s.chunks + kCombineBlock / 32 - 1) / (kCombineBlock / 32), 2 * current_sms()) : 0;
     const uint32_t clear_blocks = j.accumulate ? 0 : (uint32_t)(((uint64_t)j.total + kCombineBlock - 1) / kCombineBlock);
-    if (j.n) reduce_kernel<T, Out, N, PAIRS><<<grid, kReduceBlock, 0, st>>>(j, s, s.entry[which], log2);
+    if (j.n) {
+        static LaunchCache cache;
+        constexpr size_t smem = Ring<T, N, PAIRS>::smem;
+        const cudaError_t e = allow_smem(reduce_kernel<T, Out, N, PAIRS>, smem, cache);
+        if (e != cudaSuccess) return e;
+        reduce_kernel<T, Out, N, PAIRS><<<grid, kReduceBlock, smem, st>>>(j, s, s.entry[which], log2);
+    }
     if (combine_blocks + clear_blocks) combine_kernel<Out, (N < 4 ? N : 4)><<<combine_blocks + clear_blocks, kCombineBlock, 0, st>>>(j, s, s.entry[which], combine_blocks);
     return cudaGetLastError();
 }
