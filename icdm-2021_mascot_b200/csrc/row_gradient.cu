@@ -6,12 +6,14 @@
 // summed in that order, in fp32:
 //
 //   sort     least significant digit first, on (row, entry) pairs of 32 bits each.  All entries of both tables are sorted at once,
-//            the items' rows counted behind the users'.  Up to kSmall entries one block does all passes in shared
-//            memory; more take count / scan / scatter kernels for each digit.
+//            the items' rows counted behind the users'.  Up to kSmall entries one cluster of blocks does all passes;
+//            more take count / scan / scatter kernels for each digit.
 //   reduce   the sorted entries are cut into chunks of equal length, a team of lanes for each, so that a popular row is
 //            shared by many teams and many unpopular ones by one.  A row that ends less than a quarter of a chunk behind a chunk's
 //            end is finished by that chunk's team; of one that goes on further, each chunk's part is left in the workspace.
 //   combine  adds these parts up in the order of the chunks, and clears rows that no entry names.
+#include <cooperative_groups.h>
+
 #include <algorithm>
 #include <initializer_list>
 
@@ -21,13 +23,15 @@
 namespace mascot {
 namespace {
 
+namespace cg = cooperative_groups;
+
 constexpr int kSortBlock = 512, kSortWarps = kSortBlock / 32;
 constexpr int kFewItems = 4, kManyItems = 16;   // entries of a thread of the sort: a tile is 2048 or 8192
 constexpr uint32_t kManyFrom = 1u << 20;        // entries from which tiles are large: there are enough of them for all SMs then
 constexpr int kMaxBins = 1024;                  // digits of 8 or 10 bits
 constexpr uint32_t kScanTiles = 16;             // up to so many tiles the scatter kernel adds their counts up itself
 constexpr int kSmallBlock = 512, kSmallItems = 8, kSmallWarps = kSmallBlock / 32, kSmallBits = 8, kSmallBins = 1 << kSmallBits;
-constexpr uint32_t kSmall = kSmallBlock * kSmallItems;
+constexpr uint32_t kSmallCluster = 8, kSmall = kSmallBlock * kSmallItems * kSmallCluster;
 constexpr int kReduceBlock = 256, kCombineBlock = 512;
 
 // What is summed: where entries come from and what their values are.
@@ -58,6 +62,12 @@ struct Space {                                  // the workspace, see carve()
     uint8_t* touched;                           // a byte per row
     uint32_t pitch, chunks, tiles;
 };
+
+// For kernels that launch_behind launches, and those before them: the next kernel's blocks may be brought up; the kernel before has ended.
+__device__ __forceinline__ void follow() {
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+}
 
 // ---- sort --------------------------------------------------------------------------------------------------
 
@@ -151,20 +161,24 @@ __device__ __forceinline__ void begin_sums(const Job& j, const Space& s, size_t 
     if (!j.accumulate) for (size_t w = first; w < ((size_t)j.total + 15) / 16; w += step) reinterpret_cast<uint4*>(s.touched)[w] = make_uint4(0, 0, 0, 0);
 }
 
-// One block: entries stay in registers while they are ranked and go through shared memory to their next place.  A sort over
-// many blocks costs two launches a digit at least.
+// One cluster of eight blocks (one block for the fewest entries), a tile of entries each, that tell one another their counts through distributed shared memory and
+// meet twice a pass.  Passes of kernels of their own cost two launches each, about 3 us apiece, whatever there is to sort.
 __global__ void __launch_bounds__(kSmallBlock) small_sort_kernel(const Job j, const Space s, int passes) {
-    __shared__ uint2 at[kSmall];
+    __shared__ uint2 at[kSmallBlock * kSmallItems];
     __shared__ __align__(16) uint16_t count[kSmallWarps * kSmallBins];
-    __shared__ uint32_t start[kSmallBins], warp_sums[32];
+    __shared__ uint32_t counts[kSmallBins], start[kSmallBins], base[kSmallBins], warp_sums[32];
+    follow();
+    cg::cluster_group cluster = cg::this_cluster();
+    const uint32_t blocks = cluster.num_blocks(), block = cluster.block_rank();
     const int t = threadIdx.x, lane = t & 31, warp = t >> 5;
-    begin_sums(j, s, t, kSmallBlock);
-    const uint32_t rounds = (j.n + kSmallBlock - 1) / kSmallBlock, first = warp * rounds * 32 + lane;      // a warp's entries, in order
-    bool bad = false;
+    begin_sums(j, s, block * kSmallBlock + t, blocks * kSmallBlock);
+    const uint32_t rounds = (j.n + blocks * kSmallBlock - 1) / (blocks * kSmallBlock), tile0 = block * rounds * kSmallBlock;
+    const uint32_t here = j.n > tile0 ? min(rounds * kSmallBlock, j.n - tile0) : 0, mine0 = warp * rounds * 32 + lane;      // a warp's entries, in order
     uint32_t key[kSmallItems], val[kSmallItems];
-    entry_keys<kSmallItems>(j, s, first, 32, key, bad);
+    bool bad = false;
+    entry_keys<kSmallItems>(j, s, tile0 + mine0, 32, key, bad);
 #pragma unroll
-    for (int k = 0; k < kSmallItems; k++) val[k] = first + k * 32;
+    for (int k = 0; k < kSmallItems; k++) val[k] = tile0 + mine0 + k * 32;
     if (bad && j.flags) atomicOr(j.flags, (uint32_t)MASCOT_FLAG_BAD_ID);
     uint16_t* const mine = count + warp * kSmallBins;
     for (int p = 0; p < passes; p++) {
@@ -174,32 +188,44 @@ __global__ void __launch_bounds__(kSmallBlock) small_sort_kernel(const Job j, co
         uint32_t rank[kSmallItems];
 #pragma unroll
         for (int k = 0; k < kSmallItems; k++)
-            if (k < rounds) rank[k] = warp_rank<kSmallBits>(key[k] >> shift & (kSmallBins - 1), first + k * 32 < j.n, mine, lane);
+            if (k < rounds) rank[k] = warp_rank<kSmallBits>(key[k] >> shift & (kSmallBins - 1), mine0 + k * 32 < here, mine, lane);
         __syncthreads();
         if (t < kSmallBins / 2) {
             const uint32_t sums = warp_offsets(count, kSmallWarps, kSmallBins, t);
-            start[2 * t] = sums & 0xffff;
-            start[2 * t + 1] = sums >> 16;
+            counts[2 * t] = start[2 * t] = sums & 0xffff;
+            counts[2 * t + 1] = start[2 * t + 1] = sums >> 16;
+        }
+        cluster.sync();
+        uint32_t within = 0;                                    // entries of the bin in the tiles before
+        if (t < kSmallBins) {
+            uint32_t sum = 0;
+            for (uint32_t b = 0; b < blocks; b++) { if (b == block) within = sum; sum += *cluster.map_shared_rank(&counts[t], b); }
+            base[t] = sum;
         }
         __syncthreads();
         block_scan(start, kSmallBins, warp_sums);
+        block_scan(base, kSmallBins, warp_sums);
+        if (t < kSmallBins) base[t] += within - start[t];
 #pragma unroll
         for (int k = 0; k < kSmallItems; k++)
-            if (k < rounds && first + k * 32 < j.n) { const uint32_t d = key[k] >> shift & (kSmallBins - 1); at[start[d] + mine[d] + rank[k]] = make_uint2(key[k], val[k]); }
+            if (k < rounds && mine0 + k * 32 < here) { const uint32_t d = key[k] >> shift & (kSmallBins - 1); at[start[d] + mine[d] + rank[k]] = make_uint2(key[k], val[k]); }
         __syncthreads();
+        uint2* const to = s.entry[p & 1];
+        for (uint32_t i = t; i < here; i += kSmallBlock) { const uint2 x = at[i]; to[i + base[x.x >> shift & (kSmallBins - 1)]] = x; }
+        cluster.sync();                                         // also before a block leaves whose counts another one may read
         if (p + 1 < passes) {
 #pragma unroll
-            for (int k = 0; k < kSmallItems; k++) if (k < rounds && first + k * 32 < j.n) { key[k] = at[first + k * 32].x; val[k] = at[first + k * 32].y; }
-            // `at` is written again only behind the next pass's barriers
+            for (int k = 0; k < kSmallItems; k++)
+                if (k < rounds && mine0 + k * 32 < here) { const uint2 x = __ldcg(to + tile0 + mine0 + k * 32); key[k] = x.x; val[k] = x.y; }
         }
     }
-    for (uint32_t i = t; i < j.n; i += kSmallBlock) s.entry[0][i] = at[i];
 }
 
 // Counts of the digits of a tile, [tile][bin].  The first pass makes the keys, and keeps them.
 template <bool FIRST, int ITEMS>
 __global__ void __launch_bounds__(kSortBlock) count_kernel(const Job j, const Space s, const uint2* entry, int shift, int bits) {
     __shared__ uint32_t hist[kMaxBins];
+    follow();
     const int bins = 1 << bits;
     for (int b = threadIdx.x; b < bins; b += kSortBlock) hist[b] = 0;
     if (FIRST) begin_sums(j, s, (size_t)blockIdx.x * kSortBlock + threadIdx.x, (size_t)gridDim.x * kSortBlock);
@@ -235,6 +261,7 @@ __global__ void __launch_bounds__(kSortBlock) count_kernel(const Job j, const Sp
 // A block for 32 bins, a warp for a run of tiles: counts of the tiles become offsets within the bin, the sums go to totals.
 __global__ void __launch_bounds__(1024) scan_kernel(const Space s, int bins) {
     __shared__ uint32_t sums[32][32];
+    follow();
     const uint32_t lane = threadIdx.x & 31, warp = threadIdx.x >> 5, bin = blockIdx.x * 32 + lane;
     const uint32_t per = (s.tiles + 31) / 32, t0 = min(s.tiles, warp * per), t1 = min(s.tiles, t0 + per);
     uint32_t sum = 0;
@@ -262,6 +289,7 @@ template <bool FIRST, int ITEMS, int BITS>
 __global__ void __launch_bounds__(kSortBlock, 2) scatter_kernel(const Space s, uint32_t n, const uint2* from, uint2* to, int shift, bool scanned) {
     extern __shared__ uint2 at[];                               // entries in their order; the warps' counters; the bins' offsets
     __shared__ uint32_t warp_sums[32];
+    follow();
     const int t = threadIdx.x, lane = t & 31, warp = t >> 5;
     constexpr int bins = 1 << BITS, kTile = ITEMS * kSortBlock, kPer = (bins + kSortBlock - 1) / kSortBlock;
     uint16_t* const count = reinterpret_cast<uint16_t*>(at + kTile), *const mine = count + (warp << BITS);
@@ -319,7 +347,7 @@ __global__ void __launch_bounds__(kSortBlock, 2) scatter_kernel(const Space s, u
 template <typename Out, int N>
 __device__ __forceinline__ void write_row(const Job& j, uint32_t row, uint32_t col, const float (&sum)[N]) {
     const bool second = row >= j.rows[0];
-    Out* const at = static_cast<Out*>(j.out[second]) + (size_t)(second ? row - j.rows[0] : row) * j.out_stride[second] + col;
+    Out* const at = static_cast<Out*>(second ? j.out[1] : j.out[0]) + (size_t)(second ? row - j.rows[0] : row) * (second ? j.out_stride[1] : j.out_stride[0]) + col;
     Piece<Out, N> r;
     if (j.accumulate) {
         r = *reinterpret_cast<const Piece<Out, N>*>(at);
@@ -332,25 +360,28 @@ __device__ __forceinline__ void write_row(const Job& j, uint32_t row, uint32_t c
     store_piece<Out, N>(at, r);
 }
 
-// What an entry adds: c * (row a - row b), without b where that is kNoRow; nothing where a is.
-struct Term { uint32_t key, a, b; float c; };
+// What an entry adds: c * (row a - row b), as far as it has these rows.
+struct Term { uint32_t key, a, b; float c; bool has_a, has_b; };
 template <bool PAIRS> __device__ __forceinline__ Term term_of(const Job& j, uint2 entry, uint4 pair) {
-    Term t{entry.x, entry.y, kNoRow, 1.f};
+    Term t{entry.x, entry.y, 0, 1.f, entry.x < j.total, false};
     if (PAIRS) {
         const uint32_t kind = entry.y % 3;
         t.a = kind ? pair.x : pair.y;
-        if (kind == 0) t.b = pair.z;
+        t.b = pair.z;
         t.c = kind == 2 ? -__uint_as_float(pair.w) : __uint_as_float(pair.w);
-        if (t.c == 0.f) t.a = kNoRow;                           // whatever the rows hold
+        t.has_a = t.has_a && t.c != 0.f;                        // coef 0: whatever the rows hold
+        t.has_b = t.has_a && kind == 0;
     }
-    if (entry.x >= j.total) t.a = kNoRow;
+    if (!t.has_a) { t.a = 0; t.c = 0.f; }
+    if (!t.has_b) t.b = 0;
     return t;
 }
 
 // 4, 8 or 16 bytes on their way to shared memory; rows of a table stay in L1 (popular ones come again), gradient rows do not.
-template <int BYTES, bool KEEP> __device__ __forceinline__ void fetch_piece(uint32_t to, const void* from) {
-    if constexpr (BYTES == 16 && !KEEP) asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(to), "l"(from) : "memory");
-    else asm volatile("cp.async.ca.shared.global [%0], [%1], %2;" ::"r"(to), "l"(from), "n"(BYTES) : "memory");
+// Zeros instead where it is not there: nothing is read then.
+template <int BYTES, bool KEEP> __device__ __forceinline__ void fetch_piece(uint32_t to, const void* from, bool there) {
+    if constexpr (BYTES == 16 && !KEEP) asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to), "l"(from), "r"(there ? 16 : 0) : "memory");
+    else asm volatile("cp.async.ca.shared.global [%0], [%1], %2, %3;" ::"r"(to), "l"(from), "n"(BYTES), "r"(there ? BYTES : 0) : "memory");
 }
 
 // A team's lanes take a group of entries each and hand their rows round; what a lane can work out for a group (where rows begin, which
@@ -368,6 +399,7 @@ __global__ void __launch_bounds__(kReduceBlock, 3) reduce_kernel(const Job j, co
     using R = Ring<T, N, PAIRS>;
     constexpr int BATCH = 4;
     extern __shared__ __align__(16) uint8_t ring[];             // [ahead][sides][threads]
+    follow();
     const uint32_t team = 1u << team_log2, lane = threadIdx.x & 31, tl = lane & (team - 1), team_at = lane & ~(team - 1), ahead = min(team, (uint32_t)R::ahead);
     const uint32_t team_mask = (team == 32 ? 0xffffffffu : (1u << team) - 1) << team_at;
     const uint32_t chunk = (blockIdx.x * kReduceBlock + threadIdx.x) >> team_log2, col = ((blockIdx.y << team_log2) + tl) * N;
@@ -405,16 +437,13 @@ __global__ void __launch_bounds__(kReduceBlock, 3) reduce_kernel(const Job j, co
     const auto pair_of = [&](uint2 e) { return PAIRS && e.x < j.total ? __ldg(s.pair + e.y / 3) : make_uint4(0, 0, 0, 0); };
     const auto ballot = [&](bool b) { return __ballot_sync(0xffffffffu, b) >> team_at; };
     // rows of the entries k .. k + 3 of a group
-    const auto fetch = [&](const Term& t, uint32_t adds, uint32_t twos, uint32_t k0) {
+    const auto fetch = [&](const Term& t, uint32_t adds, uint32_t twos, bool some, uint32_t k0) {      // some: a team of the warp has second rows
 #pragma unroll
         for (int k = 0; k < BATCH; k++) {
-            const uint32_t ra = __shfl_sync(0xffffffffu, t.a, k0 + k, team), rb = PAIRS ? __shfl_sync(0xffffffffu, t.b, k0 + k, team) : kNoRow;
-            if ((adds >> (k0 + k) & 1) && writes) {
-                const uint32_t to = mine_to + ((k0 + k) & (ahead - 1)) * (R::sides * kReduceBlock * R::piece);
-                const bool two = PAIRS && (twos >> (k0 + k) & 1);
-                fetch_piece<R::piece, PAIRS>(to, two ? src1 + ra * stride1 : src0 + ra * stride0);
-                if (PAIRS && two) fetch_piece<R::piece, PAIRS>(to + kReduceBlock * R::piece, src1 + rb * stride1);
-            }
+            const uint32_t ra = __shfl_sync(0xffffffffu, t.a, k0 + k, team), to = mine_to + ((k0 + k) & (ahead - 1)) * (R::sides * kReduceBlock * R::piece);
+            const bool one = (adds >> (k0 + k) & 1) && writes, two = PAIRS && (twos >> (k0 + k) & 1);
+            fetch_piece<R::piece, PAIRS>(to, two ? src1 + ra * stride1 : src0 + ra * stride0, one);
+            if (PAIRS && some) fetch_piece<R::piece, PAIRS>(to + kReduceBlock * R::piece, src1 + __shfl_sync(0xffffffffu, t.b, k0 + k, team) * stride1, two && writes);
         }
         asm volatile("cp.async.commit_group;" ::: "memory");
     };
@@ -422,11 +451,14 @@ __global__ void __launch_bounds__(kReduceBlock, 3) reduce_kernel(const Job j, co
     const uint2 e0 = entry_at(begin + tl), e1 = entry_at(begin + team + tl);
     Term now = term_of<PAIRS>(j, e0, pair_of(e0)), next = term_of<PAIRS>(j, e1, pair_of(e1));
     uint4 pair = pair_of(after);
-    uint32_t adds = ballot(now.a != kNoRow), twos = PAIRS ? ballot(now.b != kNoRow) : 0u;
-    if constexpr (N > 1) for (uint32_t k0 = 0; k0 < ahead; k0 += BATCH) fetch(now, adds, twos, k0);
+    const auto any = [](uint32_t mask) { return __any_sync(0xffffffffu, mask != 0); };
+    uint32_t adds = ballot(now.has_a), twos = PAIRS ? ballot(now.has_b) : 0u;
+    bool some = PAIRS && any(twos);                             // seldom both: users' rows are sorted before items'
+    if constexpr (N > 1) for (uint32_t k0 = 0; k0 < ahead; k0 += BATCH) fetch(now, adds, twos, some, k0);
     for (uint32_t g = begin; __any_sync(0xffffffffu, g < until); g += team) {
         const uint32_t left = __shfl_up_sync(0xffffffffu, now.key, 1, team), begins = ballot(now.key != (tl ? left : row));
-        const uint32_t next_adds = ballot(next.a != kNoRow), next_twos = PAIRS ? ballot(next.b != kNoRow) : 0u;
+        const uint32_t next_adds = ballot(next.has_a), next_twos = PAIRS ? ballot(next.has_b) : 0u;
+        const bool next_some = PAIRS && any(next_twos);
         for (uint32_t k0 = 0; k0 < team; k0 += BATCH) {
             if (!__any_sync(0xffffffffu, g + k0 < until)) break;
             Piece<T, N> a[BATCH], b[PAIRS ? BATCH : 1];
@@ -441,14 +473,14 @@ __global__ void __launch_bounds__(kReduceBlock, 3) reduce_kernel(const Job j, co
                 if constexpr (N > 1) {
                     const uint8_t* const at = mine_at + ((k0 + k) & (ahead - 1)) * (R::sides * kReduceBlock * R::piece);
                     a[k] = *reinterpret_cast<const Piece<T, N>*>(at);
-                    if (PAIRS) b[k] = *reinterpret_cast<const Piece<T, N>*>(at + kReduceBlock * R::piece);
+                    if (PAIRS && some) b[k] = *reinterpret_cast<const Piece<T, N>*>(at + kReduceBlock * R::piece);
                 } else {
-                    const uint32_t ra = __shfl_sync(0xffffffffu, now.a, k0 + k, team), rb = PAIRS ? __shfl_sync(0xffffffffu, now.b, k0 + k, team) : kNoRow;
-                    const bool two = PAIRS && (twos >> (k0 + k) & 1);
-                    if ((adds >> (k0 + k) & 1) && writes) {
-                        a[k] = load_piece<T, N>(two ? src1 + ra * stride1 : src0 + ra * stride0);
-                        if (PAIRS && two) b[k] = load_piece<T, N>(src1 + rb * stride1);
-                    }
+                    const uint32_t ra = __shfl_sync(0xffffffffu, now.a, k0 + k, team), rb = PAIRS ? __shfl_sync(0xffffffffu, now.b, k0 + k, team) : 0u;
+                    const bool one = (adds >> (k0 + k) & 1) && writes, two = PAIRS && (twos >> (k0 + k) & 1);
+                    a[k].v[0] = from_float<T>(0.f);
+                    if (PAIRS) b[k].v[0] = from_float<T>(0.f);
+                    if (one) a[k] = load_piece<T, N>(two ? src1 + ra * stride1 : src0 + ra * stride0);
+                    if (PAIRS && two && writes) b[k] = load_piece<T, N>(src1 + rb * stride1);
                 }
             }
 #pragma unroll
@@ -459,25 +491,28 @@ __global__ void __launch_bounds__(kReduceBlock, 3) reduce_kernel(const Job j, co
 #pragma unroll
                     for (int x = 0; x < N; x++) sum[x] = 0.f;
                 }
-                if (adds >> (k0 + k) & 1) {
-                    const bool two = PAIRS && (twos >> (k0 + k) & 1);
+                if (!PAIRS) {
 #pragma unroll
-                    for (int x = 0; x < N; x++) {
-                        if (!PAIRS) sum[x] += as_float(a[k].v[x]);
-                        else sum[x] = fmaf(c[k], two ? as_float(a[k].v[x]) - as_float(b[k].v[x]) : as_float(a[k].v[x]), sum[x]);
-                    }
+                    for (int x = 0; x < N; x++) sum[x] += as_float(a[k].v[x]);
+                } else if (some) {
+#pragma unroll
+                    for (int x = 0; x < N; x++) sum[x] = fmaf(c[k], as_float(a[k].v[x]) - as_float(b[k].v[x]), sum[x]);
+                } else {
+#pragma unroll
+                    for (int x = 0; x < N; x++) sum[x] = fmaf(c[k], as_float(a[k].v[x]), sum[x]);
                 }
             }
             __syncwarp();
             if constexpr (N > 1) {                              // into the places that have just been read
                 const uint32_t k1 = k0 + ahead;
-                if (k1 < team) fetch(now, adds, twos, k1);
-                else fetch(next, next_adds, next_twos, k1 - team);
+                if (k1 < team) fetch(now, adds, twos, some, k1);
+                else fetch(next, next_adds, next_twos, next_some, k1 - team);
             }
         }
         now = next;
         adds = next_adds;
         twos = next_twos;
+        some = next_some;
         next = term_of<PAIRS>(j, after, pair);
         after = entry_at(g + 3 * team + tl);
         pair = pair_of(after);
@@ -511,6 +546,7 @@ template <int N> __device__ __forceinline__ void add_parts(const Space& s, uint3
 template <typename Out, int N>
 __global__ void __launch_bounds__(kCombineBlock, 2) combine_kernel(const Job j, const Space s, const uint2* entry, uint32_t combine_blocks) {
     constexpr uint32_t kWarps = kCombineBlock / 32;
+    follow();
     const uint32_t lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     if (blockIdx.x >= combine_blocks) {
         const uint32_t row0 = (blockIdx.x - combine_blocks) * kCombineBlock + warp * 32;
@@ -520,7 +556,7 @@ __global__ void __launch_bounds__(kCombineBlock, 2) combine_kernel(const Job j, 
             const uint32_t r = row0 + __ffs(todo) - 1;
             todo &= todo - 1;
             const bool second = r >= j.rows[0];
-            Out* const at = static_cast<Out*>(j.out[second]) + (size_t)(second ? r - j.rows[0] : r) * j.out_stride[second];
+            Out* const at = static_cast<Out*>(second ? j.out[1] : j.out[0]) + (size_t)(second ? r - j.rows[0] : r) * (second ? j.out_stride[1] : j.out_stride[0]);
             for (uint32_t c = lane * N; c < j.width; c += 32 * N) {
                 Piece<Out, N> zero;
 #pragma unroll
@@ -605,7 +641,7 @@ size_t carve(uint64_t n, uint64_t total, uint32_t width, bool pairs, char* base,
         sp.pitch = (width + 3) / 4 * 4;
         const bool small = n <= kSmall;
         sp.entry[0] = reinterpret_cast<uint2*>(take(8 * n));
-        sp.entry[1] = reinterpret_cast<uint2*>(take(small ? 0 : 8 * n));
+        sp.entry[1] = reinterpret_cast<uint2*>(take(8 * n));
         sp.key = reinterpret_cast<uint32_t*>(take(small ? 0 : 4 * n));
         sp.counts = reinterpret_cast<uint32_t*>(take(small ? 0 : 4 * (size_t)sp.tiles * kMaxBins));
         sp.totals = reinterpret_cast<uint32_t*>(take(small ? 0 : 4 * kMaxBins));
@@ -618,6 +654,23 @@ size_t carve(uint64_t n, uint64_t total, uint32_t width, bool pairs, char* base,
     }
     if (s) *s = sp;
     return at;
+}
+
+// Launches a kernel behind the first of a call: its blocks are brought up while the kernel before still runs, and wait for its end and
+// its results in follow(), the first thing that they do.  A launch less to wait for is 1 to 1.5 us.
+template <class Kernel, class... Args>
+cudaError_t launch_behind(Kernel kernel, dim3 grid, unsigned block, size_t smem, cudaStream_t st, Args... args) {
+    cudaLaunchConfig_t config = {};
+    config.gridDim = grid;
+    config.blockDim = dim3(block);
+    config.dynamicSmemBytes = smem;
+    config.stream = st;
+    cudaLaunchAttribute behind[1];
+    behind[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    behind[0].val.programmaticStreamSerializationAllowed = 1;
+    config.attrs = behind;
+    config.numAttrs = 1;
+    return cudaLaunchKernelEx(&config, kernel, args...);
 }
 
 // Raises a kernel's limit of dynamic shared memory, once for a device.
@@ -641,21 +694,33 @@ cudaError_t sort_digit(const Job& j, const Space& s, int pass, cudaStream_t st) 
     if (e != cudaSuccess) return e;
     const bool scanned = s.tiles > kScanTiles;
     uint2* const from = s.entry[pass & 1], *const to = s.entry[~pass & 1];
-    if (pass == 0) count_kernel<true, ITEMS><<<s.tiles, kSortBlock, 0, st>>>(j, s, nullptr, 0, BITS);
-    else count_kernel<false, ITEMS><<<s.tiles, kSortBlock, 0, st>>>(j, s, from, pass * BITS, BITS);
-    if (scanned) scan_kernel<<<bins / 32, 1024, 0, st>>>(s, bins);
-    if (pass == 0) scatter_kernel<true, ITEMS, BITS><<<s.tiles, kSortBlock, smem, st>>>(s, j.n, nullptr, to, 0, scanned);
-    else scatter_kernel<false, ITEMS, BITS><<<s.tiles, kSortBlock, smem, st>>>(s, j.n, from, to, pass * BITS, scanned);
-    return cudaGetLastError();
+    const uint2* const none = nullptr;
+    if (pass == 0) count_kernel<true, ITEMS><<<s.tiles, kSortBlock, 0, st>>>(j, s, none, 0, BITS);
+    else e = launch_behind(count_kernel<false, ITEMS>, s.tiles, kSortBlock, 0, st, j, s, (const uint2*)from, pass * BITS, BITS);
+    if (e == cudaSuccess && scanned) e = launch_behind(scan_kernel, bins / 32, 1024, 0, st, s, bins);
+    if (e == cudaSuccess && pass == 0) e = launch_behind(scatter_kernel<true, ITEMS, BITS>, s.tiles, kSortBlock, smem, st, s, j.n, none, to, 0, scanned);
+    else if (e == cudaSuccess) e = launch_behind(scatter_kernel<false, ITEMS, BITS>, s.tiles, kSortBlock, smem, st, s, j.n, (const uint2*)from, to, pass * BITS, scanned);
+    return e == cudaSuccess ? cudaGetLastError() : e;
 }
 
 // Sorts the entries; *which tells which of the two buffers holds them.
 cudaError_t sort_entries(const Job& j, const Space& s, int* which, cudaStream_t st) {
     const int key_bits = bits_for((uint64_t)j.total + 1);
     if (j.n <= kSmall) {
-        small_sort_kernel<<<1, kSmallBlock, 0, st>>>(j, s, (key_bits + kSmallBits - 1) / kSmallBits);
-        *which = 0;
-        return cudaGetLastError();
+        const int passes = (key_bits + kSmallBits - 1) / kSmallBits;
+        const uint32_t blocks = j.n > kSmallBlock ? kSmallCluster : 1;
+        cudaLaunchConfig_t config = {};
+        config.gridDim = dim3(blocks);
+        config.blockDim = dim3(kSmallBlock);
+        config.stream = st;
+        cudaLaunchAttribute cluster[1];
+        cluster[0].id = cudaLaunchAttributeClusterDimension;
+        cluster[0].val.clusterDim.x = blocks;
+        cluster[0].val.clusterDim.y = cluster[0].val.clusterDim.z = 1;
+        config.attrs = cluster;
+        config.numAttrs = 1;
+        *which = (passes - 1) & 1;
+        return cudaLaunchKernelEx(&config, small_sort_kernel, j, s, passes);
     }
     const bool ten = (key_bits + 9) / 10 < (key_bits + 7) / 8, many = j.n >= kManyFrom;      // wider digits where they save a pass
     const int passes = ten ? (key_bits + 9) / 10 : (key_bits + 7) / 8;
@@ -680,11 +745,13 @@ cudaError_t sum_pieces(const Job& j, const Space& s, int which, cudaStream_t st)
     if (j.n) {
         static LaunchCache cache;
         constexpr size_t smem = Ring<T, N, PAIRS>::smem;
-        const cudaError_t e = allow_smem(reduce_kernel<T, Out, N, PAIRS>, smem, cache);
+        cudaError_t e = allow_smem(reduce_kernel<T, Out, N, PAIRS>, smem, cache);
         if (e != cudaSuccess) return e;
-        reduce_kernel<T, Out, N, PAIRS><<<grid, kReduceBlock, smem, st>>>(j, s, s.entry[which], log2);
-    }
-    if (combine_blocks + clear_blocks) combine_kernel<Out, (N < 4 ? N : 4)><<<combine_blocks + clear_blocks, kCombineBlock, 0, st>>>(j, s, s.entry[which], combine_blocks);
+        e = launch_behind(reduce_kernel<T, Out, N, PAIRS>, grid, kReduceBlock, smem, st, j, s, (const uint2*)s.entry[which], log2);
+        if (e == cudaSuccess && combine_blocks + clear_blocks)
+            e = launch_behind(combine_kernel<Out, (N < 4 ? N : 4)>, combine_blocks + clear_blocks, kCombineBlock, 0, st, j, s, (const uint2*)s.entry[which], combine_blocks);
+        if (e != cudaSuccess) return e;
+    } else if (clear_blocks) combine_kernel<Out, (N < 4 ? N : 4)><<<clear_blocks, kCombineBlock, 0, st>>>(j, s, static_cast<const uint2*>(nullptr), 0u);
     return cudaGetLastError();
 }
 

@@ -434,6 +434,9 @@ class _Ops:
         self.torch = torch
         self.types = {torch.float32: F32, torch.float16: F16, torch.bfloat16: BF16, torch.float8_e4m3fn: E4M3}
         self.bits = {torch.int32: 32, torch.int64: 64}
+        # the raw handle where torch offers it: the stream object around it costs 2 us a call
+        raw = getattr(torch._C, "_cuda_getCurrentRawStream", None)
+        self.stream = raw or (lambda index: torch.cuda.current_stream(index).cuda_stream)
 
 
 def _torch_ops():
@@ -497,13 +500,13 @@ def _device_of(what, t):
 
 def _call(device, name, *args):
     """A call on `device`, on torch's current stream there."""
-    cuda = _torch_ops().torch.cuda
-    f = getattr(load(), name)
+    ops = _torch_ops()
+    cuda, f = ops.torch.cuda, getattr(load(), name)
     if cuda.current_device() == device.index:
-        rc = f(*args, cuda.current_stream(device).cuda_stream)
+        rc = f(*args, ops.stream(device.index))
     else:
         with cuda.device(device):
-            rc = f(*args, cuda.current_stream(device).cuda_stream)
+            rc = f(*args, ops.stream(device.index))
     if rc != OK:
         raise MascotError(rc, load().mascot_last_error(None).decode())
 
