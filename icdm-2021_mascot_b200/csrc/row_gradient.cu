@@ -58,7 +58,8 @@ struct Space {                                  // the workspace, see carve()
     uint2* entry[2];                            // (row, entry)
     uint4* pair;                                // user, preferred, other, bits of coef
     float *head, *tail;                         // [chunks][pitch]
-    uint32_t *owners, *n_owners;                // chunks where a row begins whose parts are added up
+    uint2* owners;                              // (chunk, row) where a row begins whose parts are added up
+    uint32_t* n_owners;
     uint8_t* touched;                           // a byte per row
     uint32_t pitch, chunks, tiles;
 };
@@ -424,7 +425,7 @@ __global__ void __launch_bounds__(kReduceBlock, 3) reduce_kernel(const Job j, co
             float* const part = (from_before ? s.head : s.tail) + (size_t)chunk * s.pitch + col;
 #pragma unroll
             for (int k = 0; k < N; k++) part[k] = sum[k];
-            if (!from_before && col == 0) s.owners[atomicAdd(s.n_owners, 1u)] = chunk;
+            if (!from_before && col == 0) s.owners[atomicAdd(s.n_owners, 1u)] = make_uint2(chunk, row);
         } else write_row<Out, N>(j, row, col, sum);
         if (!from_before && !j.accumulate && col == 0) s.touched[row] = 1;
     };
@@ -472,8 +473,8 @@ __global__ void __launch_bounds__(kReduceBlock, 3) reduce_kernel(const Job j, co
                 c[k] = PAIRS ? __shfl_sync(0xffffffffu, now.c, k0 + k, team) : 1.f;
                 if constexpr (N > 1) {
                     const uint8_t* const at = mine_at + ((k0 + k) & (ahead - 1)) * (R::sides * kReduceBlock * R::piece);
-                    a[k] = *reinterpret_cast<const Piece<T, N>*>(at);
-                    if (PAIRS && some) b[k] = *reinterpret_cast<const Piece<T, N>*>(at + kReduceBlock * R::piece);
+                    a[k] = shared_piece<T, N>(at);
+                    if (PAIRS && some) b[k] = shared_piece<T, N>(at + kReduceBlock * R::piece);
                 } else {
                     const uint32_t ra = __shfl_sync(0xffffffffu, now.a, k0 + k, team), rb = PAIRS ? __shfl_sync(0xffffffffu, now.b, k0 + k, team) : 0u;
                     const bool one = (adds >> (k0 + k) & 1) && writes, two = PAIRS && (twos >> (k0 + k) & 1);
@@ -573,7 +574,8 @@ __global__ void __launch_bounds__(kCombineBlock, 2) combine_kernel(const Job j, 
         if (threadIdx.x == 0) n_long = 0;
         __syncthreads();
         if (o0 + warp < owners) {
-            const uint32_t chunk = s.owners[o0 + warp], first = (chunk + 1) << j.chunk_log2, row = __ldg(&entry[first].x);
+            const uint2 owner = s.owners[o0 + warp];
+            const uint32_t chunk = owner.x, row = owner.y, first = (chunk + 1) << j.chunk_log2;
             // Chunks that follow with a part of the row.  Most rows end soon: lane q looks whether the row goes on in parts behind q chunks more.
             const uint64_t at = (uint64_t)first + (uint64_t)lane * size + size / 4;
             const uint32_t through = __ballot_sync(0xffffffffu, at < j.n && __ldg(&entry[at].x) == row);
@@ -648,7 +650,7 @@ size_t carve(uint64_t n, uint64_t total, uint32_t width, bool pairs, char* base,
         sp.pair = reinterpret_cast<uint4*>(take(pairs ? 16 * (n / 3) : 0));
         sp.head = reinterpret_cast<float*>(take(4 * (size_t)sp.chunks * sp.pitch));
         sp.tail = reinterpret_cast<float*>(take(4 * (size_t)sp.chunks * sp.pitch));
-        sp.owners = reinterpret_cast<uint32_t*>(take(4 * (size_t)sp.chunks));
+        sp.owners = reinterpret_cast<uint2*>(take(8 * (size_t)sp.chunks));
         sp.n_owners = reinterpret_cast<uint32_t*>(take(4));
         sp.touched = reinterpret_cast<uint8_t*>(take(total));
     }

@@ -261,24 +261,19 @@ cudaError_t launch_pair_loss(const PairArgs& a, bool aligned, cudaStream_t st) {
 // ---- quantisation ------------------------------------------------------------------------------------------
 // One pass over the rows: a block stays in registers between its maximum and its rounding.  A power of two as the scale
 // makes x / s exact, so that the only rounding is the one to four significant bits, and costs no precision: what
-// the larger scale takes from the range is at its lower end, below 2^-14 of the block's maximum.
-constexpr int kQuantBlock = 256;
+// the larger scale takes from the range is at its lower end, below 2^-14 of the block's maximum.  What bounds it is the
+// rows; a warp has those of four blocks (sixteen of a square) under way at once, since one alone leaves HBM idle (107 us for
+// 625k rows of 128 floats, 402 MB).
+constexpr int kQuantBlock = 256, kQuantWarps = kQuantBlock / 32, kQuantRows = 4;
 
 // The scale of a block from the bits of its largest finite magnitude: 448 = 1.75 * 2^8.
 __device__ __forceinline__ float scale_of(uint32_t top) {
     if (top == 0) return 1.f;
-    int e = (int)(top >> 23) - 127 - 8 + ((top & 0x7fffffu) > 0x600000u ? 1 : 0);
-    e = max(e, -126);
-    return __uint_as_float((uint32_t)(e + 127) << 23);
+    const int e = (int)(top >> 23) - 127 - 8 + ((top & 0x7fffffu) > 0x600000u ? 1 : 0);
+    return __uint_as_float((uint32_t)(max(e, -126) + 127) << 23);
 }
-__device__ __forceinline__ uint32_t finite_bits(float x) {
-    const uint32_t b = __float_as_uint(x) & 0x7fffffffu;
-    return b < 0x7f800000u ? b : 0u;
-}
-__device__ __forceinline__ uint8_t to_e4m3(float x, float inverse) {
-    const uint8_t q = __nv_cvt_float_to_fp8(x * inverse, __NV_SATFINITE, __NV_E4M3);
-    return (__float_as_uint(x) & 0x7f800000u) == 0x7f800000u ? 0x7fu : q;
-}
+constexpr uint32_t kInfinity = 0x7f800000u;
+__device__ __forceinline__ uint32_t magnitude(float x) { return __float_as_uint(x) & 0x7fffffffu; }
 
 struct QuantArgs {
     const void* x; uint8_t* q; float* scale;
@@ -286,85 +281,94 @@ struct QuantArgs {
     uint32_t rows, width, padded, row_blocks;       // padded: columns of q that are written
 };
 
-// A warp per row and column block, four elements a lane.
-template <typename T, bool ALIGNED>
-__global__ void __launch_bounds__(kQuantBlock) quantize_rows_kernel(const QuantArgs a, uint32_t col_blocks) {
-    const size_t unit = ((size_t)blockIdx.x * kQuantBlock + threadIdx.x) >> 5;
-    const uint32_t lane = threadIdx.x & 31;
-    if (unit >= (size_t)a.rows * col_blocks) return;
-    const uint32_t row = (uint32_t)(unit / col_blocks), cb = (uint32_t)(unit % col_blocks), c = cb * kScaleBlock + lane * 4;
-    const T* const x = static_cast<const T*>(a.x) + row * a.x_stride;
-    float v[4];
+// Four elements of a row from column c on, zeros behind its end.
+template <typename T, bool ALIGNED> __device__ __forceinline__ float4 load_four(const T* x, uint32_t c, uint32_t width) {
+    float v[4] = {};
     if (ALIGNED) {
-        Piece<T, 4> in = {};
-        if (c < a.width) in = load_piece<T, 4>(x + c);
+        if (c < width) {
+            const Piece<T, 4> in = load_piece<T, 4>(x + c);
 #pragma unroll
-        for (int k = 0; k < 4; k++) v[k] = c < a.width ? as_float(in.v[k]) : 0.f;
+            for (int k = 0; k < 4; k++) v[k] = as_float(in.v[k]);
+        }
     } else {
 #pragma unroll
-        for (int k = 0; k < 4; k++) v[k] = c + k < a.width ? as_float(__ldg(x + c + k)) : 0.f;
+        for (int k = 0; k < 4; k++) if (c + k < width) v[k] = as_float(load_piece<T, 1>(x + c + k).v[0]);
     }
-    uint32_t top = max(max(finite_bits(v[0]), finite_bits(v[1])), max(finite_bits(v[2]), finite_bits(v[3])));
-    top = __reduce_max_sync(0xffffffffu, top);
-    const float s = scale_of(top), inverse = __uint_as_float(0x7f000000u - __float_as_uint(s));
-    uint8_t* const q = a.q + row * a.q_stride;
-    uint8_t out[4];
-#pragma unroll
-    for (int k = 0; k < 4; k++) out[k] = to_e4m3(v[k], inverse);
-    if (ALIGNED) {
-        if (c < a.padded) *reinterpret_cast<uint32_t*>(q + c) = out[0] | out[1] << 8 | out[2] << 16 | (uint32_t)out[3] << 24;
-    } else {
-#pragma unroll
-        for (int k = 0; k < 4; k++) if (c + k < a.padded) q[c + k] = out[k];
+    return make_float4(v[0], v[1], v[2], v[3]);
+}
+// The largest magnitude among them, and `odd` set where one of them is no number or infinite (such ones do not count).
+__device__ __forceinline__ uint32_t largest(const float4& v, bool& odd) {
+    uint32_t top = max(max(magnitude(v.x), magnitude(v.y)), max(magnitude(v.z), magnitude(v.w)));
+    if (top >= kInfinity) {
+        odd = true;
+        const auto finite = [](float x) { const uint32_t b = magnitude(x); return b < kInfinity ? b : 0u; };
+        top = max(max(finite(v.x), finite(v.y)), max(finite(v.z), finite(v.w)));
     }
-    if (lane == 0) a.scale[(size_t)cb * a.row_blocks + row] = s;
+    return top;
+}
+template <bool ALIGNED> __device__ __forceinline__ void store_four(uint8_t* q, uint32_t c, uint32_t padded, const float4& v, float s, bool odd) {
+    const float inverse = __uint_as_float(0x7f000000u - __float_as_uint(s));
+    uint32_t out = __nv_cvt_float2_to_fp8x2(make_float2(v.x * inverse, v.y * inverse), __NV_SATFINITE, __NV_E4M3) |
+                   (uint32_t)__nv_cvt_float2_to_fp8x2(make_float2(v.z * inverse, v.w * inverse), __NV_SATFINITE, __NV_E4M3) << 16;
+    if (odd) {                                      // infinities as NaN
+        if (magnitude(v.x) >= kInfinity) out |= 0x7fu;
+        if (magnitude(v.y) >= kInfinity) out |= 0x7fu << 8;
+        if (magnitude(v.z) >= kInfinity) out |= 0x7fu << 16;
+        if (magnitude(v.w) >= kInfinity) out |= 0x7fu << 24;
+    }
+    if (ALIGNED) { if (c < padded) *reinterpret_cast<uint32_t*>(q + c) = out; }
+    else {
+#pragma unroll
+        for (int k = 0; k < 4; k++) if (c + k < padded) q[c + k] = (uint8_t)(out >> 8 * k);
+    }
 }
 
-// A block of threads per 128 x 128 square, a warp per 16 rows of it.
+// A warp for kQuantRows rows of a column block, four elements a lane.
 template <typename T, bool ALIGNED>
-__global__ void __launch_bounds__(kQuantBlock) quantize_square_kernel(const QuantArgs a, uint32_t col_blocks) {
-    constexpr int kRowsPerWarp = kScaleBlock / (kQuantBlock / 32);
-    __shared__ uint32_t tops[kQuantBlock / 32];
-    const uint32_t rb = blockIdx.x / col_blocks, cb = blockIdx.x % col_blocks, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    const uint32_t c = cb * kScaleBlock + lane * 4, row0 = rb * kScaleBlock + warp * kRowsPerWarp;
-    Piece<T, 4> in[kRowsPerWarp];
-    uint32_t top = 0;
+__global__ void __launch_bounds__(kQuantBlock) quantize_rows_kernel(const QuantArgs a) {
+    const uint32_t lane = threadIdx.x & 31, cb = blockIdx.y, c = cb * kScaleBlock + lane * 4;
+    const uint32_t row0 = (blockIdx.x * kQuantWarps + (threadIdx.x >> 5)) * kQuantRows;
+    if (row0 >= a.rows) return;
+    float4 v[kQuantRows];
 #pragma unroll
-    for (int r = 0; r < kRowsPerWarp; r++) {
-        const T* const x = static_cast<const T*>(a.x) + (row0 + r) * a.x_stride;
-        in[r] = Piece<T, 4>{};
-        if (row0 + r < a.rows) {
-            if (ALIGNED) { if (c < a.width) in[r] = load_piece<T, 4>(x + c); }
-            else {
+    for (int r = 0; r < kQuantRows; r++)
+        v[r] = load_four<T, ALIGNED>(static_cast<const T*>(a.x) + min(row0 + r, a.rows - 1) * a.x_stride, c, a.width);
 #pragma unroll
-                for (int k = 0; k < 4; k++) if (c + k < a.width) in[r].v[k] = __ldg(x + c + k);
-            }
-        }
+    for (int r = 0; r < kQuantRows; r++) {
+        if (row0 + r >= a.rows) break;
+        bool odd = false;
+        const float s = scale_of(__reduce_max_sync(0xffffffffu, largest(v[r], odd)));
+        store_four<ALIGNED>(a.q + (row0 + r) * a.q_stride, c, a.padded, v[r], s, odd);
+        if (lane == 0) a.scale[(size_t)cb * a.row_blocks + row0 + r] = s;
     }
+}
+
+// A block of threads per 128 x 128 square, a warp for 16 rows of it.
+template <typename T, bool ALIGNED>
+__global__ void __launch_bounds__(kQuantBlock) quantize_square_kernel(const QuantArgs a) {
+    constexpr int kRows = kScaleBlock / kQuantWarps;
+    __shared__ uint32_t tops[kQuantWarps];
+    const uint32_t rb = blockIdx.x, cb = blockIdx.y, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const uint32_t c = cb * kScaleBlock + lane * 4, row0 = rb * kScaleBlock + warp * kRows;
+    float4 v[kRows];
 #pragma unroll
-    for (int r = 0; r < kRowsPerWarp; r++)
+    for (int r = 0; r < kRows; r++) {
+        v[r] = make_float4(0.f, 0.f, 0.f, 0.f);
+        if (row0 + r < a.rows) v[r] = load_four<T, ALIGNED>(static_cast<const T*>(a.x) + (row0 + r) * a.x_stride, c, a.width);
+    }
+    uint32_t top = 0;
+    bool odd = false;
 #pragma unroll
-        for (int k = 0; k < 4; k++) top = max(top, finite_bits(as_float(in[r].v[k])));
+    for (int r = 0; r < kRows; r++) top = max(top, largest(v[r], odd));
     top = __reduce_max_sync(0xffffffffu, top);
     if (lane == 0) tops[warp] = top;
     __syncthreads();
 #pragma unroll
-    for (int w = 0; w < kQuantBlock / 32; w++) top = max(top, tops[w]);
-    const float s = scale_of(top), inverse = __uint_as_float(0x7f000000u - __float_as_uint(s));
+    for (int w = 0; w < kQuantWarps; w++) top = max(top, tops[w]);
+    const float s = scale_of(top);
 #pragma unroll
-    for (int r = 0; r < kRowsPerWarp; r++) {
-        if (row0 + r >= a.rows) break;
-        uint8_t* const q = a.q + (row0 + r) * a.q_stride;
-        uint8_t out[4];
-#pragma unroll
-        for (int k = 0; k < 4; k++) out[k] = to_e4m3(as_float(in[r].v[k]), inverse);
-        if (ALIGNED) {
-            if (c < a.padded) *reinterpret_cast<uint32_t*>(q + c) = out[0] | out[1] << 8 | out[2] << 16 | (uint32_t)out[3] << 24;
-        } else {
-#pragma unroll
-            for (int k = 0; k < 4; k++) if (c + k < a.padded) q[c + k] = out[k];
-        }
-    }
+    for (int r = 0; r < kRows; r++)
+        if (row0 + r < a.rows) store_four<ALIGNED>(a.q + (row0 + r) * a.q_stride, c, a.padded, v[r], s, odd);
     if (threadIdx.x == 0) a.scale[(size_t)cb * a.row_blocks + rb] = s;
 }
 
@@ -478,16 +482,13 @@ int mascot_rows_quantize(const mascot_rows* x, uint32_t block_rows, const mascot
     const bool aligned = aligned_rows(*x, 4) && aligned_rows(q_written, 4);
     const cudaError_t launched = with_type(x->type, [&](auto* t) {
         using T = std::remove_pointer_t<decltype(t)>;
+        const dim3 grid(block_rows == 1 ? (a.rows + kQuantWarps * kQuantRows - 1) / (kQuantWarps * kQuantRows) : row_blocks, col_blocks);
         if (block_rows == 1) {
-            const size_t blocks = ((size_t)a.rows * col_blocks + kQuantBlock / 32 - 1) / (kQuantBlock / 32);
-            if (blocks > 0x7fffffffu) return cudaErrorInvalidConfiguration;
-            if (aligned) quantize_rows_kernel<T, true><<<(unsigned)blocks, kQuantBlock, 0, st>>>(a, col_blocks);
-            else quantize_rows_kernel<T, false><<<(unsigned)blocks, kQuantBlock, 0, st>>>(a, col_blocks);
+            if (aligned) quantize_rows_kernel<T, true><<<grid, kQuantBlock, 0, st>>>(a);
+            else quantize_rows_kernel<T, false><<<grid, kQuantBlock, 0, st>>>(a);
         } else {
-            const size_t blocks = (size_t)row_blocks * col_blocks;
-            if (blocks > 0x7fffffffu) return cudaErrorInvalidConfiguration;
-            if (aligned) quantize_square_kernel<T, true><<<(unsigned)blocks, kQuantBlock, 0, st>>>(a, col_blocks);
-            else quantize_square_kernel<T, false><<<(unsigned)blocks, kQuantBlock, 0, st>>>(a, col_blocks);
+            if (aligned) quantize_square_kernel<T, true><<<grid, kQuantBlock, 0, st>>>(a);
+            else quantize_square_kernel<T, false><<<grid, kQuantBlock, 0, st>>>(a);
         }
         return cudaGetLastError();
     });

@@ -94,6 +94,17 @@ template <typename T, int N> __device__ __forceinline__ Piece<T, N> load_piece(c
     else *reinterpret_cast<uint8_t*>(&r) = __ldg(reinterpret_cast<const uint8_t*>(p));
     return r;
 }
+// The same from shared memory.
+template <typename T, int N> __device__ __forceinline__ Piece<T, N> shared_piece(const uint8_t* p) {
+    Piece<T, N> r;
+    constexpr int bytes = sizeof(T) * N;
+    if constexpr (bytes % 16 == 0) {
+#pragma unroll
+        for (int i = 0; i < bytes / 16; i++) reinterpret_cast<uint4*>(&r)[i] = reinterpret_cast<const uint4*>(p)[i];
+    } else if constexpr (bytes == 8) *reinterpret_cast<uint2*>(&r) = *reinterpret_cast<const uint2*>(p);
+    else r = *reinterpret_cast<const Piece<T, N>*>(p);
+    return r;
+}
 template <typename T, int N> __device__ __forceinline__ void store_piece(T* p, const Piece<T, N>& r) { *reinterpret_cast<Piece<T, N>*>(p) = r; }
 #endif
 
