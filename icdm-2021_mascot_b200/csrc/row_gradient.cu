@@ -378,11 +378,11 @@ template <bool PAIRS> __device__ __forceinline__ Term term_of(const Job& j, uint
     return t;
 }
 
-// 4, 8 or 16 bytes on their way to shared memory; rows of a table stay in L1 (popular ones come again), gradient rows do not.
+// 8 or 16 bytes on their way to shared memory, past L1 (with it, pairs on a popular law take 6 % longer).
 // Zeros instead where it is not there: nothing is read then.
-template <int BYTES, bool KEEP> __device__ __forceinline__ void fetch_piece(uint32_t to, const void* from, bool there) {
-    if constexpr (BYTES == 16 && !KEEP) asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to), "l"(from), "r"(there ? 16 : 0) : "memory");
-    else asm volatile("cp.async.ca.shared.global [%0], [%1], %2, %3;" ::"r"(to), "l"(from), "n"(BYTES), "r"(there ? BYTES : 0) : "memory");
+template <int BYTES> __device__ __forceinline__ void fetch_piece(uint32_t to, const void* from, bool there) {
+    if constexpr (BYTES == 16) asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to), "l"(from), "r"(there ? 16 : 0) : "memory");
+    else asm volatile("cp.async.ca.shared.global [%0], [%1], 8, %2;" ::"r"(to), "l"(from), "r"(there ? 8 : 0) : "memory");
 }
 
 // A team's lanes take a group of entries each and hand their rows round; what a lane can work out for a group (where rows begin, which
@@ -396,9 +396,9 @@ template <typename T, int N, bool PAIRS> struct Ring {
 };
 
 template <typename T, typename Out, int N, bool PAIRS>
-__global__ void __launch_bounds__(kReduceBlock, 3) reduce_kernel(const Job j, const Space s, const uint2* entry, int team_log2) {
+__global__ void __launch_bounds__(kReduceBlock, PAIRS && N == 8 ? 2 : 3) reduce_kernel(const Job j, const Space s, const uint2* entry, int team_log2) {
     using R = Ring<T, N, PAIRS>;
-    constexpr int BATCH = 4;
+    constexpr int BATCH = 4, kSlot = R::sides * kReduceBlock * R::piece;
     extern __shared__ __align__(16) uint8_t ring[];             // [ahead][sides][threads]
     follow();
     const uint32_t team = 1u << team_log2, lane = threadIdx.x & 31, tl = lane & (team - 1), team_at = lane & ~(team - 1), ahead = min(team, (uint32_t)R::ahead);
@@ -437,14 +437,20 @@ __global__ void __launch_bounds__(kReduceBlock, 3) reduce_kernel(const Job j, co
     };
     const auto pair_of = [&](uint2 e) { return PAIRS && e.x < j.total ? __ldg(s.pair + e.y / 3) : make_uint4(0, 0, 0, 0); };
     const auto ballot = [&](bool b) { return __ballot_sync(0xffffffffu, b) >> team_at; };
-    // rows of the entries k .. k + 3 of a group
-    const auto fetch = [&](const Term& t, uint32_t adds, uint32_t twos, bool some, uint32_t k0) {      // some: a team of the warp has second rows
+    // rows of the entries k .. k + 3 of a group; `some`: a team of the warp has second rows
+    const auto fetch = [&](const Term& t, uint32_t adds, uint32_t twos, bool some, uint32_t k0) {
+        const uint32_t to = mine_to + (k0 & (ahead - 1)) * kSlot, ones = writes ? adds >> k0 : 0u, pairs = writes ? twos >> k0 : 0u;
+        if (PAIRS && some) {
 #pragma unroll
-        for (int k = 0; k < BATCH; k++) {
-            const uint32_t ra = __shfl_sync(0xffffffffu, t.a, k0 + k, team), to = mine_to + ((k0 + k) & (ahead - 1)) * (R::sides * kReduceBlock * R::piece);
-            const bool one = (adds >> (k0 + k) & 1) && writes, two = PAIRS && (twos >> (k0 + k) & 1);
-            fetch_piece<R::piece, PAIRS>(to, two ? src1 + ra * stride1 : src0 + ra * stride0, one);
-            if (PAIRS && some) fetch_piece<R::piece, PAIRS>(to + kReduceBlock * R::piece, src1 + __shfl_sync(0xffffffffu, t.b, k0 + k, team) * stride1, two && writes);
+            for (int k = 0; k < BATCH; k++) {
+                const uint32_t ra = __shfl_sync(0xffffffffu, t.a, k0 + k, team), rb = __shfl_sync(0xffffffffu, t.b, k0 + k, team);
+                const bool two = pairs >> k & 1;
+                fetch_piece<R::piece>(to + k * kSlot, two ? src1 + ra * stride1 : src0 + ra * stride0, ones >> k & 1);
+                fetch_piece<R::piece>(to + k * kSlot + kReduceBlock * R::piece, src1 + rb * stride1, two);
+            }
+        } else {
+#pragma unroll
+            for (int k = 0; k < BATCH; k++) fetch_piece<R::piece>(to + k * kSlot, src0 + __shfl_sync(0xffffffffu, t.a, k0 + k, team) * stride0, ones >> k & 1);
         }
         asm volatile("cp.async.commit_group;" ::: "memory");
     };
@@ -472,7 +478,7 @@ __global__ void __launch_bounds__(kReduceBlock, 3) reduce_kernel(const Job j, co
             for (int k = 0; k < BATCH; k++) {
                 c[k] = PAIRS ? __shfl_sync(0xffffffffu, now.c, k0 + k, team) : 1.f;
                 if constexpr (N > 1) {
-                    const uint8_t* const at = mine_at + ((k0 + k) & (ahead - 1)) * (R::sides * kReduceBlock * R::piece);
+                    const uint8_t* const at = mine_at + (k0 & (ahead - 1)) * kSlot + k * kSlot;
                     a[k] = shared_piece<T, N>(at);
                     if (PAIRS && some) b[k] = shared_piece<T, N>(at + kReduceBlock * R::piece);
                 } else {
