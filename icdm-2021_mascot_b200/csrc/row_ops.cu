@@ -262,9 +262,9 @@ cudaError_t launch_pair_loss(const PairArgs& a, bool aligned, cudaStream_t st) {
 // One pass over the rows: a block stays in registers between its maximum and its rounding.  A power of two as the scale
 // makes x / s exact, so that the only rounding is the one to four significant bits, and costs no precision: what
 // the larger scale takes from the range is at its lower end, below 2^-14 of the block's maximum.  What bounds it is the
-// rows; a warp has those of four blocks (sixteen of a square) under way at once, since one alone leaves HBM idle (107 us for
+// rows; a warp has those of four blocks (eight of a square) under way at once, since one alone leaves HBM idle (107 us for
 // 625k rows of 128 floats, 402 MB).
-constexpr int kQuantBlock = 256, kQuantWarps = kQuantBlock / 32, kQuantRows = 4;
+constexpr int kQuantBlock = 256, kQuantWarps = kQuantBlock / 32, kQuantRows = 4, kSquareBlock = 512, kSquareWarps = kSquareBlock / 32;
 
 // The scale of a block from the bits of its largest finite magnitude: 448 = 1.75 * 2^8.
 __device__ __forceinline__ float scale_of(uint32_t top) {
@@ -282,20 +282,18 @@ struct QuantArgs {
 };
 
 // Four elements of a row from column c on, zeros behind its end.
-template <typename T, bool ALIGNED> __device__ __forceinline__ float4 load_four(const T* x, uint32_t c, uint32_t width) {
-    float v[4] = {};
-    if (ALIGNED) {
-        if (c < width) {
-            const Piece<T, 4> in = load_piece<T, 4>(x + c);
+template <typename T, bool ALIGNED> __device__ __forceinline__ Piece<T, 4> load_four(const T* x, uint32_t c, uint32_t width) {
+    Piece<T, 4> in;
 #pragma unroll
-            for (int k = 0; k < 4; k++) v[k] = as_float(in.v[k]);
-        }
-    } else {
+    for (int k = 0; k < 4; k++) in.v[k] = from_float<T>(0.f);
+    if (ALIGNED) { if (c < width) in = load_piece<T, 4>(x + c); }
+    else {
 #pragma unroll
-        for (int k = 0; k < 4; k++) if (c + k < width) v[k] = as_float(load_piece<T, 1>(x + c + k).v[0]);
+        for (int k = 0; k < 4; k++) if (c + k < width) in.v[k] = load_piece<T, 1>(x + c + k).v[0];
     }
-    return make_float4(v[0], v[1], v[2], v[3]);
+    return in;
 }
+template <typename T> __device__ __forceinline__ float4 values(const Piece<T, 4>& p) { return make_float4(as_float(p.v[0]), as_float(p.v[1]), as_float(p.v[2]), as_float(p.v[3])); }
 // The largest magnitude among them, and `odd` set where one of them is no number or infinite (such ones do not count).
 __device__ __forceinline__ uint32_t largest(const float4& v, bool& odd) {
     uint32_t top = max(max(magnitude(v.x), magnitude(v.y)), max(magnitude(v.z), magnitude(v.w)));
@@ -329,7 +327,7 @@ __global__ void __launch_bounds__(kQuantBlock) quantize_rows_kernel(const QuantA
     const uint32_t lane = threadIdx.x & 31, cb = blockIdx.y, c = cb * kScaleBlock + lane * 4;
     const uint32_t row0 = (blockIdx.x * kQuantWarps + (threadIdx.x >> 5)) * kQuantRows;
     if (row0 >= a.rows) return;
-    float4 v[kQuantRows];
+    Piece<T, 4> v[kQuantRows];
 #pragma unroll
     for (int r = 0; r < kQuantRows; r++)
         v[r] = load_four<T, ALIGNED>(static_cast<const T*>(a.x) + min(row0 + r, a.rows - 1) * a.x_stride, c, a.width);
@@ -337,38 +335,35 @@ __global__ void __launch_bounds__(kQuantBlock) quantize_rows_kernel(const QuantA
     for (int r = 0; r < kQuantRows; r++) {
         if (row0 + r >= a.rows) break;
         bool odd = false;
-        const float s = scale_of(__reduce_max_sync(0xffffffffu, largest(v[r], odd)));
-        store_four<ALIGNED>(a.q + (row0 + r) * a.q_stride, c, a.padded, v[r], s, odd);
+        const float s = scale_of(__reduce_max_sync(0xffffffffu, largest(values(v[r]), odd)));
+        store_four<ALIGNED>(a.q + (row0 + r) * a.q_stride, c, a.padded, values(v[r]), s, odd);
         if (lane == 0) a.scale[(size_t)cb * a.row_blocks + row0 + r] = s;
     }
 }
 
-// A block of threads per 128 x 128 square, a warp for 16 rows of it.
+// A block of threads per 128 x 128 square, a warp for 8 rows of it.
 template <typename T, bool ALIGNED>
-__global__ void __launch_bounds__(kQuantBlock) quantize_square_kernel(const QuantArgs a) {
-    constexpr int kRows = kScaleBlock / kQuantWarps;
-    __shared__ uint32_t tops[kQuantWarps];
+__global__ void __launch_bounds__(kSquareBlock) quantize_square_kernel(const QuantArgs a) {
+    constexpr int kRows = kScaleBlock / kSquareWarps;
+    __shared__ uint32_t tops[kSquareWarps];
     const uint32_t rb = blockIdx.x, cb = blockIdx.y, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const uint32_t c = cb * kScaleBlock + lane * 4, row0 = rb * kScaleBlock + warp * kRows;
-    float4 v[kRows];
+    Piece<T, 4> v[kRows];
 #pragma unroll
-    for (int r = 0; r < kRows; r++) {
-        v[r] = make_float4(0.f, 0.f, 0.f, 0.f);
-        if (row0 + r < a.rows) v[r] = load_four<T, ALIGNED>(static_cast<const T*>(a.x) + (row0 + r) * a.x_stride, c, a.width);
-    }
+    for (int r = 0; r < kRows; r++) v[r] = load_four<T, ALIGNED>(static_cast<const T*>(a.x) + min(row0 + r, a.rows - 1) * a.x_stride, c, a.width);     // the last row again does not matter
     uint32_t top = 0;
     bool odd = false;
 #pragma unroll
-    for (int r = 0; r < kRows; r++) top = max(top, largest(v[r], odd));
+    for (int r = 0; r < kRows; r++) top = max(top, largest(values(v[r]), odd));
     top = __reduce_max_sync(0xffffffffu, top);
     if (lane == 0) tops[warp] = top;
     __syncthreads();
 #pragma unroll
-    for (int w = 0; w < kQuantWarps; w++) top = max(top, tops[w]);
+    for (int w = 0; w < kSquareWarps; w++) top = max(top, tops[w]);
     const float s = scale_of(top);
 #pragma unroll
     for (int r = 0; r < kRows; r++)
-        if (row0 + r < a.rows) store_four<ALIGNED>(a.q + (row0 + r) * a.q_stride, c, a.padded, v[r], s, odd);
+        if (row0 + r < a.rows) store_four<ALIGNED>(a.q + (row0 + r) * a.q_stride, c, a.padded, values(v[r]), s, odd);
     if (threadIdx.x == 0) a.scale[(size_t)cb * a.row_blocks + rb] = s;
 }
 
@@ -487,8 +482,8 @@ int mascot_rows_quantize(const mascot_rows* x, uint32_t block_rows, const mascot
             if (aligned) quantize_rows_kernel<T, true><<<grid, kQuantBlock, 0, st>>>(a);
             else quantize_rows_kernel<T, false><<<grid, kQuantBlock, 0, st>>>(a);
         } else {
-            if (aligned) quantize_square_kernel<T, true><<<grid, kQuantBlock, 0, st>>>(a);
-            else quantize_square_kernel<T, false><<<grid, kQuantBlock, 0, st>>>(a);
+            if (aligned) quantize_square_kernel<T, true><<<grid, kSquareBlock, 0, st>>>(a);
+            else quantize_square_kernel<T, false><<<grid, kSquareBlock, 0, st>>>(a);
         }
         return cudaGetLastError();
     });

@@ -10,7 +10,7 @@
 // of b (items) are fetched from HBM once and from L2 after that.  What differs is which side the lanes are (Mode):
 //   ONE     rows of 128 columns and less: items.  What is written bounds it.  Four warps read 8 columns of all lanes at a time, meet
 //           over shared memory and store whole rows of 128 scores, in pieces as wide as the row's address allows (32 scores a
-//           warp, straight from the accumulator, took 1.4 times as long).  Nothing is summed up, so registers allow 16 such warps.
+//           warp, straight from the accumulator, took 1.4 times as long; that is how up to 16 users are stored).  Nothing is summed up, so registers allow 16 such warps.
 //   ROWS    longer rows, a scale for each row of b, or few users: items too.  A column's scale is a broadcast from shared memory,
 //           whose 128 bytes to a warp bound the step at 4 CN cycles, twice what the matrix instructions take.
 //   SQUARE  longer rows, a scale for 128 rows of b: users.  The scale of a lane and half of the columns is one number, kept in a
@@ -40,7 +40,7 @@ template <int CN, Mode MODE> struct Shape {
     static constexpr int readers = 4 * groups, threads = 32 * readers + 128;
     static constexpr int stage_bytes = kLaneTileBytes + CN * kScaleBlock;
     static constexpr int step_scales = kLanes + (MODE == SQUARE ? 4 : CN);
-    static constexpr int transit = MODE == SQUARE ? readers * 32 * kStagePitch : MODE == ONE ? groups * 2 * (CN / groups < 16 ? 8 : 16) * kLanes * 4 : 0;
+    static constexpr int transit = MODE == SQUARE ? readers * 32 * kStagePitch : MODE == ONE && CN > 16 ? groups * 2 * 16 * kLanes * 4 : 0;
     static constexpr size_t smem = 1024 + (size_t)stages * stage_bytes + transit + kScaleSteps * step_scales * 4 + 8 * (2 * stages + 2 * buffers + 2 * kScaleSteps) + 16;
     static_assert(smem <= 227 * 1024, "shared memory of a block");
 };
@@ -330,7 +330,17 @@ __global__ void __launch_bounds__(Shape<CN, MODE>::threads, 1) product_kernel(co
                     __syncwarp();
                     if (lane == 0) barrier_arrive(spare + b);
                 };
-                if constexpr (MODE == ONE) {
+                if constexpr (MODE == ONE && CN == 16) {        // few users: a store of 32 scores for each, and no meeting
+                    if (cols > 0) {
+                        uint32_t part[kRead];
+                        read_columns<kRead>(from, part);
+                        wait_columns<kRead>(part);
+                        release();
+#pragma unroll
+                        for (int k = 0; k < kRead; k++)
+                            if (k < cols && lane < rows) reinterpret_cast<Out*>(out + k * pitch)[lane] = from_float<Out>(__uint_as_float(part[k]) * lane_scale * scale[group * kGroup + k]);
+                    } else release();
+                } else if constexpr (MODE == ONE) {
                     constexpr int kRows = kRead / 4;            // of a chunk, for each of the four warps
                     const int items = (int)min(p.lane.rows - (l - lanes), (uint32_t)kLanes), row0 = warp % 4 * kRows;
                     uint8_t* row = out - lanes * sizeof(Out) + row0 * pitch;
