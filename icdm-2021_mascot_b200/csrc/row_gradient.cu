@@ -790,21 +790,21 @@ using namespace mascot;
 
 extern "C" {
 
-int mascot_rows_gradient_workspace(uint64_t count, uint64_t rows, uint32_t width, uint64_t* bytes) {
+int mascot_rows_gradient_workspace(uint64_t count, uint64_t rows, uint32_t width, uint64_t* bytes) try {
     if (!bytes || count >= kMaxRows || rows >= kMaxRows || width == 0 || width > kMaxWidth) return fail(nullptr, MASCOT_ERR_BAD_ARG, "null pointer or size out of range");
     *bytes = carve(count, rows, width, false, nullptr, nullptr);
     return MASCOT_OK;
-}
+} ROW_CATCH
 
-int mascot_pair_gradient_workspace(uint64_t count, uint64_t n_users, uint64_t n_items, uint32_t width, uint64_t* bytes) {
+int mascot_pair_gradient_workspace(uint64_t count, uint64_t n_users, uint64_t n_items, uint32_t width, uint64_t* bytes) try {
     if (!bytes || count >= kMaxRows || n_users >= kMaxRows || n_items >= kMaxRows || width == 0 || width > kMaxWidth || 3 * count >= kMaxRows || n_users + n_items >= kMaxRows)
         return fail(nullptr, MASCOT_ERR_BAD_ARG, "null pointer or size out of range");
     *bytes = carve(3 * count, n_users + n_items, width, true, nullptr, nullptr);
     return MASCOT_OK;
-}
+} ROW_CATCH
 
 int mascot_rows_gradient(const mascot_rows* grad, const mascot_ids* ids, float scale, const mascot_rows* out, int accumulate, void* workspace,
-                         uint64_t workspace_bytes, uint32_t* flags, void* stream) {
+                         uint64_t workspace_bytes, uint32_t* flags, void* stream) try {
     ROW_CHECK(check_rows("grad", grad, false));
     ROW_CHECK(check_ids("ids", ids));
     ROW_CHECK(check_rows("out", out, false));
@@ -851,11 +851,11 @@ int mascot_rows_gradient(const mascot_rows* grad, const mascot_ids* ids, float s
     });
     CU(nullptr, launched);
     return MASCOT_OK;
-}
+} ROW_CATCH
 
 int mascot_pair_gradient(const mascot_rows* P, const mascot_rows* Q, const mascot_ids* users, const mascot_ids* preferred, const mascot_ids* other,
                          const float* coef, float scale, const mascot_rows* dP, const mascot_rows* dQ, int accumulate, void* workspace,
-                         uint64_t workspace_bytes, uint32_t* flags, void* stream) {
+                         uint64_t workspace_bytes, uint32_t* flags, void* stream) try {
     const struct { const char* what; const mascot_rows* m; } mats[] = {{"P", P}, {"Q", Q}, {"dP", dP}, {"dQ", dQ}};
     const struct { const char* what; const mascot_ids* ids; } idss[] = {{"users", users}, {"preferred", preferred}, {"other", other}};
     for (const auto& m : mats) ROW_CHECK(check_rows(m.what, m.m, false));
@@ -916,6 +916,6 @@ int mascot_pair_gradient(const mascot_rows* P, const mascot_rows* Q, const masco
     });
     CU(nullptr, launched);
     return MASCOT_OK;
-}
+} ROW_CATCH
 
 }  // extern "C"

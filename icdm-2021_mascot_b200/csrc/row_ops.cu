@@ -118,10 +118,14 @@ __global__ void __launch_bounds__(kLookupBlock) lookup_kernel(const LookupArgs a
     const int tl = threadIdx.x & ((1 << team_log2) - 1);
     const size_t first = (((size_t)blockIdx.x * kLookupBlock + threadIdx.x) >> team_log2) * kLookupRows;
     if (first >= a.n) return;
-    uint32_t row[kLookupRows];
+    uint32_t at[kLookupRows], row[kLookupRows];
+    RawId id[kLookupRows];
     bool bad = false;
 #pragma unroll
-    for (int k = 0; k < kLookupRows; k++) row[k] = first + k < a.n ? row_of(a.ids, (uint32_t)(first + k), a.rows, bad) : kNoRow;
+    for (int k = 0; k < kLookupRows; k++) at[k] = (uint32_t)min(first + k, a.n - 1);
+    load_ids<kLookupRows>(a.ids, at, id);
+#pragma unroll
+    for (int k = 0; k < kLookupRows; k++) row[k] = row_of(id[k], a.ids, a.rows, bad);
     if (bad && tl == 0 && a.flags) atomicOr(a.flags, (uint32_t)MASCOT_FLAG_BAD_ID);
     for (uint32_t c = tl * N; c < a.width; c += N << team_log2) {
         Piece<In, N> in[kLookupRows];
@@ -375,7 +379,7 @@ using namespace mascot;
 extern "C" {
 
 int mascot_rows_lookup(const mascot_rows* table, const float* table_scale, uint32_t block_rows, const mascot_ids* ids, float scale,
-                       const mascot_rows* out, uint32_t* flags, void* stream) {
+                       const mascot_rows* out, uint32_t* flags, void* stream) try {
     const bool e4m3 = table && table->type == MASCOT_E4M3;
     ROW_CHECK(check_rows("table", table, e4m3));
     ROW_CHECK(check_ids("ids", ids));
@@ -408,11 +412,11 @@ int mascot_rows_lookup(const mascot_rows* table, const float* table_scale, uint3
     });
     CU(nullptr, launched);
     return MASCOT_OK;
-}
+} ROW_CATCH
 
 int mascot_pair_loss(const mascot_rows* P, const mascot_rows* Q, const mascot_ids* users, const mascot_ids* preferred, const mascot_ids* other,
                      float beta, float smoothing, const float* reference, const float* weight, float* loss, float* margin, float* coef,
-                     uint32_t* flags, void* stream) {
+                     uint32_t* flags, void* stream) try {
     ROW_CHECK(check_rows("P", P, false));
     ROW_CHECK(check_rows("Q", Q, false));
     ROW_CHECK(check_ids("users", users));
@@ -450,9 +454,9 @@ int mascot_pair_loss(const mascot_rows* P, const mascot_rows* Q, const mascot_id
     });
     CU(nullptr, launched);
     return MASCOT_OK;
-}
+} ROW_CATCH
 
-int mascot_rows_quantize(const mascot_rows* x, uint32_t block_rows, const mascot_rows* q, float* scale, void* stream) {
+int mascot_rows_quantize(const mascot_rows* x, uint32_t block_rows, const mascot_rows* q, float* scale, void* stream) try {
     ROW_CHECK(check_rows("x", x, false));
     ROW_CHECK(check_rows("q", q, true));
     if (q->rows != x->rows || q->width != x->width) return fail(nullptr, MASCOT_ERR_BAD_ARG, "q: must have the shape of x");
@@ -489,6 +493,6 @@ int mascot_rows_quantize(const mascot_rows* x, uint32_t block_rows, const mascot
     });
     CU(nullptr, launched);
     return MASCOT_OK;
-}
+} ROW_CATCH
 
 }  // extern "C"

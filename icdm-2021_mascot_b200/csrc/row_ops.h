@@ -7,6 +7,7 @@
 #include <cuda_runtime.h>
 
 #include <cstdint>
+#include <new>
 
 #include "handle.h"
 
@@ -29,6 +30,9 @@ int check_memory(const char* what, const void* p);                       // devi
 int current_sms();                                                          // of the current device
 
 #define ROW_CHECK(call) do { const int rc_ = (call); if (rc_ != MASCOT_OK) return rc_; } while (0)
+
+// Nothing leaves a C entry as an exception: behind the body of one that begins with `try`.
+#define ROW_CATCH catch (const std::bad_alloc&) { return MASCOT_ERR_OOM; } catch (...) { return MASCOT_ERR_CUDA; }
 
 inline bool is_empty(const mascot_rows& m) { return m.rows == 0; }
 // Whether rows of `m` can be moved in pieces of `elements` aligned elements.

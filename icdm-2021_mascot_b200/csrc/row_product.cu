@@ -483,7 +483,7 @@ cudaError_t launch_tiles(const mascot_rows& a, const mascot_rows& b, const Produ
 using namespace mascot;
 
 extern "C" int mascot_rows_product(const mascot_rows* a, const float* a_scale, const mascot_rows* b, const float* b_scale, uint32_t b_block_rows,
-                                   const mascot_rows* out, uint32_t* flags, void* stream) {
+                                   const mascot_rows* out, uint32_t* flags, void* stream) try {
     ROW_CHECK(check_rows("a", a, true));
     ROW_CHECK(check_rows("b", b, true));
     if (((a->rows + 15) / 16) * ((b->rows + kLanes - 1) / kLanes) > 0x3fffffffull) return fail(nullptr, MASCOT_ERR_UNSUPPORTED, "too many scores for one call: split a or b");
@@ -522,4 +522,4 @@ extern "C" int mascot_rows_product(const mascot_rows* a, const float* a_scale, c
     const cudaError_t launched = with_type(out->type, [&](auto* o) { return launch_tiles<std::remove_pointer_t<decltype(o)>>(*a, *b, p, static_cast<cudaStream_t>(stream)); });
     CU(nullptr, launched);
     return MASCOT_OK;
-}
+} ROW_CATCH

@@ -116,7 +116,7 @@ def plain_gradient(grad, ids, rows, scale):
 
 # one chunk and less; one block's sort and one entry more; tiles with and without a scan; one, two and three digits
 @pytest.mark.parametrize("n,rows", [(1, 1), (2, 5), (15, 3), (16, 3), (17, 40), (1000, 7), (12_287, 900), (12_288, 900), (12_289, 900), (12_289, 1), (40_000, 1023), (40_000, 1024),
-                                    (131_072, 100_000), (200_001, 50), (140_001, 1_200_000)])
+                                    (32_768, 900), (32_769, 900), (131_072, 100_000), (200_001, 50), (140_001, 1_200_000), (1_048_575, 3000), (1_200_001, 300_000), (1_050_000, 200)])
 def test_gradient_is_exact_on_integers(mascot, n, rows):
     g = gen(n + rows)
     for width, dtype, src in ((4, torch.int32, torch.float32), (7, torch.int64, torch.bfloat16), (132, torch.int32, torch.float16)):
@@ -156,6 +156,15 @@ def test_gradient(mascot, src, dst, width):
     within(got, whole, sums + whole.abs() * (half(dst) + 2 * U) * 1.01 + (2.0 ** -24 if dst == torch.float16 else 0), "accumulate")
     untouched = terms[:, 0] == 0
     assert torch.equal(got[untouched], base[untouched])
+
+
+def test_gradient_of_a_long_table(mascot):
+    """Keys of more than 24 bits: three digits of ten."""
+    rows, n = 40_000_000, 70_000
+    ids = some_ids(n, rows, gen(4), torch.int64)
+    grad = torch.randint(-8, 9, (n, 1), generator=gen(5), device=DEV).half()
+    want, _, _ = plain_gradient(grad, ids, rows, 1.0)
+    assert torch.equal(mascot.rows_gradient(grad, ids, rows, out_dtype=torch.float32).double(), want)
 
 
 @pytest.mark.parametrize("n", [3000, 300_000, 2_300_000])
@@ -287,7 +296,7 @@ def test_pair_loss_at_its_ends(mascot):
 
 @pytest.mark.parametrize("dtype", TYPES)
 @pytest.mark.parametrize("dst", TYPES)
-@pytest.mark.parametrize("width", [3, 64, 128, 260])
+@pytest.mark.parametrize("width", [3, 16, 64, 100, 128, 260])
 def test_pair_gradient(mascot, dtype, dst, width):
     for n, users, items, id_type in ((1, 4, 3, torch.int64), (700, 60, 30, torch.int32), (4096, 300, 5, torch.int32), (9001, 2000, 100, torch.int32)):
         P, Q, u, i, j, ref, w = pairs(n, users, items, width, dtype, width + n, id_type)
@@ -316,9 +325,9 @@ def test_pair_gradient(mascot, dtype, dst, width):
             within(got, whole, 2 * (count + 4) * U * mass + whole.abs() * (half(dst) + 2 * U) * 1.01 + tiny, "accumulate")
 
 
-def test_pair_gradient_of_many_pairs_is_exact_on_integers(mascot):
+@pytest.mark.parametrize("n,users,items", [(1, 2, 2), (171, 5, 2), (1366, 900, 40), (10_923, 3000, 40), (150_001, 70_000, 900), (400_003, 70_000, 9000)])
+def test_pair_gradient_is_exact_on_integers(mascot, n, users, items):
     g = gen(5)
-    n, users, items = 150_001, 70_000, 900
     P = torch.randint(-2, 3, (users, 64), generator=g, device=DEV).float()
     Q = torch.randint(-2, 3, (items, 64), generator=g, device=DEV).float()
     u, i, j = some_ids(n, users, g), some_ids(n, items, g), some_ids(n, items, g)
@@ -330,12 +339,48 @@ def test_pair_gradient_of_many_pairs_is_exact_on_integers(mascot):
     gotP, gotQ = mascot.pair_gradient(P, Q, u, i, j, coef)
     assert torch.equal(gotP.double(), dP) and torch.equal(gotQ.double(), dQ)
     f = flag()
-    u[7], j[9] = users, items
+    a, b = 7 % n, 9 % n
+    u[a], j[b] = users, items
     mascot.pair_gradient(P, Q, u, i, j, coef, flags=f)
     assert f.item() == mascot.FLAG_BAD_ID
     f = flag()
     loss, m, c = mascot.pair_loss(P, Q, u, i, j, flags=f)
-    assert f.item() == mascot.FLAG_BAD_ID and loss[[7, 9]].tolist() == [0, 0] and c[[7, 9]].tolist() == [0, 0]
+    assert f.item() == mascot.FLAG_BAD_ID and loss[[a, b]].tolist() == [0, 0] and c[[a, b]].tolist() == [0, 0]
+
+
+def test_pair_tables_without_rows(mascot):
+    """Pairs that name rows of an empty table add nothing, and say so."""
+    P, Q = torch.empty(0, 64, device=DEV), torch.ones(3, 64, device=DEV)
+    u = torch.tensor([0, -1], device=DEV)
+    f = flag()
+    loss, m, c = mascot.pair_loss(P, Q, u, u.clamp(min=0), u.clamp(min=0), flags=f)
+    assert loss.tolist() == [0, 0] and f.item() == mascot.FLAG_BAD_ID
+    f = flag()
+    dP, dQ = mascot.pair_gradient(P, Q, u, u.clamp(min=0), u.clamp(min=0), torch.ones(2, device=DEV), dP=torch.empty(0, 64, device=DEV), dQ=torch.ones(3, 64, device=DEV), flags=f)
+    assert dP.shape == (0, 64) and (dQ == 0).all() and f.item() == mascot.FLAG_BAD_ID
+    none = torch.empty(0, dtype=torch.int64, device=DEV)
+    assert all(t.shape == (0,) for t in mascot.pair_loss(Q, Q, none, none, none))
+    dP, dQ = mascot.pair_gradient(Q, Q, none, none, none, torch.empty(0, device=DEV), dP=torch.ones(3, 64, device=DEV), dQ=torch.ones(3, 64, device=DEV))
+    assert (dP == 0).all() and (dQ == 0).all()
+
+
+def test_two_streams_at_once(mascot):
+    """Calls in flight on two streams, each with scratch of its own, do not touch one another."""
+    args = [pairs(60_000, 5000, 700, 64, torch.float32, s) for s in (1, 2)]
+    def both(a):
+        P, Q, u, i, j, ref, w = a
+        c = mascot.pair_loss(P, Q, u, i, j, weight=w)[2]
+        return mascot.pair_gradient(P, Q, u, i, j, c)
+    want = [[t.clone() for t in both(a)] for a in args]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in args]
+    for _ in range(20):
+        got = []
+        for a, st in zip(args, streams):
+            with torch.cuda.stream(st):
+                got.append(both(a))
+        torch.cuda.synchronize()
+        assert all(torch.equal(x, y) for g, w in zip(got, want) for x, y in zip(g, w))
 
 
 def test_pair_gradient_against_differences(mascot):
