@@ -820,14 +820,15 @@ int mascot_rows_gradient(const mascot_rows* grad, const mascot_ids* ids, float s
     ROW_CHECK(check_distinct("workspace", workspace, workspace_bytes, "flags", flags, 4));
     ROW_CHECK(check_distinct("flags", flags, 4, "out", out));
     if (ids->count == 0 && (accumulate || out->rows == 0)) return MASCOT_OK;
-    ROW_CHECK(check_device());
+    int device = 0;
+    ROW_CHECK(check_device(&device));
     if (ids->count) {
-        ROW_CHECK(check_memory("grad", grad->data));
-        ROW_CHECK(check_memory("ids", ids->data));
-        ROW_CHECK(check_memory("workspace", workspace));
+        ROW_CHECK(check_memory("grad", grad->data, device));
+        ROW_CHECK(check_memory("ids", ids->data, device));
+        ROW_CHECK(check_memory("workspace", workspace, device));
     }
-    if (out->rows) ROW_CHECK(check_memory("out", out->data));
-    ROW_CHECK(check_memory("flags", flags));
+    if (out->rows) ROW_CHECK(check_memory("out", out->data, device));
+    ROW_CHECK(check_memory("flags", flags, device));
     Job j = {};
     j.ids[0] = ids_of(*ids);
     j.per = j.n = (uint32_t)ids->count;
@@ -883,14 +884,15 @@ int mascot_pair_gradient(const mascot_rows* P, const mascot_rows* Q, const masco
     ROW_CHECK(check_distinct("workspace", workspace, workspace_bytes, "coef", coef, n * 4));
     ROW_CHECK(check_distinct("workspace", workspace, workspace_bytes, "flags", flags, 4));
     if (n == 0 && (accumulate || total == 0)) return MASCOT_OK;
-    ROW_CHECK(check_device());
-    for (const auto& m : mats) if (m.m->rows) ROW_CHECK(check_memory(m.what, m.m->data));
+    int device = 0;
+    ROW_CHECK(check_device(&device));
+    for (const auto& m : mats) if (m.m->rows) ROW_CHECK(check_memory(m.what, m.m->data, device));
     if (n) {
-        for (const auto& x : idss) ROW_CHECK(check_memory(x.what, x.ids->data));
-        ROW_CHECK(check_memory("coef", coef));
-        ROW_CHECK(check_memory("workspace", workspace));
+        for (const auto& x : idss) ROW_CHECK(check_memory(x.what, x.ids->data, device));
+        ROW_CHECK(check_memory("coef", coef, device));
+        ROW_CHECK(check_memory("workspace", workspace, device));
     }
-    ROW_CHECK(check_memory("flags", flags));
+    ROW_CHECK(check_memory("flags", flags, device));
     Job j = {};
     j.ids[0] = ids_of(*users); j.ids[1] = ids_of(*preferred); j.ids[2] = ids_of(*other);
     j.per = (uint32_t)n; j.kinds = 3; j.n = (uint32_t)(3 * n);

@@ -73,9 +73,8 @@ int check_distinct(const char* what_a, const void* a, size_t bytes_a, const char
     return check_distinct(what_a, a, bytes_a, what_b, b->data, s.end - s.begin);
 }
 
-int check_device() {
-    int dev = -1;
-    if (cudaGetDevice(&dev) == cudaSuccess) return MASCOT_OK;
+int check_device(int* device) {
+    if (cudaGetDevice(device) == cudaSuccess) return MASCOT_OK;
     cudaGetLastError();
     return fail(nullptr, MASCOT_ERR_NO_DEVICE, "no usable CUDA device; libmascot has no CPU path");
 }
@@ -85,15 +84,14 @@ int current_sms() {
     return cudaGetDevice(&dev) == cudaSuccess && cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev) == cudaSuccess ? n : 1;
 }
 
-int check_memory(const char* what, const void* p) {
+int check_memory(const char* what, const void* p, int device) {
     if (!p) return MASCOT_OK;
     cudaPointerAttributes at;
-    int dev = -1;
-    if (cudaPointerGetAttributes(&at, p) != cudaSuccess || cudaGetDevice(&dev) != cudaSuccess) {
+    if (cudaPointerGetAttributes(&at, p) != cudaSuccess) {
         cudaGetLastError();
         return fail(nullptr, MASCOT_ERR_NO_DEVICE, "no usable CUDA device; libmascot has no CPU path");
     }
-    if (at.type == cudaMemoryTypeManaged || (at.type == cudaMemoryTypeDevice && at.device == dev)) return MASCOT_OK;
+    if (at.type == cudaMemoryTypeManaged || (at.type == cudaMemoryTypeDevice && at.device == device)) return MASCOT_OK;
     return refuse(MASCOT_ERR_BAD_ARG, what, "not memory of the current device");
 }
 
@@ -395,12 +393,13 @@ int mascot_rows_lookup(const mascot_rows* table, const float* table_scale, uint3
     ROW_CHECK(check_distinct("table_scale", table_scale, row_blocks * ((table->width + kScaleBlock - 1) / kScaleBlock) * 4, "out", out));
     ROW_CHECK(check_distinct("flags", flags, 4, "out", out));
     if (is_empty(*out)) return MASCOT_OK;
-    ROW_CHECK(check_device());
-    if (table->rows) ROW_CHECK(check_memory("table", table->data));
-    ROW_CHECK(check_memory("table_scale", table_scale));
-    ROW_CHECK(check_memory("ids", ids->data));
-    ROW_CHECK(check_memory("out", out->data));
-    ROW_CHECK(check_memory("flags", flags));
+    int device = 0;
+    ROW_CHECK(check_device(&device));
+    if (table->rows) ROW_CHECK(check_memory("table", table->data, device));
+    ROW_CHECK(check_memory("table_scale", table_scale, device));
+    ROW_CHECK(check_memory("ids", ids->data, device));
+    ROW_CHECK(check_memory("out", out->data, device));
+    ROW_CHECK(check_memory("flags", flags, device));
     LookupArgs a{table->data, table_scale, out->data, table->stride, out->stride, ids->count, ids_of(*ids), (uint32_t)table->rows, table->width,
                  (uint32_t)row_blocks, block_rows == kScaleBlock ? 7u : 0u, scale, flags};
     const cudaStream_t st = static_cast<cudaStream_t>(stream);
@@ -441,11 +440,12 @@ int mascot_pair_loss(const mascot_rows* P, const mascot_rows* Q, const mascot_id
         }
     }
     if (n == 0) return MASCOT_OK;
-    ROW_CHECK(check_device());
-    if (P->rows) ROW_CHECK(check_memory("P", P->data));
-    if (Q->rows) ROW_CHECK(check_memory("Q", Q->data));
-    for (const auto& x : in) ROW_CHECK(check_memory(x.what, x.p));
-    for (const auto& x : out) ROW_CHECK(check_memory(x.what, x.p));
+    int device = 0;
+    ROW_CHECK(check_device(&device));
+    if (P->rows) ROW_CHECK(check_memory("P", P->data, device));
+    if (Q->rows) ROW_CHECK(check_memory("Q", Q->data, device));
+    for (const auto& x : in) ROW_CHECK(check_memory(x.what, x.p, device));
+    for (const auto& x : out) ROW_CHECK(check_memory(x.what, x.p, device));
     const PairArgs a{P->data, Q->data, P->stride, Q->stride, n, ids_of(*users), ids_of(*preferred), ids_of(*other), (uint32_t)P->rows, (uint32_t)Q->rows,
                      P->width, beta, smoothing, reference, weight, loss, margin, coef, flags};
     const cudaError_t launched = with_type(P->type, [&](auto* t) {
@@ -472,10 +472,11 @@ int mascot_rows_quantize(const mascot_rows* x, uint32_t block_rows, const mascot
     ROW_CHECK(check_distinct("x", x, "q", &q_written));
     ROW_CHECK(check_distinct("scale", scale, scale_bytes, "q", &q_written));
     ROW_CHECK(check_distinct("scale", scale, scale_bytes, "x", x));
-    ROW_CHECK(check_device());
-    ROW_CHECK(check_memory("x", x->data));
-    ROW_CHECK(check_memory("q", q->data));
-    ROW_CHECK(check_memory("scale", scale));
+    int device = 0;
+    ROW_CHECK(check_device(&device));
+    ROW_CHECK(check_memory("x", x->data, device));
+    ROW_CHECK(check_memory("q", q->data, device));
+    ROW_CHECK(check_memory("scale", scale, device));
     const QuantArgs a{x->data, static_cast<uint8_t*>(q->data), scale, x->stride, q->stride, (uint32_t)x->rows, x->width, padded, row_blocks};
     const cudaStream_t st = static_cast<cudaStream_t>(stream);
     const bool aligned = aligned_rows(*x, 4) && aligned_rows(q_written, 4);

@@ -25,8 +25,8 @@ int check_ids(const char* what, const mascot_ids* ids);
 int check_distinct(const char* what_a, const mascot_rows* a, const char* what_b, const mascot_rows* b);   // no element in common
 int check_distinct(const char* what_a, const void* a, size_t bytes_a, const char* what_b, const mascot_rows* b);
 int check_distinct(const char* what_a, const void* a, size_t bytes_a, const char* what_b, const void* b, size_t bytes_b);
-int check_device();                                                     // there is one (a launch refuses a stream of another one itself)
-int check_memory(const char* what, const void* p);                       // device memory of the current device
+int check_device(int* device);                                           // the current one (a launch refuses a stream of another one itself)
+int check_memory(const char* what, const void* p, int device);           // device memory of that device, or null
 int current_sms();                                                          // of the current device
 
 #define ROW_CHECK(call) do { const int rc_ = (call); if (rc_ != MASCOT_OK) return rc_; } while (0)

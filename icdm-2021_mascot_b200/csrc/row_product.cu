@@ -505,13 +505,14 @@ extern "C" int mascot_rows_product(const mascot_rows* a, const float* a_scale, c
     ROW_CHECK(check_distinct("a_scale", a_scale, 4 * (size_t)col_blocks * a->rows, "out", out));
     ROW_CHECK(check_distinct("b_scale", b_scale, 4 * (size_t)col_blocks * n_scales, "out", out));
     ROW_CHECK(check_distinct("flags", flags, 4, "out", out));
-    ROW_CHECK(check_device());
-    ROW_CHECK(check_memory("a", a->data));
-    ROW_CHECK(check_memory("b", b->data));
-    ROW_CHECK(check_memory("a_scale", a_scale));
-    ROW_CHECK(check_memory("b_scale", b_scale));
-    ROW_CHECK(check_memory("out", out->data));
-    ROW_CHECK(check_memory("flags", flags));
+    int device = 0;
+    ROW_CHECK(check_device(&device));
+    ROW_CHECK(check_memory("a", a->data, device));
+    ROW_CHECK(check_memory("b", b->data, device));
+    ROW_CHECK(check_memory("a_scale", a_scale, device));
+    ROW_CHECK(check_memory("b_scale", b_scale, device));
+    ROW_CHECK(check_memory("out", out->data, device));
+    ROW_CHECK(check_memory("flags", flags, device));
     if (!encode_tiled()) return fail(nullptr, MASCOT_ERR_UNSUPPORTED, "the driver has no cuTensorMapEncodeTiled");
     ProductArgs p = {};
     p.lane = Side{b_scale, (uint32_t)b->rows, n_scales, b_block_rows == 1 ? 0u : 7u};

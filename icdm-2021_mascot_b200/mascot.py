@@ -472,7 +472,7 @@ def _id_vector(what, t, device):
     bits = _torch_ops().bits.get(t.dtype)
     if bits is None:
         _refuse(f"{what}: must be int32 or int64, not {t.dtype}")
-    if t.dim() != 1 or (t.shape[0] > 1 and t.stride(0) != 1):
+    if t.dim() != 1 or not t.is_contiguous():
         _refuse(f"{what}: must be a contiguous vector")
     if t.device != device:
         _refuse(f"{what}: is on {t.device}, not on {device}")
@@ -511,9 +511,10 @@ def _call(device, name, *args):
         raise MascotError(rc, load().mascot_last_error(None).decode())
 
 
-def _result(what, out, shape, dtype, device):
+def _result(what, out, shape, dtype, like):
+    """`out` where it fits, else a new tensor on the device of `like`."""
     if out is None:
-        return _torch_ops().torch.empty(shape, dtype=dtype, device=device)
+        return like.new_empty(shape) if dtype == like.dtype else like.new_empty(shape, dtype=dtype)
     if tuple(out.shape) != tuple(shape):
         _refuse(f"{what}: must have shape {tuple(shape)}")
     if dtype is not None and out.dtype != dtype:
@@ -538,17 +539,17 @@ def rows_lookup(table, ids, scale=1.0, table_scale=None, out=None, out_dtype=Non
         each, ts = _scale_rows("table_scale", table_scale, t.rows, t.width, device)
     if out_dtype is None and out is None:
         out_dtype = _torch_ops().torch.float32 if t.type == E4M3 else table.dtype
-    out = _result("out", out, (i.count, t.width), out_dtype, device)
+    out = _result("out", out, (i.count, t.width), out_dtype, table)
     _call(device, "mascot_rows_lookup", t, ts, each, i, scale, _rows("out", out, device), _flag_word(flags, device))
     return out
 
 
-def _workspace(workspace, name, device, *sizes):
+def _workspace(workspace, name, like, device, *sizes):
     need = C.c_uint64()
     if getattr(load(), name)(*sizes, C.byref(need)) != OK:
         _refuse(load().mascot_last_error(None).decode())
     if workspace is None:
-        workspace = _torch_ops().torch.empty(need.value, dtype=_torch_ops().torch.uint8, device=device)
+        workspace = like.new_empty(need.value, dtype=_torch_ops().torch.uint8)
     elif not workspace.is_contiguous() or workspace.device != device:
         _refuse(f"workspace: must be a contiguous tensor on {device}")
     return workspace, workspace.data_ptr(), workspace.numel() * workspace.element_size()
@@ -561,8 +562,8 @@ def rows_gradient(grad, ids, rows, scale=1.0, out=None, out_dtype=None, accumula
     g, i = _rows("grad", grad, device), _id_vector("ids", ids, device)
     if accumulate and out is None:
         _refuse("accumulate: needs an out")
-    out = _result("out", out, (rows, g.width), out_dtype if out_dtype is not None or out is not None else grad.dtype, device)
-    keep, ws, size = _workspace(workspace, "mascot_rows_gradient_workspace", device, i.count, rows, g.width)
+    out = _result("out", out, (rows, g.width), out_dtype if out_dtype is not None or out is not None else grad.dtype, grad)
+    keep, ws, size = _workspace(workspace, "mascot_rows_gradient_workspace", grad, device, i.count, rows, g.width)
     _call(device, "mascot_rows_gradient", g, i, scale, _rows("out", out, device), 1 if accumulate else 0, ws, size, _flag_word(flags, device))
     return out
 
@@ -575,7 +576,7 @@ def pair_loss(P, Q, users, preferred, other, beta=1.0, smoothing=0.0, reference=
     u, i, j = _id_vector("users", users, device), _id_vector("preferred", preferred, device), _id_vector("other", other, device)
     n = u.count
     ref, w = _plain("reference", reference, torch.float32, device, (n,)), _plain("weight", weight, torch.float32, device, (n,))
-    loss, margin, coef = (torch.empty(n, dtype=torch.float32, device=device) for _ in range(3))
+    loss, margin, coef = P.new_empty((3, n), dtype=torch.float32).unbind(0)
     _call(device, "mascot_pair_loss", p, q, u, i, j, beta, smoothing, ref, w, loss.data_ptr(), margin.data_ptr(), coef.data_ptr(),
           _flag_word(flags, device))
     return loss, margin, coef
@@ -589,10 +590,10 @@ def pair_gradient(P, Q, users, preferred, other, coef, scale=1.0, dP=None, dQ=No
     u, i, j = _id_vector("users", users, device), _id_vector("preferred", preferred, device), _id_vector("other", other, device)
     if accumulate and (dP is None or dQ is None):
         _refuse("accumulate: needs dP and dQ")
-    dP = _result("dP", dP, P.shape, out_dtype if out_dtype is not None or dP is not None else P.dtype, device)
-    dQ = _result("dQ", dQ, Q.shape, out_dtype if out_dtype is not None or dQ is not None else Q.dtype, device)
+    dP = _result("dP", dP, P.shape, out_dtype if out_dtype is not None or dP is not None else P.dtype, P)
+    dQ = _result("dQ", dQ, Q.shape, out_dtype if out_dtype is not None or dQ is not None else Q.dtype, Q)
     c = _plain("coef", coef, _torch_ops().torch.float32, device, (u.count,))
-    keep, ws, size = _workspace(workspace, "mascot_pair_gradient_workspace", device, u.count, p.rows, q.rows, p.width)
+    keep, ws, size = _workspace(workspace, "mascot_pair_gradient_workspace", P, device, u.count, p.rows, q.rows, p.width)
     _call(device, "mascot_pair_gradient", p, q, u, i, j, c, scale, _rows("dP", dP, device), _rows("dQ", dQ, device), 1 if accumulate else 0, ws,
           size, _flag_word(flags, device))
     return dP, dQ
@@ -607,7 +608,7 @@ def rows_quantize(x, block_rows=1, q=None, scale=None):
     if q is None:
         q = torch.empty((r.rows, -(-r.width // 128) * 128), dtype=torch.float8_e4m3fn, device=device)[:, :r.width]
     else:
-        q = _result("q", q, (r.rows, r.width), torch.float8_e4m3fn, device)
+        q = _result("q", q, (r.rows, r.width), torch.float8_e4m3fn, x)
     shape = (-(-r.width // 128), -(-r.rows // block_rows) if block_rows > 0 else 0)
     if scale is None:
         scale = torch.empty(shape, dtype=torch.float32, device=device)
@@ -624,6 +625,6 @@ def rows_product(a, a_scale, b, b_scale, out=None, out_dtype=None, flags=None):
     x, y = _rows("a", a, device), _rows("b", b, device)
     sa = _plain("a_scale", a_scale, torch.float32, device, (-(-x.width // 128), x.rows))
     each, sb = _scale_rows("b_scale", b_scale, y.rows, y.width, device)
-    out = _result("out", out, (x.rows, y.rows), out_dtype if out_dtype is not None or out is not None else torch.float32, device)
+    out = _result("out", out, (x.rows, y.rows), out_dtype if out_dtype is not None or out is not None else torch.float32, a)
     _call(device, "mascot_rows_product", x, sa, y, sb, each, _rows("out", out, device), _flag_word(flags, device))
     return out
