@@ -199,8 +199,11 @@ __global__ void __launch_bounds__(kSmallBlock) small_sort_kernel(const Job j, co
         cluster.sync();
         uint32_t within = 0;                                    // entries of the bin in the tiles before
         if (t < kSmallBins) {
-            uint32_t sum = 0;
-            for (uint32_t b = 0; b < blocks; b++) { if (b == block) within = sum; sum += *cluster.map_shared_rank(&counts[t], b); }
+            uint32_t of[kSmallCluster], sum = 0;
+#pragma unroll
+            for (uint32_t b = 0; b < kSmallCluster; b++) of[b] = b < blocks ? *cluster.map_shared_rank(&counts[t], b) : 0u;
+#pragma unroll
+            for (uint32_t b = 0; b < kSmallCluster; b++) { if (b == block) within = sum; sum += of[b]; }
             base[t] = sum;
         }
         __syncthreads();
@@ -635,7 +638,7 @@ __global__ void __launch_bounds__(kCombineBlock, 2) combine_kernel(const Job j, 
 // ---- host ---------------------------------------------------------------------------------------------------
 
 // Entries of a chunk: enough chunks to fill the GPU, and no more parts than that needs.
-int chunk_log2(uint64_t n) { return n < (1u << 17) ? 4 : n < (1u << 19) ? 5 : n < (1u << 21) ? 6 : 7; }
+int chunk_log2(uint64_t n) { return n < (1u << 14) ? 3 : n < (1u << 17) ? 4 : n < (1u << 19) ? 5 : n < (1u << 21) ? 6 : 7; }
 int bits_for(uint64_t keys) { int b = 1; while (b < 32 && (1ull << b) < keys) b++; return b; }      // of the largest key, keys - 1
 
 size_t carve(uint64_t n, uint64_t total, uint32_t width, bool pairs, char* base, Space* s) {
