@@ -99,7 +99,8 @@ namespace {
 
 // ---- lookup ------------------------------------------------------------------------------------------------
 // What bounds it: the rows written, and those read where they are not in L2.  Lanes of a row write 16 bytes each next
-// to one another, and a team has the loads of kRows rows in flight before its first store.
+// to one another, and a team has the loads of kLookupRows rows in flight before its first store.  2M rows of 128 elements, binary16
+// into fp32, from a table of a million: 206 us, 6.2 TB/s of what has to move (a copy: 6.55).
 constexpr int kLookupBlock = 256, kLookupRows = 4;
 
 struct LookupArgs {
@@ -167,7 +168,8 @@ cudaError_t launch_lookup(const LookupArgs& a, bool aligned, cudaStream_t st) {
 // ---- preference loss -------------------------------------------------------------------------------------------
 // A pair is three rows and a dot product: bound by fetching rows, and by the instructions around them.  A team of lanes takes a
 // run of pairs: each lane finds the rows of one of them and hands them round, the rows of kPairs pairs are in flight at once, and
-// in the end each lane works out the loss of its own pair.
+// in the end each lane works out the loss of its own pair.  1M pairs of binary16 rows of 128: 105 us, 7.3 TB/s from L2 and HBM
+// together; 180 us while all lanes of a team looked at the ids of every pair.
 constexpr int kPairBlock = 256, kPairs = 4;
 
 struct PairArgs {
@@ -264,8 +266,8 @@ cudaError_t launch_pair_loss(const PairArgs& a, bool aligned, cudaStream_t st) {
 // One pass over the rows: a block stays in registers between its maximum and its rounding.  A power of two as the scale
 // makes x / s exact, so that the only rounding is the one to four significant bits, and costs no precision: what
 // the larger scale takes from the range is at its lower end, below 2^-14 of the block's maximum.  What bounds it is the
-// rows; a warp has those of four blocks (eight of a square) under way at once, since one alone leaves HBM idle (107 us for
-// 625k rows of 128 floats, 402 MB).
+// rows; a warp has those of four blocks (eight of a square) under way at once: 625k rows of 128 floats, 402 MB, take 60 us
+// (6.7 TB/s), and took 107 with one block a warp and values converted one by one.
 constexpr int kQuantBlock = 256, kQuantWarps = kQuantBlock / 32, kQuantRows = 4, kSquareBlock = 512, kSquareWarps = kSquareBlock / 32;
 
 // The scale of a block from the bits of its largest finite magnitude: 448 = 1.75 * 2^8.
