@@ -65,6 +65,7 @@ struct Space {                                  // the workspace, see carve()
 };
 
 // For kernels that launch_behind launches, and those before them: the next kernel's blocks may be brought up; the kernel before has ended.
+// What one kernel of a call leaves for the next is read with plain loads, since it changes while the next one's blocks are already there.
 __device__ __forceinline__ void follow() {
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     asm volatile("griddepcontrol.wait;" ::: "memory");
@@ -122,7 +123,7 @@ template <int BITS> __device__ __forceinline__ uint32_t warp_rank(uint32_t digit
 
 // Counters of `warps` warps, [warp][bins], become offsets of the warps within a bin, for two bins (2 b, 2 b + 1) at once; their sums come back.
 __device__ __forceinline__ uint32_t warp_offsets(uint16_t* count, int warps, int bins, int b) {
-    uint32_t sum = 0;                                           // two halves that never carry: at most 12288 entries
+    uint32_t sum = 0;                                           // two halves that never carry: a tile has at most 8192 entries
     for (int w = 0; w < warps; w++) {
         uint32_t* const c = reinterpret_cast<uint32_t*>(count + w * bins) + b;
         const uint32_t x = *c;
@@ -413,7 +414,7 @@ __global__ void __launch_bounds__(kReduceBlock, PAIRS && N == 8 ? 2 : 3) reduce_
     const uint32_t begin = min(j.n, chunk << j.chunk_log2), end = min(j.n, begin + size);
     const bool writes = chunk < s.chunks && col < j.width;
     // rows across the chunk's ends: finished by the chunk before where they end within `over` entries, else in parts
-    const auto row_at = [&](uint32_t i) { return i < j.n ? __ldg(&entry[i].x) : kNoRow; };
+    const auto row_at = [&](uint32_t i) { return i < j.n ? entry[i].x : kNoRow; };
     const uint32_t before = chunk < s.chunks && begin ? row_at(begin - 1) : kNoRow, last = end > begin ? row_at(end - 1) : kNoRow;
     const bool in_parts = before != kNoRow && row_at(begin + over) == before, on_in_parts = end < j.n && row_at(end + over) == last;
     const uint32_t until = on_in_parts || end == begin ? end : min(j.n, end + over);
@@ -436,11 +437,11 @@ __global__ void __launch_bounds__(kReduceBlock, PAIRS && N == 8 ? 2 : 3) reduce_
     };
     const auto entry_at = [&](uint32_t i) {
         uint2 e = make_uint2(j.total, 0);
-        if (i < until) e = __ldg(entry + i);
+        if (i < until) e = entry[i];
         if (i >= end ? e.x != last : !in_parts && e.x == before) e.x = j.total;
         return e;
     };
-    const auto pair_of = [&](uint2 e) { return PAIRS && e.x < j.total ? __ldg(s.pair + e.y / 3) : make_uint4(0, 0, 0, 0); };
+    const auto pair_of = [&](uint2 e) { return PAIRS && e.x < j.total ? s.pair[e.y / 3] : make_uint4(0, 0, 0, 0); };
     const auto ballot = [&](bool b) { return __ballot_sync(0xffffffffu, b) >> team_at; };
     // rows of the entries k .. k + 3 of a group; `some`: a team of the warp has second rows
     const auto fetch = [&](const Term& t, uint32_t adds, uint32_t twos, bool some, uint32_t k0) {
@@ -537,7 +538,7 @@ __device__ __forceinline__ uint32_t row_end(const uint2* entry, uint32_t at, uin
     uint32_t lo = at, hi = n;                                   // the entry at lo is one, that at hi is none
     while (hi - lo > 1) {
         const uint32_t step = (hi - lo + 31) / 32, mid = lo + lane * step;      // lane 0: lo
-        const uint32_t in = __popc(__ballot_sync(0xffffffffu, mid < hi && __ldg(&entry[mid].x) == row));      // the first `in` places
+        const uint32_t in = __popc(__ballot_sync(0xffffffffu, mid < hi && entry[mid].x == row));      // the first `in` places
         hi = min(hi, lo + in * step);
         lo += (in - 1) * step;
     }
@@ -589,7 +590,7 @@ __global__ void __launch_bounds__(kCombineBlock, 2) combine_kernel(const Job j, 
             const uint32_t chunk = owner.x, row = owner.y, first = (chunk + 1) << j.chunk_log2;
             // Chunks that follow with a part of the row.  Most rows end soon: lane q looks whether the row goes on in parts behind q chunks more.
             const uint64_t at = (uint64_t)first + (uint64_t)lane * size + size / 4;
-            const uint32_t through = __ballot_sync(0xffffffffu, at < j.n && __ldg(&entry[at].x) == row);
+            const uint32_t through = __ballot_sync(0xffffffffu, at < j.n && entry[at].x == row);
             uint32_t count = __popc(through);
             if (through == 0xffffffffu) {                       // all but one where it ends within a quarter of a chunk: those entries are in the part before
                 const uint32_t stop = row_end(entry, first, j.n, row, lane), whole = (stop - first) >> j.chunk_log2;

@@ -282,7 +282,7 @@ __device__ __forceinline__ uint32_t magnitude(float x) { return __float_as_uint(
 struct QuantArgs {
     const void* x; uint8_t* q; float* scale;
     size_t x_stride, q_stride;
-    uint32_t rows, width, padded, row_blocks;       // padded: columns of q that are written
+    uint32_t rows, width, row_blocks;
 };
 
 // Four elements of a row from column c on, zeros behind its end.
@@ -308,7 +308,7 @@ __device__ __forceinline__ uint32_t largest(const float4& v, bool& odd) {
     }
     return top;
 }
-template <bool ALIGNED> __device__ __forceinline__ void store_four(uint8_t* q, uint32_t c, uint32_t padded, const float4& v, float s, bool odd) {
+template <bool ALIGNED> __device__ __forceinline__ void store_four(uint8_t* q, uint32_t c, uint32_t width, const float4& v, float s, bool odd) {
     const float inverse = __uint_as_float(0x7f000000u - __float_as_uint(s));
     uint32_t out = __nv_cvt_float2_to_fp8x2(make_float2(v.x * inverse, v.y * inverse), __NV_SATFINITE, __NV_E4M3) |
                    (uint32_t)__nv_cvt_float2_to_fp8x2(make_float2(v.z * inverse, v.w * inverse), __NV_SATFINITE, __NV_E4M3) << 16;
@@ -318,10 +318,10 @@ template <bool ALIGNED> __device__ __forceinline__ void store_four(uint8_t* q, u
         if (magnitude(v.z) >= kInfinity) out |= 0x7fu << 16;
         if (magnitude(v.w) >= kInfinity) out |= 0x7fu << 24;
     }
-    if (ALIGNED) { if (c < padded) *reinterpret_cast<uint32_t*>(q + c) = out; }
+    if (ALIGNED) { if (c < width) *reinterpret_cast<uint32_t*>(q + c) = out; }
     else {
 #pragma unroll
-        for (int k = 0; k < 4; k++) if (c + k < padded) q[c + k] = (uint8_t)(out >> 8 * k);
+        for (int k = 0; k < 4; k++) if (c + k < width) q[c + k] = (uint8_t)(out >> 8 * k);
     }
 }
 
@@ -340,7 +340,7 @@ __global__ void __launch_bounds__(kQuantBlock) quantize_rows_kernel(const QuantA
         if (row0 + r >= a.rows) break;
         bool odd = false;
         const float s = scale_of(__reduce_max_sync(0xffffffffu, largest(values(v[r]), odd)));
-        store_four<ALIGNED>(a.q + (row0 + r) * a.q_stride, c, a.padded, values(v[r]), s, odd);
+        store_four<ALIGNED>(a.q + (row0 + r) * a.q_stride, c, a.width, values(v[r]), s, odd);
         if (lane == 0) a.scale[(size_t)cb * a.row_blocks + row0 + r] = s;
     }
 }
@@ -367,7 +367,7 @@ __global__ void __launch_bounds__(kSquareBlock) quantize_square_kernel(const Qua
     const float s = scale_of(top);
 #pragma unroll
     for (int r = 0; r < kRows; r++)
-        if (row0 + r < a.rows) store_four<ALIGNED>(a.q + (row0 + r) * a.q_stride, c, a.padded, values(v[r]), s, odd);
+        if (row0 + r < a.rows) store_four<ALIGNED>(a.q + (row0 + r) * a.q_stride, c, a.width, values(v[r]), s, odd);
     if (threadIdx.x == 0) a.scale[(size_t)cb * a.row_blocks + rb] = s;
 }
 
@@ -467,21 +467,18 @@ int mascot_rows_quantize(const mascot_rows* x, uint32_t block_rows, const mascot
     if (!scale) return fail(nullptr, MASCOT_ERR_BAD_ARG, "scale: null pointer");
     if (reinterpret_cast<uintptr_t>(scale) % 4) return fail(nullptr, MASCOT_ERR_BAD_ARG, "scale: address is not a multiple of the element's size");
     const uint32_t col_blocks = (x->width + kScaleBlock - 1) / kScaleBlock, row_blocks = (uint32_t)((x->rows + block_rows - 1) / block_rows);
-    const uint32_t padded = (uint32_t)std::min<uint64_t>((x->width + 15) / 16 * 16, q->stride);
-    mascot_rows q_written = *q;
-    q_written.width = padded;
     const size_t scale_bytes = (size_t)col_blocks * row_blocks * 4;
-    ROW_CHECK(check_distinct("x", x, "q", &q_written));
-    ROW_CHECK(check_distinct("scale", scale, scale_bytes, "q", &q_written));
+    ROW_CHECK(check_distinct("x", x, "q", q));
+    ROW_CHECK(check_distinct("scale", scale, scale_bytes, "q", q));
     ROW_CHECK(check_distinct("scale", scale, scale_bytes, "x", x));
     int device = 0;
     ROW_CHECK(check_device(&device));
     ROW_CHECK(check_memory("x", x->data, device));
     ROW_CHECK(check_memory("q", q->data, device));
     ROW_CHECK(check_memory("scale", scale, device));
-    const QuantArgs a{x->data, static_cast<uint8_t*>(q->data), scale, x->stride, q->stride, (uint32_t)x->rows, x->width, padded, row_blocks};
+    const QuantArgs a{x->data, static_cast<uint8_t*>(q->data), scale, x->stride, q->stride, (uint32_t)x->rows, x->width, row_blocks};
     const cudaStream_t st = static_cast<cudaStream_t>(stream);
-    const bool aligned = aligned_rows(*x, 4) && aligned_rows(q_written, 4);
+    const bool aligned = aligned_rows(*x, 4) && aligned_rows(*q, 4);
     const cudaError_t launched = with_type(x->type, [&](auto* t) {
         using T = std::remove_pointer_t<decltype(t)>;
         const dim3 grid(block_rows == 1 ? (a.rows + kQuantWarps * kQuantRows - 1) / (kQuantWarps * kQuantRows) : row_blocks, col_blocks);

@@ -489,8 +489,7 @@ MASCOT_API int mascot_pair_gradient_workspace(uint64_t count, uint64_t n_users, 
 /* Rows to 8 bits: q = e4m3(x / s), rounded to nearest even, with one scale s for each block of `block_rows` (1 or 128) rows by
  * 128 columns, the smallest power of two (not below 2^-126) with |x| / s <= 448 for every finite x of the block, 1 where they
  * are all zero.  The division is exact, so each value is rounded once.  NaN and infinities become NaN in their place alone.
- * scale[c * ceil(rows / block_rows) + r] belongs to column block c, row block r.  Columns of q from the width to the next
- * multiple of 16, as far as the stride reaches, become zeros. */
+ * scale[c * ceil(rows / block_rows) + r] belongs to column block c, row block r. */
 MASCOT_API int mascot_rows_quantize(const mascot_rows* x, uint32_t block_rows, const mascot_rows* q, float* scale, void* stream);
 
 /* Scores of all pairs of rows: out[m][n] = sum over column blocks c of a_scale * b_scale * (sum of a[m] * b[n] within c), for two

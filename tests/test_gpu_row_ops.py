@@ -459,10 +459,21 @@ def test_quantize_borders_and_what_is_not_finite(mascot):
     assert mascot.rows_quantize(x[:0])[0].shape == (0, 4)
 
 
-def test_quantize_clears_the_tail_of_a_row_and_no_more(mascot):
-    store = torch.full((5, 160), 77, dtype=torch.uint8, device=DEV)
-    mascot.rows_quantize(torch.ones(5, 100, device=DEV), q=store.view(torch.float8_e4m3fn)[:, :100])
-    assert (store[:, 100:112] == 0).all() and (store[:, 112:] == 77).all()
+def test_quantize_and_lookup_write_rows_and_no_more(mascot):
+    """What lies between the rows, and behind the last one, stays as it was."""
+    for width in (100, 97, 128):
+        store = torch.full((5 * 160 + 7,), 77, dtype=torch.uint8, device=DEV)
+        q = store[3 * (width == 97):].as_strided((5, width), (160, 1), 3 * (width == 97)).view(torch.float8_e4m3fn)
+        mascot.rows_quantize(torch.ones(5, width, device=DEV), q=q)
+        mark = torch.zeros_like(store)
+        mark.as_strided((5, width), (160, 1), 3 * (width == 97)).fill_(1)
+        assert (store[mark == 0] == 77).all() and (store[mark == 1] != 77).all()
+        out = torch.full((5 * 160 + 7,), 7.0, device=DEV)
+        mascot.rows_lookup(torch.ones(9, width, device=DEV), torch.arange(5, device=DEV), out=out.as_strided((5, width), (160, 1), 3 * (width == 97)))
+        assert (out[mark == 0] == 7).all() and (out[mark == 1] == 1).all()
+        out.fill_(7)
+        mascot.rows_gradient(torch.ones(2, width, device=DEV), torch.tensor([1, 4], device=DEV), 5, out=out.as_strided((5, width), (160, 1), 3 * (width == 97)))
+        assert (out[mark == 0] == 7).all() and out[mark == 1].sum().item() == 2 * width
 
 
 # ---- scores ----------------------------------------------------------------------------------------------------------
