@@ -31,8 +31,8 @@ constexpr int kLanes = 128;                          // lanes of tensor memory
 constexpr int kLaneTileBytes = kLanes * kScaleBlock;
 constexpr int kScaleSteps = 8;                       // steps whose scales are under way or in use: a step may be shorter than a fetch from HBM
 constexpr int kStagePitch = 80;                      // bytes of a row's piece of 64 on its way through shared memory (SQUARE)
-constexpr uint32_t kNap = 10'000'000;                // ns; a wait gives up after kTries of them (at least: a try may end early)
-constexpr int kTries = 4000;
+constexpr uint32_t kNap = 1'000'000;                 // ns
+constexpr long long kPatience = 1ll << 33;           // cycles: more than four seconds
 
 template <int CN, Mode MODE> struct Shape {
     static constexpr int stages = CN == 256 ? (MODE == ONE ? 3 : 4) : CN == 128 ? (MODE == ONE ? 4 : 6) : MODE == ONE && CN == 64 ? 6 : 8;
@@ -71,16 +71,20 @@ __device__ __forceinline__ void barrier_arrive(uint64_t* b) {
 __device__ __forceinline__ void barrier_expect(uint64_t* b, uint32_t bytes) {
     asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(smem_at(b)), "r"(bytes) : "memory");
 }
-// Waits for the phase of that parity to end, but not for ever: each try sleeps up to kNap ns.
+// Waits for the phase of that parity to end, but not for ever: each try sleeps up to kNap ns, and what has not come kPatience cycles
+// after the first few gives up.
 __device__ __forceinline__ bool barrier_wait(uint64_t* b, uint32_t parity) {
+    constexpr uint32_t kFew = 64;
     const uint32_t at = smem_at(b);
+    long long begin = 0;
 #pragma unroll 1
-    for (int tries = 0; tries < kTries; tries++) {
+    for (uint32_t tries = 0;; tries++) {
         uint32_t done;
         asm volatile("{ .reg .pred p; mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, %3; selp.u32 %0, 1, 0, p; }" : "=r"(done) : "r"(at), "r"(parity), "r"(kNap) : "memory");
         if (done) return true;
+        if (tries < kFew) begin = clock64();
+        else if (clock64() - begin > kPatience) return false;
     }
-    return false;
 }
 
 // Box of 128 columns by the map's rows at (column, row) into shared memory; what lies outside the matrix is zero.
