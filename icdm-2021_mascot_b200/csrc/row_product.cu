@@ -87,6 +87,14 @@ __device__ __forceinline__ bool barrier_wait(uint64_t* b, uint32_t parity) {
     }
 }
 
+// True in one lane of a converged warp, always the same one.  The compiler knows that it is one, and keeps what tcgen05 and TMA
+// instructions take in uniform registers; behind `lane == 0` each of them is wrapped into a loop over lanes.
+__device__ __forceinline__ bool elect_one() {
+    uint32_t one;
+    asm volatile("{ .reg .pred p; elect.sync _|p, 0xffffffff; selp.u32 %0, 1, 0, p; }" : "=r"(one));
+    return one;
+}
+
 // Box of 128 columns by the map's rows at (column, row) into shared memory; what lies outside the matrix is zero.
 __device__ __forceinline__ void fetch_tile(const CUtensorMap* map, void* to, uint64_t* bar, int col, int row) {
     asm volatile("cp.async.bulk.tensor.2d.shared::cta.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];" ::"r"(smem_at(to)),
@@ -244,34 +252,41 @@ __global__ void __launch_bounds__(Shape<CN, MODE>::threads, 1) product_kernel(co
         if (MODE != ONE) asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
         uint32_t step = 0;
         bool ok = true;
-        if (warp == S::readers && lane == 0) {                  // operands
+        const auto wait = [&](uint64_t* bar, uint32_t parity) { return __all_sync(0xffffffffu, barrier_wait(bar, parity)); };
+        if (warp == S::readers) {                               // operands
             for (uint32_t t = blockIdx.x; ok && t < p.tiles; t += gridDim.x) {
                 const int lane0 = (int)lane_of(t), col0 = (int)col_of(t);
                 for (uint32_t c = 0; c < p.blocks; c++, step++) {
                     const int s = step % kStages;
-                    if (step >= kStages && !(ok = barrier_wait(empty + s, (step / kStages + 1) & 1))) break;
-                    barrier_expect(full + s, S::stage_bytes);
-                    fetch_tile(&lane_map, stages + s * S::stage_bytes, full + s, (int)(c * kScaleBlock), lane0);
-                    fetch_tile(&col_map, stages + s * S::stage_bytes + kLaneTileBytes, full + s, (int)(c * kScaleBlock), col0);
+                    if (step >= kStages && !(ok = wait(empty + s, (step / kStages + 1) & 1))) break;
+                    if (elect_one()) {
+                        barrier_expect(full + s, S::stage_bytes);
+                        fetch_tile(&lane_map, stages + s * S::stage_bytes, full + s, (int)(c * kScaleBlock), lane0);
+                        fetch_tile(&col_map, stages + s * S::stage_bytes + kLaneTileBytes, full + s, (int)(c * kScaleBlock), col0);
+                    }
+                    __syncwarp();
                 }
             }
             // copies in flight end before the block does
-            for (uint32_t q = step > kStages ? step - kStages : 0; q < step; q++) ok &= barrier_wait(full + q % kStages, q / kStages & 1);
+            for (uint32_t q = step > kStages ? step - kStages : 0; q < step; q++) ok &= wait(full + q % kStages, q / kStages & 1);
         }
-        if (warp == S::readers + 1 && lane == 0) {              // matrix instructions
+        if (warp == S::readers + 1) {                           // matrix instructions
             // accumulators fp32 (1 << 4), both operands e4m3 (0) and K-major (0), N / 8, M / 16
             constexpr uint32_t idesc = 1u << 4 | (uint32_t)(CN / 8) << 17 | (uint32_t)(kLanes / 16) << 24;
             for (uint32_t t = blockIdx.x; ok && t < p.tiles; t += gridDim.x)
                 for (uint32_t c = 0; c < p.blocks; c++, step++) {
                     const int s = step % kStages, b = step % kBuffers;
-                    if (step >= kBuffers && !(ok = barrier_wait(spare + b, (step / kBuffers + 1) & 1))) break;
-                    if (!(ok = barrier_wait(full + s, step / kStages & 1))) break;
+                    if (step >= kBuffers && !(ok = wait(spare + b, (step / kBuffers + 1) & 1))) break;
+                    if (!(ok = wait(full + s, step / kStages & 1))) break;
                     fence_after();
                     const uint64_t lanes = operand_desc(stages + s * S::stage_bytes), cols = operand_desc(stages + s * S::stage_bytes + kLaneTileBytes);
+                    if (elect_one()) {
 #pragma unroll
-                    for (int k = 0; k < 4; k++) multiply(tmem + b * CN, lanes + 2 * k, cols + 2 * k, idesc, k > 0);      // 32 columns each
-                    commit(empty + s);
-                    commit(ready + b);
+                        for (int k = 0; k < 4; k++) multiply(tmem + b * CN, lanes + 2 * k, cols + 2 * k, idesc, k > 0);      // 32 columns each
+                        commit(empty + s);
+                        commit(ready + b);
+                    }
+                    __syncwarp();
                 }
         }
         if (warp == S::readers + 2) {                           // scales, 0 for rows that are not there
@@ -279,7 +294,7 @@ __global__ void __launch_bounds__(Shape<CN, MODE>::threads, 1) product_kernel(co
                 const uint32_t lane0 = lane_of(t), col0 = col_of(t);
                 for (uint32_t c = 0; c < p.blocks; c++, step++) {
                     const int q = step % kScaleSteps;
-                    if (step >= kScaleSteps && !(ok = __all_sync(0xffffffffu, barrier_wait(used + q, (step / kScaleSteps + 1) & 1)))) break;
+                    if (step >= kScaleSteps && !(ok = wait(used + q, (step / kScaleSteps + 1) & 1))) break;
                     float* const to = scales + q * S::step_scales;
                     const float* const of_lanes = p.lane.scale + (size_t)c * p.lane.scales, *const of_cols = p.col.scale + (size_t)c * p.col.scales;
                     const auto fetch = [&](float* at, const float* from, const Side& side, uint32_t row) {
@@ -297,7 +312,7 @@ __global__ void __launch_bounds__(Shape<CN, MODE>::threads, 1) product_kernel(co
             }
             asm volatile("cp.async.wait_all;" ::: "memory");
         }
-        if (!ok && p.flags) atomicOr(p.flags, (uint32_t)MASCOT_FLAG_GAVE_UP);
+        if (!ok && lane == 0 && p.flags) atomicOr(p.flags, (uint32_t)MASCOT_FLAG_GAVE_UP);
     } else {                                                    // sums and scores
         if (MODE != ONE) asm volatile("setmaxnreg.inc.sync.aligned.u32 224;");
         const int group = warp / 4;
