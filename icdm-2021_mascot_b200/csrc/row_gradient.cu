@@ -350,20 +350,23 @@ __global__ void __launch_bounds__(kSortBlock, 2) scatter_kernel(const Space s, u
 
 // ---- sums --------------------------------------------------------------------------------------------------
 
-template <typename Out, int N>
-__device__ __forceinline__ void write_row(const Job& j, uint32_t row, uint32_t col, const float (&sum)[N]) {
+// N columns of a row: ALIGNED ones from `col` on as one piece, else those `gap` apart, as far as the row goes.
+template <typename Out, int N, bool ALIGNED>
+__device__ __forceinline__ void write_row(const Job& j, uint32_t row, uint32_t col, uint32_t gap, const float (&sum)[N]) {
     const bool second = row >= j.rows[0];
     Out* const at = static_cast<Out*>(second ? j.out[1] : j.out[0]) + (size_t)(second ? row - j.rows[0] : row) * (second ? j.out_stride[1] : j.out_stride[0]) + col;
-    Piece<Out, N> r;
-    if (j.accumulate) {
-        r = *reinterpret_cast<const Piece<Out, N>*>(at);
+    const auto value = [&](float x, Out was) { return from_float<Out>(j.accumulate ? fmaf(x, j.scale, as_float(was)) : x * j.scale); };
+    if constexpr (ALIGNED) {
+        Piece<Out, N> r = {};
+        if (j.accumulate) r = *reinterpret_cast<const Piece<Out, N>*>(at);
 #pragma unroll
-        for (int k = 0; k < N; k++) r.v[k] = from_float<Out>(fmaf(sum[k], j.scale, as_float(r.v[k])));
+        for (int k = 0; k < N; k++) r.v[k] = value(sum[k], r.v[k]);
+        store_piece<Out, N>(at, r);
     } else {
 #pragma unroll
-        for (int k = 0; k < N; k++) r.v[k] = from_float<Out>(sum[k] * j.scale);
+        for (int k = 0; k < N; k++)
+            if (col + k * gap < j.width) at[k * gap] = value(sum[k], j.accumulate ? at[k * gap] : from_float<Out>(0.f));
     }
-    store_piece<Out, N>(at, r);
 }
 
 // What an entry adds: c * (row a - row b), as far as it has these rows.
@@ -395,21 +398,23 @@ template <int BYTES> __device__ __forceinline__ void fetch_piece(uint32_t to, co
 // L2, so AHEAD of them are under way for each team: every lane copies its pieces into shared memory of its own, which needs
 // no registers and no meeting of threads.  4M rows of 256 bytes into 480k of 512: 211 us for 1.29 GB, 6.1 TB/s (286 with four rows in
 // flight in registers).  The gradients of 1M pairs, binary16 rows of 128: 237 us, bound by instructions and by the latency of L2.
-// Single elements (N = 1) are loaded where they are added.
-template <typename T, int N, bool PAIRS> struct Ring {
+// Rows that cannot be moved in pieces are loaded where they are added, element by element, four for each lane a team's width apart
+// (20,000 rows of 333 binary16 numbers: 41 us in all; 91 with one for each lane).
+template <typename T, int N, bool PAIRS, bool ALIGNED> struct Ring {
     static constexpr int piece = sizeof(T) * N, ahead = PAIRS ? 8 : 16, sides = PAIRS ? 2 : 1;      // rows of an entry
-    static constexpr size_t smem = N > 1 ? (size_t)ahead * sides * kReduceBlock * piece : 0;
+    static constexpr size_t smem = ALIGNED ? (size_t)ahead * sides * kReduceBlock * piece : 0;
 };
 
-template <typename T, typename Out, int N, bool PAIRS>
+template <typename T, typename Out, int N, bool PAIRS, bool ALIGNED>
 __global__ void __launch_bounds__(kReduceBlock, PAIRS && N == 8 ? 2 : 3) reduce_kernel(const Job j, const Space s, const uint2* entry, int team_log2) {
-    using R = Ring<T, N, PAIRS>;
+    using R = Ring<T, N, PAIRS, ALIGNED>;
     constexpr int BATCH = 4, kSlot = R::sides * kReduceBlock * R::piece;
     extern __shared__ __align__(16) uint8_t ring[];             // [ahead][sides][threads]
     follow();
     const uint32_t team = 1u << team_log2, lane = threadIdx.x & 31, tl = lane & (team - 1), team_at = lane & ~(team - 1), ahead = min(team, (uint32_t)R::ahead);
     const uint32_t team_mask = (team == 32 ? 0xffffffffu : (1u << team) - 1) << team_at;
-    const uint32_t chunk = (blockIdx.x * kReduceBlock + threadIdx.x) >> team_log2, col = ((blockIdx.y << team_log2) + tl) * N;
+    const uint32_t chunk = (blockIdx.x * kReduceBlock + threadIdx.x) >> team_log2, gap = ALIGNED ? 1 : team;
+    const uint32_t col = (blockIdx.y << team_log2) * N + tl * (ALIGNED ? N : 1);      // this lane's first column; the others are `gap` apart
     const uint32_t size = 1u << j.chunk_log2, over = size / 4;
     const uint32_t begin = min(j.n, chunk << j.chunk_log2), end = min(j.n, begin + size);
     const bool writes = chunk < s.chunks && col < j.width;
@@ -430,9 +435,9 @@ __global__ void __launch_bounds__(kReduceBlock, PAIRS && N == 8 ? 2 : 3) reduce_
         if (from_before || (on_in_parts && row == last)) {
             float* const part = (from_before ? s.head : s.tail) + (size_t)chunk * s.pitch + col;
 #pragma unroll
-            for (int k = 0; k < N; k++) part[k] = sum[k];
+            for (int k = 0; k < N; k++) if (ALIGNED || col + k * gap < j.width) part[k * gap] = sum[k];
             if (!from_before && col == 0) s.owners[atomicAdd(s.n_owners, 1u)] = make_uint2(chunk, row);
-        } else write_row<Out, N>(j, row, col, sum);
+        } else write_row<Out, N, ALIGNED>(j, row, col, gap, sum);
         if (!from_before && !j.accumulate && col == 0) s.touched[row] = 1;
     };
     const auto entry_at = [&](uint32_t i) {
@@ -467,7 +472,7 @@ __global__ void __launch_bounds__(kReduceBlock, PAIRS && N == 8 ? 2 : 3) reduce_
     const auto any = [](uint32_t mask) { return __any_sync(0xffffffffu, mask != 0); };
     uint32_t adds = ballot(now.has_a), twos = PAIRS ? ballot(now.has_b) : 0u;
     bool some = PAIRS && any(twos);                             // seldom both: users' rows are sorted before items'
-    if constexpr (N > 1) for (uint32_t k0 = 0; k0 < ahead; k0 += BATCH) fetch(now, adds, twos, some, k0);
+    if constexpr (ALIGNED) for (uint32_t k0 = 0; k0 < ahead; k0 += BATCH) fetch(now, adds, twos, some, k0);
     for (uint32_t g = begin; __any_sync(0xffffffffu, g < until); g += team) {
         const uint32_t left = __shfl_up_sync(0xffffffffu, now.key, 1, team), begins = ballot(now.key != (tl ? left : row));
         const uint32_t next_adds = ballot(next.has_a), next_twos = PAIRS ? ballot(next.has_b) : 0u;
@@ -476,24 +481,31 @@ __global__ void __launch_bounds__(kReduceBlock, PAIRS && N == 8 ? 2 : 3) reduce_
             if (!__any_sync(0xffffffffu, g + k0 < until)) break;
             Piece<T, N> a[BATCH], b[PAIRS ? BATCH : 1];
             float c[BATCH];
-            if constexpr (N > 1) {
+            if constexpr (ALIGNED) {
                 if (ahead == 16) asm volatile("cp.async.wait_group 3;" ::: "memory");
                 else asm volatile("cp.async.wait_group 1;" ::: "memory");
             }
 #pragma unroll
             for (int k = 0; k < BATCH; k++) {
                 c[k] = PAIRS ? __shfl_sync(0xffffffffu, now.c, k0 + k, team) : 1.f;
-                if constexpr (N > 1) {
+                if constexpr (ALIGNED) {
                     const uint8_t* const at = mine_at + (k0 & (ahead - 1)) * kSlot + k * kSlot;
                     a[k] = shared_piece<T, N>(at);
                     if (PAIRS && some) b[k] = shared_piece<T, N>(at + kReduceBlock * R::piece);
                 } else {
                     const uint32_t ra = __shfl_sync(0xffffffffu, now.a, k0 + k, team), rb = PAIRS ? __shfl_sync(0xffffffffu, now.b, k0 + k, team) : 0u;
                     const bool one = (adds >> (k0 + k) & 1) && writes, two = PAIRS && (twos >> (k0 + k) & 1);
-                    a[k].v[0] = from_float<T>(0.f);
-                    if (PAIRS) b[k].v[0] = from_float<T>(0.f);
-                    if (one) a[k] = load_piece<T, N>(two ? src1 + ra * stride1 : src0 + ra * stride0);
-                    if (PAIRS && two && writes) b[k] = load_piece<T, N>(src1 + rb * stride1);
+                    const T* const from_a = two ? src1 + ra * stride1 : src0 + ra * stride0, *const from_b = src1 + rb * stride1;
+#pragma unroll
+                    for (int x = 0; x < N; x++) {
+                        const bool there = col + x * gap < j.width;
+                        a[k].v[x] = from_float<T>(0.f);
+                        if (one && there) a[k].v[x] = load_piece<T, 1>(from_a + x * gap).v[0];
+                        if (PAIRS) {
+                            b[k].v[x] = from_float<T>(0.f);
+                            if (two && writes && there) b[k].v[x] = load_piece<T, 1>(from_b + x * gap).v[0];
+                        }
+                    }
                 }
             }
 #pragma unroll
@@ -516,7 +528,7 @@ __global__ void __launch_bounds__(kReduceBlock, PAIRS && N == 8 ? 2 : 3) reduce_
                 }
             }
             __syncwarp();
-            if constexpr (N > 1) {                              // into the places that have just been read
+            if constexpr (ALIGNED) {                              // into the places that have just been read
                 const uint32_t k1 = k0 + ahead;
                 if (k1 < team) fetch(now, adds, twos, some, k1);
                 else fetch(next, next_adds, next_twos, next_some, k1 - team);
@@ -546,7 +558,8 @@ __device__ __forceinline__ uint32_t row_end(const uint2* entry, uint32_t at, uin
 }
 
 // Blocks below `combine_blocks` add up the parts of the rows that the owners name: a warp each, and all warps of the block a slice
-// each where a row has more parts than the block has warps.  The other blocks clear the rows that no entry names, a warp for 32 of them.
+// each where a row has more parts than the block has warps (200,000 entries on 30 rows of 336: 77 us in all, 234 when neighbouring owners
+// shared a block).  The other blocks clear the rows that no entry names, a warp for 32 of them.
 template <int N> __device__ __forceinline__ void add_parts(const Space& s, uint32_t first, uint32_t end, uint32_t col, float (&sum)[N]) {
 #pragma unroll 16
     for (uint32_t q = first; q < end; q++) {
@@ -556,9 +569,10 @@ template <int N> __device__ __forceinline__ void add_parts(const Space& s, uint3
     }
 }
 
-template <typename Out, int N>
+template <typename Out, bool ALIGNED>
 __global__ void __launch_bounds__(kCombineBlock, 2) combine_kernel(const Job j, const Space s, const uint2* entry, uint32_t combine_blocks) {
     constexpr uint32_t kWarps = kCombineBlock / 32;
+    constexpr int N = 4;                                        // parts lie in rows of whole pieces, whatever the output's do
     follow();
     const uint32_t lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     if (blockIdx.x >= combine_blocks) {
@@ -570,11 +584,12 @@ __global__ void __launch_bounds__(kCombineBlock, 2) combine_kernel(const Job j, 
             todo &= todo - 1;
             const bool second = r >= j.rows[0];
             Out* const at = static_cast<Out*>(second ? j.out[1] : j.out[0]) + (size_t)(second ? r - j.rows[0] : r) * (second ? j.out_stride[1] : j.out_stride[0]);
-            for (uint32_t c = lane * N; c < j.width; c += 32 * N) {
-                Piece<Out, N> zero;
+            constexpr int kZeros = ALIGNED ? N : 1;
+            for (uint32_t c = lane * kZeros; c < j.width; c += 32 * kZeros) {
+                Piece<Out, kZeros> zero;
 #pragma unroll
-                for (int k = 0; k < N; k++) zero.v[k] = from_float<Out>(0.f);
-                store_piece<Out, N>(at + c, zero);
+                for (int k = 0; k < kZeros; k++) zero.v[k] = from_float<Out>(0.f);
+                store_piece<Out, kZeros>(at + c, zero);
             }
         }
         return;
@@ -582,11 +597,12 @@ __global__ void __launch_bounds__(kCombineBlock, 2) combine_kernel(const Job j, 
     __shared__ float slice[kWarps][32 * N];
     __shared__ uint32_t long_chunk[kWarps], long_count[kWarps], long_row[kWarps], n_long;
     const uint32_t owners = *s.n_owners, size = 1u << j.chunk_log2;
-    for (uint32_t o0 = blockIdx.x * kWarps; o0 < owners; o0 += combine_blocks * kWarps) {
+    for (uint32_t o0 = blockIdx.x; o0 < owners; o0 += combine_blocks * kWarps) {      // a block's warps take owners far apart: few owners, a block each
+        const uint32_t o = o0 + warp * combine_blocks;
         if (threadIdx.x == 0) n_long = 0;
         __syncthreads();
-        if (o0 + warp < owners) {
-            const uint2 owner = s.owners[o0 + warp];
+        if (o < owners) {
+            const uint2 owner = s.owners[o];
             const uint32_t chunk = owner.x, row = owner.y, first = (chunk + 1) << j.chunk_log2;
             // Chunks that follow with a part of the row.  Most rows end soon: lane q looks whether the row goes on in parts behind q chunks more.
             const uint64_t at = (uint64_t)first + (uint64_t)lane * size + size / 4;
@@ -604,7 +620,7 @@ __global__ void __launch_bounds__(kCombineBlock, 2) combine_kernel(const Job j, 
 #pragma unroll
                     for (int k = 0; k < N; k++) sum[k] = s.tail[(size_t)chunk * s.pitch + c + k];
                     add_parts<N>(s, chunk + 1, chunk + 1 + count, c, sum);
-                    write_row<Out, N>(j, row, c, sum);
+                    write_row<Out, N, ALIGNED>(j, row, c, 1, sum);
                 }
             }
         }
@@ -629,7 +645,7 @@ __global__ void __launch_bounds__(kCombineBlock, 2) combine_kernel(const Job j, 
                     for (int w = 1; w < (int)kWarps; w++)
 #pragma unroll
                         for (int k = 0; k < N; k++) sum[k] += slice[w][lane * N + k];
-                    write_row<Out, N>(j, long_row[l], c, sum);
+                    write_row<Out, N, ALIGNED>(j, long_row[l], c, 1, sum);
                 }
                 __syncthreads();
             }
@@ -748,33 +764,33 @@ cudaError_t sort_entries(const Job& j, const Space& s, int* which, cudaStream_t 
     return cudaSuccess;
 }
 
-template <typename T, typename Out, int N, bool PAIRS>
+template <typename T, typename Out, int N, bool PAIRS, bool ALIGNED>
 cudaError_t sum_pieces(const Job& j, const Space& s, int which, cudaStream_t st) {
     const uint32_t pieces = (j.width + N - 1) / N;
     int log2 = 3;
     while (log2 < 5 && (1u << log2) < pieces) log2++;
     const uint32_t teams_per_block = kReduceBlock >> log2;
     const dim3 grid((s.chunks + teams_per_block - 1) / teams_per_block, (pieces + (1u << log2) - 1) >> log2);
-    const uint32_t combine_blocks = s.chunks > 1 ? std::min<uint32_t>((s.chunks + kCombineBlock / 32 - 1) / (kCombineBlock / 32), 2 * current_sms()) : 0;
+    const uint32_t combine_blocks = s.chunks > 1 ? std::min<uint32_t>(s.chunks - 1, 2 * current_sms()) : 0;
     const uint32_t clear_blocks = j.accumulate ? 0 : (uint32_t)(((uint64_t)j.total + kCombineBlock - 1) / kCombineBlock);
     if (j.n) {
         static LaunchCache cache;
-        constexpr size_t smem = Ring<T, N, PAIRS>::smem;
-        cudaError_t e = allow_smem(reduce_kernel<T, Out, N, PAIRS>, smem, cache);
+        constexpr size_t smem = Ring<T, N, PAIRS, ALIGNED>::smem;
+        cudaError_t e = allow_smem(reduce_kernel<T, Out, N, PAIRS, ALIGNED>, smem, cache);
         if (e != cudaSuccess) return e;
-        e = launch_behind(reduce_kernel<T, Out, N, PAIRS>, grid, kReduceBlock, smem, st, j, s, (const uint2*)s.entry[which], log2);
+        e = launch_behind(reduce_kernel<T, Out, N, PAIRS, ALIGNED>, grid, kReduceBlock, smem, st, j, s, (const uint2*)s.entry[which], log2);
         if (e == cudaSuccess && combine_blocks + clear_blocks)
-            e = launch_behind(combine_kernel<Out, (N < 4 ? N : 4)>, combine_blocks + clear_blocks, kCombineBlock, 0, st, j, s, (const uint2*)s.entry[which], combine_blocks);
+            e = launch_behind(combine_kernel<Out, ALIGNED>, combine_blocks + clear_blocks, kCombineBlock, 0, st, j, s, (const uint2*)s.entry[which], combine_blocks);
         if (e != cudaSuccess) return e;
-    } else if (clear_blocks) combine_kernel<Out, (N < 4 ? N : 4)><<<clear_blocks, kCombineBlock, 0, st>>>(j, s, static_cast<const uint2*>(nullptr), 0u);
+    } else if (clear_blocks) combine_kernel<Out, ALIGNED><<<clear_blocks, kCombineBlock, 0, st>>>(j, s, static_cast<const uint2*>(nullptr), 0u);
     return cudaGetLastError();
 }
 
 // `pieces`: elements that all rows may be moved in.
 template <typename T, typename Out, bool PAIRS>
 cudaError_t sum_entries(const Job& j, const Space& s, int which, uint32_t pieces, cudaStream_t st) {
-    if (sizeof(T) == 2 && pieces == 8) return sum_pieces<T, Out, (sizeof(T) == 2 ? 8 : 4), PAIRS>(j, s, which, st);
-    return pieces >= 4 ? sum_pieces<T, Out, 4, PAIRS>(j, s, which, st) : sum_pieces<T, Out, 1, PAIRS>(j, s, which, st);
+    if (sizeof(T) == 2 && pieces == 8) return sum_pieces<T, Out, (sizeof(T) == 2 ? 8 : 4), PAIRS, true>(j, s, which, st);
+    return pieces >= 4 ? sum_pieces<T, Out, 4, PAIRS, true>(j, s, which, st) : sum_pieces<T, Out, 4, PAIRS, false>(j, s, which, st);
 }
 uint32_t pieces_of(std::initializer_list<const mascot_rows*> all) {
     uint32_t n = 8;
