@@ -43,7 +43,7 @@ template <int CN, Mode MODE> struct Shape {
     static constexpr int stage_bytes = kLaneTileBytes + CN * kScaleBlock;
     static constexpr int step_scales = kLanes + (MODE == SQUARE ? 4 : CN);
     static constexpr int transit = MODE == SQUARE ? readers * 32 * kStagePitch : MODE == ONE && CN > 16 ? groups * 2 * 16 * kLanes * 4 : 0;
-    static constexpr size_t smem = 1024 + (size_t)stages * stage_bytes + transit + kScaleSteps * step_scales * 4 + 8 * (2 * stages + 2 * buffers + 2 * kScaleSteps) + 16;
+    static constexpr size_t smem = 1024 + (size_t)stages * stage_bytes + transit + kScaleSteps * step_scales * 4 + 8 * (2 * stages + 2 * buffers + 3 * kScaleSteps) + 16;
     static_assert(smem <= 227 * 1024, "shared memory of a block");
 };
 
@@ -51,12 +51,16 @@ template <int CN, Mode MODE> struct Shape {
 struct Side {
     const float* scale;
     uint32_t rows, scales, shift;                    // scales of a column block, rows to a scale (log2)
+    const uint8_t* row_data;
+    size_t stride;                                   // bytes
+    __device__ float of(uint32_t block, uint32_t row) const { return __ldg(scale + (size_t)block * scales + (row >> shift)); }
 };
 struct ProductArgs {
     Side lane, col;
     void* out;
     size_t lane_step, col_step;                      // elements of `out` from one row of a side to the next
     uint32_t blocks, user_tiles, tiles;              // blocks of 128 columns
+    uint32_t width;                                  // columns
     uint32_t* flags;
 };
 
@@ -147,6 +151,41 @@ __device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) { u
 
 __device__ __forceinline__ float half_of(uint64_t pair, int which) { return __uint_as_float((uint32_t)(pair >> 32 * which)); }
 
+// Scales may be any numbers of fp32, and a step on the way may leave its range where the score does not.  A block's sum x is 0 or between 2^-18
+// and 2^25 in magnitude (128 products of e4m3 values, multiples of 2^-9 and at most 448): times a scale of 2^-100 to 2^100 it is a normal
+// number, and times the other scale it is the block's part of the score.  So the first factor decides: the lane's scale, or in SQUARE the
+// product of both.  Where it is a far one the score is worked out a second time, from its rows.
+__device__ __forceinline__ bool is_far(float lane_scale) {
+    const uint32_t m = __float_as_uint(lane_scale) & 0x7fffffffu;
+    return m != 0 && m - (27u << 23) > (200u << 23);
+}
+__device__ __forceinline__ bool is_far(float lane_scale, float col_scale) {
+    const uint32_t m = __float_as_uint(lane_scale * col_scale) & 0x7fffffffu;
+    return m - (1u << 23) >= (254u << 23) && lane_scale != 0.f && col_scale != 0.f;
+}
+
+// One score with its scales applied in fp64, from rows that start on 16 bytes.
+__device__ __forceinline__ float exact_score(const ProductArgs& p, uint32_t l, uint32_t c) {
+    const uint8_t* const x = p.lane.row_data + l * p.lane.stride, *const y = p.col.row_data + c * p.col.stride;
+    float sum = 0.f;
+#pragma unroll 1
+    for (uint32_t b = 0; b < p.blocks; b++) {
+        const uint32_t end = min(p.width, (b + 1) * kScaleBlock);
+        float dot = 0.f;
+        uint32_t k = b * kScaleBlock;
+#pragma unroll 1
+        for (; k + 16 <= end; k += 16) {
+            const Piece<E4m3, 16> u = load_piece<E4m3, 16>(reinterpret_cast<const E4m3*>(x + k)), v = load_piece<E4m3, 16>(reinterpret_cast<const E4m3*>(y + k));
+#pragma unroll
+            for (int i = 0; i < 16; i++) dot = fmaf(as_float(u.v[i]), as_float(v.v[i]), dot);
+        }
+#pragma unroll 1
+        for (; k < end; k++) dot = fmaf(as_float(load_piece<E4m3, 1>(reinterpret_cast<const E4m3*>(x + k)).v[0]), as_float(load_piece<E4m3, 1>(reinterpret_cast<const E4m3*>(y + k)).v[0]), dot);
+        sum += __double2float_rn((double)dot * p.lane.of(b, l) * p.col.of(b, c));
+    }
+    return sum;
+}
+
 // Stores N columns of the warp's lanes, two to an element of v, at the offsets `at` from an address that is the same for the warp.
 template <typename Out, int N>
 __device__ __forceinline__ void store_columns(uint8_t* base, const uint32_t* at, const uint64_t* v, bool there, int cols) {
@@ -224,13 +263,13 @@ __global__ void __launch_bounds__(Shape<CN, MODE>::threads, 1) product_kernel(co
     float* const scales = reinterpret_cast<float*>(transit + S::transit);                                            // [kScaleSteps][columns', lanes']
     uint64_t* const full = reinterpret_cast<uint64_t*>(scales + kScaleSteps * S::step_scales), *const empty = full + kStages;
     uint64_t* const ready = empty + kStages, *const spare = ready + kBuffers;                                        // accumulators: summed, read back
-    uint64_t* const scaled = spare + kBuffers, *const used = scaled + kScaleSteps;                                   // scales: there, used
-    uint32_t* const tmem_slot = reinterpret_cast<uint32_t*>(used + kScaleSteps);
+    uint64_t* const fetched = spare + kBuffers, *const judged = fetched + kScaleSteps, *const used = judged + kScaleSteps;      // scales: there, looked at, used
+    uint32_t* const tmem_slot = reinterpret_cast<uint32_t*>(used + kScaleSteps), *const any_far = tmem_slot + 1;
     const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;     // the same for the warp, and known to be
     if (threadIdx.x == 0) {
         for (int s = 0; s < kStages; s++) { barrier_init(full + s, 1); barrier_init(empty + s, 1); }
         for (int b = 0; b < kBuffers; b++) { barrier_init(ready + b, 1); barrier_init(spare + b, S::readers); }
-        for (int s = 0; s < kScaleSteps; s++) { barrier_init(scaled + s, 32); barrier_init(used + s, S::readers); }
+        for (int s = 0; s < kScaleSteps; s++) { barrier_init(fetched + s, 32); barrier_init(judged + s, 1); barrier_init(used + s, S::readers); }
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
     if (warp == 0) {
@@ -246,7 +285,7 @@ __global__ void __launch_bounds__(Shape<CN, MODE>::threads, 1) product_kernel(co
     const auto item_of = [&](uint32_t t) { return t / p.user_tiles * (MODE == SQUARE ? CN : kLanes); };
     const auto lane_of = [&](uint32_t t) { return MODE == SQUARE ? user_of(t) : item_of(t); };
     const auto col_of = [&](uint32_t t) { return MODE == SQUARE ? item_of(t) : user_of(t); };
-
+    const auto scores_stored = [&]() { asm volatile("bar.sync %0, %1;" ::"n"(1 + S::groups), "n"(S::threads) : "memory"); };      // the whole block meets, from both branches
     if (warp >= S::readers) {
         // Where sums take registers, 384 threads are launched with 168 each; those that hold sums take what the others leave: 128 * 56 + 256 * 224
         if (MODE != ONE) asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
@@ -307,12 +346,42 @@ __global__ void __launch_bounds__(Shape<CN, MODE>::threads, 1) product_kernel(co
                     }
 #pragma unroll
                     for (int k = lane; k < kLanes; k += 32) fetch(to + S::step_scales - kLanes + k, of_lanes, p.lane, lane0 + k);
-                    asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(smem_at(scaled + q)) : "memory");
+                    asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(smem_at(fetched + q)) : "memory");
                 }
             }
             asm volatile("cp.async.wait_all;" ::: "memory");
         }
+        if (warp == S::readers + 3) {                           // looks for far scales ahead of the readers, whom a look and a branch of their own cost a fifth
+            bool far = false;                                   // of any step
+            for (uint32_t t = blockIdx.x; ok && t < p.tiles; t += gridDim.x)
+                for (uint32_t c = 0; c < p.blocks; c++, step++) {
+                    const int q = step % kScaleSteps;
+                    if (!(ok = wait(fetched + q, step / kScaleSteps & 1))) break;
+                    const float* const of_cols = scales + q * S::step_scales, *const of_lanes = of_cols + S::step_scales - kLanes;
+#pragma unroll
+                    for (int k = lane; k < kLanes; k += 32) {
+                        if (MODE == SQUARE) {
+#pragma unroll
+                            for (int g = 0; g < S::groups; g++) far |= is_far(of_lanes[k], of_cols[g]);
+                        } else far |= is_far(of_lanes[k]);
+                    }
+                    __syncwarp();
+                    if (lane == 0) barrier_arrive(judged + q);
+                }
+            far = __any_sync(0xffffffffu, far);
+            if (lane == 0) *any_far = far;
+        }
         if (!ok && lane == 0 && p.flags) atomicOr(p.flags, (uint32_t)MASCOT_FLAG_GAVE_UP);
+        scores_stored();
+        if (*any_far)
+            for (uint32_t t = blockIdx.x; t < p.tiles; t += gridDim.x)
+                for (uint32_t i = threadIdx.x - 32 * S::readers; i < kLanes * CN; i += S::threads - 32 * S::readers) {
+                    const uint32_t l = lane_of(t) + i % kLanes, c = col_of(t) + i / kLanes;
+                    bool far = false;
+                    if (l < p.lane.rows && c < p.col.rows)
+                        for (uint32_t b = 0; b < p.blocks && !far; b++) far = MODE == SQUARE ? is_far(p.lane.of(b, l), p.col.of(b, c)) : is_far(p.lane.of(b, l));
+                    if (far) static_cast<Out*>(p.out)[l * p.lane_step + c * p.col_step] = from_float<Out>(exact_score(p, l, c));
+                }
     } else {                                                    // sums and scores
         if (MODE != ONE) asm volatile("setmaxnreg.inc.sync.aligned.u32 224;");
         const int group = warp / 4;
@@ -340,7 +409,7 @@ __global__ void __launch_bounds__(Shape<CN, MODE>::threads, 1) product_kernel(co
                 const int b = step % kBuffers, q = step % kScaleSteps;
                 const float* const scale = scales + q * S::step_scales;
                 const uint32_t from = tmem + (lanes << 16) + b * CN + group * kGroup;
-                ok = __all_sync(0xffffffffu, ok && barrier_wait(scaled + q, step / kScaleSteps & 1) && barrier_wait(ready + b, step / kBuffers & 1));
+                ok = __all_sync(0xffffffffu, ok && barrier_wait(judged + q, step / kScaleSteps & 1) && barrier_wait(ready + b, step / kBuffers & 1));
                 fence_after();
                 float lane_scale = scale[S::step_scales - kLanes + lanes + lane];
                 if (MODE == SQUARE) lane_scale *= scale[group];
@@ -429,6 +498,7 @@ __global__ void __launch_bounds__(Shape<CN, MODE>::threads, 1) product_kernel(co
             if constexpr (MODE == SQUARE) store_rows<Out, kGroup>(sum, transit + warp * 32 * kStagePitch, reinterpret_cast<Out*>(out), p.lane_step, rows, cols, lane);
         }
         if (!ok && lane == 0 && p.flags) atomicOr(p.flags, (uint32_t)MASCOT_FLAG_GAVE_UP);
+        scores_stored();
         fence_before();
     }
     __syncthreads();
@@ -536,10 +606,10 @@ extern "C" int mascot_rows_product(const mascot_rows* a, const float* a_scale, c
     ROW_CHECK(check_memory("flags", flags, device));
     if (!encode_tiled()) return fail(nullptr, MASCOT_ERR_UNSUPPORTED, "the driver has no cuTensorMapEncodeTiled");
     ProductArgs p = {};
-    p.lane = Side{b_scale, (uint32_t)b->rows, n_scales, b_block_rows == 1 ? 0u : 7u};
-    p.col = Side{a_scale, (uint32_t)a->rows, (uint32_t)a->rows, 0};
+    p.lane = Side{b_scale, (uint32_t)b->rows, n_scales, b_block_rows == 1 ? 0u : 7u, static_cast<const uint8_t*>(b->data), b->stride};
+    p.col = Side{a_scale, (uint32_t)a->rows, (uint32_t)a->rows, 0, static_cast<const uint8_t*>(a->data), a->stride};
     p.out = out->data; p.lane_step = 1; p.col_step = out->stride;
-    p.blocks = col_blocks;
+    p.width = a->width; p.blocks = col_blocks;
     p.flags = flags;
     const cudaError_t launched = with_type(out->type, [&](auto* o) { return launch_tiles<std::remove_pointer_t<decltype(o)>>(*a, *b, p, static_cast<cudaStream_t>(stream)); });
     CU(nullptr, launched);

@@ -495,7 +495,9 @@ MASCOT_API int mascot_rows_quantize(const mascot_rows* x, uint32_t block_rows, c
 /* Scores of all pairs of rows: out[m][n] = sum over column blocks c of a_scale * b_scale * (sum of a[m] * b[n] within c), for two
  * matrices of MASCOT_E4M3 of one width with any fp32 scales in the layout of mascot_rows_quantize: a with a scale for each row
  * and block of 128 columns, b with b_block_rows = 1 or 128 rows to a scale.  Products of a block are summed by the tensor
- * cores, blocks in fp32.  a and b: base and stride multiples of 16 bytes; out: a_rows x b_rows, any type but MASCOT_E4M3, stride below 2^26.
+ * cores, blocks in fp32.  Whatever the scales are, a score is right where its parts and their sums are numbers of fp32; a row of b
+ * whose scale is outside of 2^-100 .. 2^100 (128 rows to a scale: a product a_scale * b_scale that is no normal number) takes a slower way.
+ * a and b: base and stride multiples of 16 bytes; out: a_rows x b_rows, any type but MASCOT_E4M3, stride below 2^26.
  * Should a wait inside the kernel run out, MASCOT_FLAG_GAVE_UP is set in *flags and the scores it concerns are NaN. */
 MASCOT_API int mascot_rows_product(const mascot_rows* a, const float* a_scale, const mascot_rows* b, const float* b_scale,
                                    uint32_t b_block_rows, const mascot_rows* out, uint32_t* flags, void* stream);
