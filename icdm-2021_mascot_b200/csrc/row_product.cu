@@ -21,6 +21,7 @@
 
 #include <algorithm>
 
+#include "reader.h"
 #include "row_ops.h"
 
 namespace mascot {
@@ -200,10 +201,7 @@ __device__ __forceinline__ void store_columns(uint8_t* base, const uint32_t* at,
 
 // Stores R rows of 128 scores, fp32 in shared memory, each times its scale: a warp, WIDE neighbours a lane.
 template <typename Out, int R, int WIDE>
-__device__ __forceinline__ void store_whole(uint8_t* to, size_t pitch, const float* from, const float* scale, int lane) {
-    float s[R];
-#pragma unroll
-    for (int r = 0; r < R; r++) s[r] = scale[r];
+__device__ __forceinline__ void store_whole(uint8_t* to, size_t pitch, const float* from, const float (&s)[R], int lane) {
 #pragma unroll
     for (int r = 0; r < R; r++, to += pitch) {
 #pragma unroll
@@ -399,7 +397,7 @@ __global__ void __launch_bounds__(Shape<CN, MODE>::threads, 1) product_kernel(co
         float* chunk = reinterpret_cast<float*>(transit) + group * 2 * kRead * kLanes;
         bool turn = false;
         uint32_t step = 0;
-        bool ok = true;
+        Reader reader;
         for (uint32_t t = blockIdx.x; t < p.tiles; t += gridDim.x) {
             const uint32_t l = lane_of(t) + lanes, c0 = col_of(t) + group * kGroup;      // the warp's first lane and column
             uint8_t* const out = static_cast<uint8_t*>(p.out) + (l * p.lane_step + c0 * p.col_step) * sizeof(Out);
@@ -409,16 +407,16 @@ __global__ void __launch_bounds__(Shape<CN, MODE>::threads, 1) product_kernel(co
                 const int b = step % kBuffers, q = step % kScaleSteps;
                 const float* const scale = scales + q * S::step_scales;
                 const uint32_t from = tmem + (lanes << 16) + b * CN + group * kGroup;
-                ok = __all_sync(0xffffffffu, ok && barrier_wait(judged + q, step / kScaleSteps & 1) && barrier_wait(ready + b, step / kBuffers & 1));
+                reader.waited(__all_sync(0xffffffffu, reader.ok() && barrier_wait(judged + q, step / kScaleSteps & 1) && barrier_wait(ready + b, step / kBuffers & 1)));
                 fence_after();
                 float lane_scale = scale[S::step_scales - kLanes + lanes + lane];
                 if (MODE == SQUARE) lane_scale *= scale[group];
-                if (!ok) lane_scale = __int_as_float(0x7fffffff);
+                lane_scale = reader.factor(lane_scale);
                 const uint64_t lane_scales = pair_of(lane_scale, lane_scale);
                 const auto release = [&]() {                    // the accumulator has been read
                     fence_before();
                     __syncwarp();
-                    if (lane == 0) barrier_arrive(spare + b);
+                    if (lane == 0) reader.hand_back([&] { barrier_arrive(spare + b); });
                 };
                 if constexpr (MODE == ONE && CN == 16) {        // few users: a store of 32 scores for each, and no meeting
                     if (cols > 0) {
@@ -451,13 +449,19 @@ __global__ void __launch_bounds__(Shape<CN, MODE>::threads, 1) product_kernel(co
                         else release();
                         asm volatile("bar.sync %0, 128;" ::"r"(1 + group) : "memory");     // one a chunk: its half of `transit` is written again two chunks on
                         const float* const rows_at = chunk + row0 * kLanes;
+                        float s[kRows];
+#pragma unroll
+                        for (int r = 0; r < kRows; r++) s[r] = reader.factor(of_rows[r]);
                         if (items == kLanes && left >= kRows) {
-                            if (wide == 4) store_whole<Out, kRows, 4>(row, pitch, rows_at, of_rows, lane);
-                            else if (sizeof(Out) == 2 && wide == 2) store_whole<Out, kRows, 2>(row, pitch, rows_at, of_rows, lane);
-                            else store_whole<Out, kRows, 1>(row, pitch, rows_at, of_rows, lane);
+                            if (wide == 4) store_whole<Out, kRows, 4>(row, pitch, rows_at, s, lane);
+                            else if (sizeof(Out) == 2 && wide == 2) store_whole<Out, kRows, 2>(row, pitch, rows_at, s, lane);
+                            else store_whole<Out, kRows, 1>(row, pitch, rows_at, s, lane);
                         } else {
-                            for (int r = 0; r < min(kRows, left); r++)
-                                for (int i = lane; i < items; i += 32) reinterpret_cast<Out*>(row + r * pitch)[i] = from_float<Out>(rows_at[r * kLanes + i] * of_rows[r]);
+#pragma unroll
+                            for (int r = 0; r < kRows; r++) {
+                                if (r >= left) break;
+                                for (int i = lane; i < items; i += 32) reinterpret_cast<Out*>(row + r * pitch)[i] = from_float<Out>(rows_at[r * kLanes + i] * s[r]);
+                            }
                         }
                         chunk = turn ? chunk - kRead * kLanes : chunk + kRead * kLanes;
                         turn = !turn;
@@ -486,7 +490,7 @@ __global__ void __launch_bounds__(Shape<CN, MODE>::threads, 1) product_kernel(co
                     }
                 }
                 __syncwarp();
-                if (lane == 0) barrier_arrive(used + q);
+                if (lane == 0) reader.hand_back([&] { barrier_arrive(used + q); });
             }
             if constexpr (MODE == ROWS) {
 #pragma unroll
@@ -497,7 +501,7 @@ __global__ void __launch_bounds__(Shape<CN, MODE>::threads, 1) product_kernel(co
             }
             if constexpr (MODE == SQUARE) store_rows<Out, kGroup>(sum, transit + warp * 32 * kStagePitch, reinterpret_cast<Out*>(out), p.lane_step, rows, cols, lane);
         }
-        if (!ok && lane == 0 && p.flags) atomicOr(p.flags, (uint32_t)MASCOT_FLAG_GAVE_UP);
+        if (!reader.ok() && lane == 0 && p.flags) atomicOr(p.flags, (uint32_t)MASCOT_FLAG_GAVE_UP);
         scores_stored();
         fence_before();
     }

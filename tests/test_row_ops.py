@@ -200,3 +200,23 @@ def test_tensors_off_the_gpu_are_refused(mascot):
         with pytest.raises(mascot.MascotError) as e:
             f()
         assert e.value.status == mascot.ERR_BAD_ARG and "GPU" in str(e.value)
+
+
+def test_a_reader_that_gave_up_spoils_nothing(tmp_path):
+    """csrc/reader.h, the rule of the scores' kernel for a warp whose wait ran out: whatever the order in which warps take their turns, what
+    the others store is right or NaN, and all come to their end.  Going on as if nothing had been leaves wrong finite scores."""
+    import os
+    import subprocess
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    exe = str(tmp_path / "reader_check")
+    subprocess.check_call(["g++", "-O1", "-std=c++17", "-I", os.path.join(root, "icdm-2021_mascot_b200", "csrc"), os.path.join(root, "tests", "reader_check.cpp"), "-o", exe])
+
+    def run(rule, barrier, group):
+        return [int(x) for x in subprocess.run([exe, rule, str(barrier), str(group)], capture_output=True, text=True, check=True).stdout.split()]
+    for group in (1, 2, 4):
+        whole = run("reader", -1, group)
+        assert whole[:2] == [0, 0] and whole[2] == 400 * 40 * 4 * group              # nothing gives up: all scores, all right
+        for barrier in (0, 1):
+            wrong, nan, right = run("reader", barrier, group)
+            assert wrong == 0 and nan > 0 and right > 0 and nan + right == whole[2]
+    assert run("always", 0, 1)[0] > 0 and run("always", 1, 2)[0] > 0
