@@ -832,6 +832,7 @@ int mascot_rows_gradient(const mascot_rows* grad, const mascot_ids* ids, float s
     ROW_CHECK(check_ids("ids", ids));
     ROW_CHECK(check_rows("out", out, false));
     if (grad->width != out->width) return fail(nullptr, MASCOT_ERR_BAD_ARG, "out: width is not the gradient's");
+    ROW_CHECK(check_words("flags", flags));
     if (grad->rows != ids->count) return fail(nullptr, MASCOT_ERR_BAD_ARG, "grad: must have a row for each id");
     ROW_CHECK(check_workspace(ids->count, out->rows, out->width, false, workspace, workspace_bytes));
     const size_t id_bytes = ids->count * ids->bits / 8;
@@ -891,7 +892,8 @@ int mascot_pair_gradient(const mascot_rows* P, const mascot_rows* Q, const masco
     const uint64_t n = users->count, total = P->rows + Q->rows;
     if (3 * n >= kMaxRows || total >= kMaxRows) return fail(nullptr, MASCOT_ERR_BAD_ARG, "three times the pairs, and the rows of both tables, must be below 2^31 - 1");
     if (n && !coef) return fail(nullptr, MASCOT_ERR_BAD_ARG, "coef: null pointer");
-    if (reinterpret_cast<uintptr_t>(coef) % 4) return fail(nullptr, MASCOT_ERR_BAD_ARG, "coef: address is not a multiple of the element's size");
+    ROW_CHECK(check_words("coef", coef));
+    ROW_CHECK(check_words("flags", flags));
     ROW_CHECK(check_workspace(3 * n, total, P->width, true, workspace, workspace_bytes));
     ROW_CHECK(check_distinct("dP", dP, "dQ", dQ));
     for (const auto* out : {dP, dQ}) {

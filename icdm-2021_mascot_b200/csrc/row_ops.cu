@@ -73,6 +73,10 @@ int check_distinct(const char* what_a, const void* a, size_t bytes_a, const char
     return check_distinct(what_a, a, bytes_a, what_b, b->data, s.end - s.begin);
 }
 
+int check_words(const char* what, const void* p) {
+    return reinterpret_cast<uintptr_t>(p) % 4 ? refuse(MASCOT_ERR_BAD_ARG, what, "address is not a multiple of the element's size") : MASCOT_OK;
+}
+
 int check_device(int* device) {
     if (cudaGetDevice(device) == cudaSuccess) return MASCOT_OK;
     cudaGetLastError();
@@ -389,6 +393,8 @@ int mascot_rows_lookup(const mascot_rows* table, const float* table_scale, uint3
     if (e4m3 && (block_rows != 1 && block_rows != kScaleBlock)) return fail(nullptr, MASCOT_ERR_BAD_ARG, "block_rows must be 1 or 128");
     if (e4m3 && !table_scale && table->rows) return fail(nullptr, MASCOT_ERR_BAD_ARG, "table_scale: null pointer");
     if (!e4m3 && (table_scale || block_rows)) return fail(nullptr, MASCOT_ERR_BAD_ARG, "table_scale and block_rows belong to a table of MASCOT_E4M3");
+    ROW_CHECK(check_words("table_scale", table_scale));
+    ROW_CHECK(check_words("flags", flags));
     const uint64_t row_blocks = e4m3 ? (table->rows + block_rows - 1) / block_rows : 0;
     ROW_CHECK(check_distinct("table", table, "out", out));
     ROW_CHECK(check_distinct("ids", ids->data, ids->count * ids->bits / 8, "out", out));
@@ -432,8 +438,11 @@ int mascot_pair_loss(const mascot_rows* P, const mascot_rows* Q, const mascot_id
     struct { const char* what; const void* p; size_t bytes; } in[] = {{"users", users->data, n * users->bits / 8}, {"preferred", preferred->data, n * preferred->bits / 8},
         {"other", other->data, n * other->bits / 8}, {"reference", reference, vector}, {"weight", weight, vector}, {"flags", flags, 4}},
         out[] = {{"loss", loss, vector}, {"margin", margin, vector}, {"coef", coef, vector}};
+    ROW_CHECK(check_words("reference", reference));
+    ROW_CHECK(check_words("weight", weight));
+    ROW_CHECK(check_words("flags", flags));
     for (int o = 0; o < 3; o++) {
-        if (reinterpret_cast<uintptr_t>(out[o].p) % 4) return fail(nullptr, MASCOT_ERR_BAD_ARG, "an output's address is not a multiple of the element's size");
+        ROW_CHECK(check_words(out[o].what, out[o].p));
         for (const auto& x : in) ROW_CHECK(check_distinct(x.what, x.p, x.bytes, out[o].what, out[o].p, vector));
         for (int q = 0; q < o; q++) ROW_CHECK(check_distinct(out[q].what, out[q].p, vector, out[o].what, out[o].p, vector));
         if (out[o].p) {
@@ -465,7 +474,7 @@ int mascot_rows_quantize(const mascot_rows* x, uint32_t block_rows, const mascot
     if (block_rows != 1 && block_rows != kScaleBlock) return fail(nullptr, MASCOT_ERR_BAD_ARG, "block_rows must be 1 or 128");
     if (is_empty(*x)) return MASCOT_OK;
     if (!scale) return fail(nullptr, MASCOT_ERR_BAD_ARG, "scale: null pointer");
-    if (reinterpret_cast<uintptr_t>(scale) % 4) return fail(nullptr, MASCOT_ERR_BAD_ARG, "scale: address is not a multiple of the element's size");
+    ROW_CHECK(check_words("scale", scale));
     const uint32_t col_blocks = (x->width + kScaleBlock - 1) / kScaleBlock, row_blocks = (uint32_t)((x->rows + block_rows - 1) / block_rows);
     const size_t scale_bytes = (size_t)col_blocks * row_blocks * 4;
     ROW_CHECK(check_distinct("x", x, "q", q));

@@ -25,6 +25,7 @@ int check_ids(const char* what, const mascot_ids* ids);
 int check_distinct(const char* what_a, const mascot_rows* a, const char* what_b, const mascot_rows* b);   // no element in common
 int check_distinct(const char* what_a, const void* a, size_t bytes_a, const char* what_b, const mascot_rows* b);
 int check_distinct(const char* what_a, const void* a, size_t bytes_a, const char* what_b, const void* b, size_t bytes_b);
+int check_words(const char* what, const void* p);                        // an address of 4-byte elements, or null
 int check_device(int* device);                                           // the current one (a launch refuses a stream of another one itself)
 int check_memory(const char* what, const void* p, int device);           // device memory of that device, or null
 int current_sms();                                                          // of the current device

@@ -590,8 +590,10 @@ extern "C" int mascot_rows_product(const mascot_rows* a, const float* a_scale, c
     if (out->type > MASCOT_BF16) return fail(nullptr, MASCOT_ERR_BAD_ARG, "out: must be MASCOT_F32, MASCOT_F16 or MASCOT_BF16");
     if (out->stride < out->width || out->stride >= (1ull << 26)) return fail(nullptr, MASCOT_ERR_BAD_ARG, "out: stride must be from the width to 2^26");
     if (!out->data || !a_scale || !b_scale) return fail(nullptr, MASCOT_ERR_BAD_ARG, "null pointer");
-    if (reinterpret_cast<uintptr_t>(out->data) % type_bytes(out->type) || reinterpret_cast<uintptr_t>(a_scale) % 4 || reinterpret_cast<uintptr_t>(b_scale) % 4)
-        return fail(nullptr, MASCOT_ERR_BAD_ARG, "an address is not a multiple of the element's size");
+    if (reinterpret_cast<uintptr_t>(out->data) % type_bytes(out->type)) return fail(nullptr, MASCOT_ERR_BAD_ARG, "out: address is not a multiple of the element's size");
+    ROW_CHECK(check_words("a_scale", a_scale));
+    ROW_CHECK(check_words("b_scale", b_scale));
+    ROW_CHECK(check_words("flags", flags));
     for (const auto* m : {a, b})
         if ((m->rows > 1 && m->stride % 16) || reinterpret_cast<uintptr_t>(m->data) % 16) return fail(nullptr, MASCOT_ERR_BAD_ARG, "a and b: base and stride must be multiples of 16 bytes");
     const uint32_t col_blocks = (a->width + kScaleBlock - 1) / kScaleBlock, n_scales = (uint32_t)((b->rows + b_block_rows - 1) / b_block_rows);

@@ -220,3 +220,29 @@ def test_a_reader_that_gave_up_spoils_nothing(tmp_path):
             wrong, nan, right = run("reader", barrier, group)
             assert wrong == 0 and nan > 0 and right > 0 and nan + right == whole[2]
     assert run("always", 0, 1)[0] > 0 and run("always", 1, 2)[0] > 0
+
+
+def test_odd_addresses_are_refused(mascot):
+    """Every pointer to 4-byte elements, the flag word of every entry included: a load or an atomic at an odd address would fault."""
+    M, lib = mascot, mascot.load()
+    t, i, o = rows(M, 10, 64), ids(M, 5), rows(M, 5, 64, at=1)
+    e4m3, g = rows(M, 10, 64, M.E4M3), rows(M, 5, 64, at=2)
+    u, p, n = ids(M, 5, 8), ids(M, 5, 9), ids(M, 5, 10)
+    dP, dQ = rows(M, 10, 64, at=3), rows(M, 10, 64, at=4)
+    a, b, s = rows(M, 5, 64, M.E4M3), rows(M, 10, 64, M.E4M3, 1), rows(M, 5, 10, M.BF16, 2)
+    x, q = rows(M, 10, 64, at=5), rows(M, 10, 64, M.E4M3, 6)
+    f = [AT + k * GAP for k in range(11, 16)]
+    calls = {                              # a call with its 4-byte pointers, in order; each name as in the messages
+        "lookup": (lambda w: lib.mascot_rows_lookup(e4m3, w[0], 1, i, 1.0, o, w[1], None), ["table_scale", "flags"]),
+        "gradient": (lambda w: lib.mascot_rows_gradient(g, i, 1.0, dP, 0, AT + 7 * GAP, 1 << 30, w[0], None), ["flags"]),
+        "loss": (lambda w: lib.mascot_pair_loss(t, t, u, p, n, 1.0, 0.0, w[0], w[1], w[2], None, None, w[3], None), ["reference", "weight", "loss", "flags"]),
+        "pairs": (lambda w: lib.mascot_pair_gradient(t, t, u, p, n, w[0], 1.0, dP, dQ, 0, AT + 7 * GAP, 1 << 30, w[1], None), ["coef", "flags"]),
+        "quantize": (lambda w: lib.mascot_rows_quantize(x, 1, q, w[0], None), ["scale"]),
+        "product": (lambda w: lib.mascot_rows_product(a, w[0], b, w[1], 1, s, w[2], None), ["a_scale", "b_scale", "flags"]),
+    }
+    for call, names in calls.values():
+        at = f[:len(names)]
+        reached_the_device(M, call(at))
+        for k, name in enumerate(names):
+            for off in (1, 2, 3):
+                refused(M, call(at[:k] + [at[k] + off] + at[k + 1:]), name, "address")
