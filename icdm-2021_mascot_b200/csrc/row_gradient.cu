@@ -17,7 +17,6 @@
 #include <algorithm>
 #include <initializer_list>
 
-#include "launch_cache.h"
 #include "row_ops.h"
 
 namespace mascot {
@@ -701,17 +700,7 @@ cudaError_t launch_behind(Kernel kernel, dim3 grid, unsigned block, size_t smem,
     behind[0].val.programmaticStreamSerializationAllowed = 1;
     config.attrs = behind;
     config.numAttrs = 1;
-    return cudaLaunchKernelEx(&config, kernel, args...);
-}
-
-// Raises a kernel's limit of dynamic shared memory, once for a device.
-template <class Kernel>
-cudaError_t allow_smem(Kernel kernel, size_t bytes, LaunchCache& cache) {
-    int dev = 0, fit = 0;
-    const cudaError_t e = cudaGetDevice(&dev);
-    if (e != cudaSuccess) return e;
-    return (cudaError_t)cache.lookup(dev, 0, 0, bytes, [&](size_t most) { return (int)cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)most); },
-                                     [](int, size_t, int*) { return 0; }, &fit);
+    return reported(cudaLaunchKernelEx(&config, kernel, args...));
 }
 
 // One digit of BITS bits: the first pass takes its entries from `key`.
@@ -726,12 +715,12 @@ cudaError_t sort_digit(const Job& j, const Space& s, int pass, cudaStream_t st) 
     const bool scanned = s.tiles > kScanTiles;
     uint2* const from = s.entry[pass & 1], *const to = s.entry[~pass & 1];
     const uint2* const none = nullptr;
-    if (pass == 0) count_kernel<true, ITEMS><<<s.tiles, kSortBlock, 0, st>>>(j, s, none, 0, BITS);
+    if (pass == 0) e = launch(count_kernel<true, ITEMS>, s.tiles, kSortBlock, 0, st, j, s, none, 0, BITS);
     else e = launch_behind(count_kernel<false, ITEMS>, s.tiles, kSortBlock, 0, st, j, s, (const uint2*)from, pass * BITS, BITS);
     if (e == cudaSuccess && scanned) e = launch_behind(scan_kernel, bins / 32, 1024, 0, st, s, bins);
     if (e == cudaSuccess && pass == 0) e = launch_behind(scatter_kernel<true, ITEMS, BITS>, s.tiles, kSortBlock, smem, st, s, j.n, none, to, 0, scanned);
     else if (e == cudaSuccess) e = launch_behind(scatter_kernel<false, ITEMS, BITS>, s.tiles, kSortBlock, smem, st, s, j.n, (const uint2*)from, to, pass * BITS, scanned);
-    return e == cudaSuccess ? cudaGetLastError() : e;
+    return e;
 }
 
 // Sorts the entries; *which tells which of the two buffers holds them.
@@ -751,7 +740,7 @@ cudaError_t sort_entries(const Job& j, const Space& s, int* which, cudaStream_t 
         config.attrs = cluster;
         config.numAttrs = 1;
         *which = (passes - 1) & 1;
-        return cudaLaunchKernelEx(&config, small_sort_kernel, j, s, passes);
+        return reported(cudaLaunchKernelEx(&config, small_sort_kernel, j, s, passes));
     }
     const bool ten = (key_bits + 9) / 10 < (key_bits + 7) / 8, many = j.n >= kManyFrom;      // wider digits where they save a pass
     const int passes = ten ? (key_bits + 9) / 10 : (key_bits + 7) / 8;
@@ -781,9 +770,9 @@ cudaError_t sum_pieces(const Job& j, const Space& s, int which, cudaStream_t st)
         e = launch_behind(reduce_kernel<T, Out, N, PAIRS, ALIGNED>, grid, kReduceBlock, smem, st, j, s, (const uint2*)s.entry[which], log2);
         if (e == cudaSuccess && combine_blocks + clear_blocks)
             e = launch_behind(combine_kernel<Out, ALIGNED>, combine_blocks + clear_blocks, kCombineBlock, 0, st, j, s, (const uint2*)s.entry[which], combine_blocks);
-        if (e != cudaSuccess) return e;
-    } else if (clear_blocks) combine_kernel<Out, ALIGNED><<<clear_blocks, kCombineBlock, 0, st>>>(j, s, static_cast<const uint2*>(nullptr), 0u);
-    return cudaGetLastError();
+        return e;
+    }
+    return clear_blocks ? launch(combine_kernel<Out, ALIGNED>, clear_blocks, kCombineBlock, 0, st, j, s, static_cast<const uint2*>(nullptr), 0u) : cudaSuccess;
 }
 
 // `pieces`: elements that all rows may be moved in.

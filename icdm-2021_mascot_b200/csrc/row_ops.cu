@@ -164,9 +164,7 @@ cudaError_t launch_lookup(const LookupArgs& a, bool aligned, cudaStream_t st) {
     while (log2 < 5 && (1u << log2) < pieces) log2++;
     const size_t teams = (a.n + kLookupRows - 1) / kLookupRows;
     const unsigned grid = (unsigned)((teams + (kLookupBlock >> log2) - 1) / (kLookupBlock >> log2));
-    if (aligned) lookup_kernel<In, Out, N><<<grid, kLookupBlock, 0, st>>>(a, log2);
-    else lookup_kernel<In, Out, 1><<<grid, kLookupBlock, 0, st>>>(a, log2);
-    return cudaGetLastError();
+    return aligned ? launch(lookup_kernel<In, Out, N>, grid, kLookupBlock, 0, st, a, log2) : launch(lookup_kernel<In, Out, 1>, grid, kLookupBlock, 0, st, a, log2);
 }
 
 // ---- preference loss -------------------------------------------------------------------------------------------
@@ -261,9 +259,7 @@ cudaError_t launch_pair_loss(const PairArgs& a, bool aligned, cudaStream_t st) {
     const uint32_t run = (uint32_t)std::min<size_t>(1u << log2, std::max<size_t>(kPairs, a.n / teams / kPairs * kPairs));
     const size_t runs = (a.n + run - 1) / run;
     const unsigned grid = (unsigned)((runs + (kPairBlock >> log2) - 1) / (kPairBlock >> log2));
-    if (aligned) pair_loss_kernel<T, N><<<grid, kPairBlock, 0, st>>>(a, log2, run);
-    else pair_loss_kernel<T, 1><<<grid, kPairBlock, 0, st>>>(a, log2, run);
-    return cudaGetLastError();
+    return aligned ? launch(pair_loss_kernel<T, N>, grid, kPairBlock, 0, st, a, log2, run) : launch(pair_loss_kernel<T, 1>, grid, kPairBlock, 0, st, a, log2, run);
 }
 
 // ---- quantisation ------------------------------------------------------------------------------------------
@@ -491,14 +487,8 @@ int mascot_rows_quantize(const mascot_rows* x, uint32_t block_rows, const mascot
     const cudaError_t launched = with_type(x->type, [&](auto* t) {
         using T = std::remove_pointer_t<decltype(t)>;
         const dim3 grid(block_rows == 1 ? (a.rows + kQuantWarps * kQuantRows - 1) / (kQuantWarps * kQuantRows) : row_blocks, col_blocks);
-        if (block_rows == 1) {
-            if (aligned) quantize_rows_kernel<T, true><<<grid, kQuantBlock, 0, st>>>(a);
-            else quantize_rows_kernel<T, false><<<grid, kQuantBlock, 0, st>>>(a);
-        } else {
-            if (aligned) quantize_square_kernel<T, true><<<grid, kSquareBlock, 0, st>>>(a);
-            else quantize_square_kernel<T, false><<<grid, kSquareBlock, 0, st>>>(a);
-        }
-        return cudaGetLastError();
+        if (block_rows == 1) return launch(aligned ? quantize_rows_kernel<T, true> : quantize_rows_kernel<T, false>, grid, kQuantBlock, 0, st, a);
+        return launch(aligned ? quantize_square_kernel<T, true> : quantize_square_kernel<T, false>, grid, kSquareBlock, 0, st, a);
     });
     CU(nullptr, launched);
     return MASCOT_OK;

@@ -10,6 +10,7 @@
 #include <new>
 
 #include "handle.h"
+#include "launch_cache.h"
 
 namespace mascot {
 
@@ -47,7 +48,35 @@ struct Ids {
 };
 inline Ids ids_of(const mascot_ids& ids) { return Ids{ids.data, ids.bits == 64}; }
 
+// Hands on what a CUDA call returned.  An error that is reported that way does not stay behind as the thread's last one as well, where the
+// next check of somebody else would find it.
+inline cudaError_t reported(cudaError_t e) {
+    if (e != cudaSuccess) cudaGetLastError();
+    return e;
+}
+
 #ifdef __CUDACC__
+// A launch with its own status: the thread's last error may be an old one of the caller's, which is not ours to report or to take away.
+template <class Kernel, class... Args>
+cudaError_t launch(Kernel kernel, dim3 grid, unsigned block, size_t smem, cudaStream_t st, Args... args) {
+    cudaLaunchConfig_t config = {};
+    config.gridDim = grid;
+    config.blockDim = dim3(block);
+    config.dynamicSmemBytes = smem;
+    config.stream = st;
+    return reported(cudaLaunchKernelEx(&config, kernel, args...));
+}
+
+// Raises a kernel's limit of dynamic shared memory, once for a device.
+template <class Kernel>
+cudaError_t allow_smem(Kernel kernel, size_t bytes, LaunchCache& cache) {
+    int dev = 0, fit = 0;
+    const cudaError_t e = cudaGetDevice(&dev);
+    if (e != cudaSuccess) return reported(e);
+    return (cudaError_t)cache.lookup(dev, 0, 0, bytes, [&](size_t most) { return (int)reported(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)most)); },
+                                     [](int, size_t, int*) { return 0; }, &fit);
+}
+
 constexpr uint32_t kNoRow = 0xffffffffu;
 
 // Ids as they come, COUNT of them at once: all loads are under way together, whatever the ids' width.

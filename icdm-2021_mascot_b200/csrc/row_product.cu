@@ -537,10 +537,10 @@ cudaError_t launch_product(const mascot_rows& a, const mascot_rows& b, const Pro
     if (!tile_map(&lane_map, MODE == SQUARE ? a : b, kLanes) || !tile_map(&col_map, MODE == SQUARE ? b : a, CN)) return cudaErrorInvalidValue;
     p.user_tiles = (uint32_t)((a.rows + users - 1) / users);
     p.tiles = p.user_tiles * (uint32_t)((b.rows + items - 1) / items);
-    const cudaError_t e = cudaFuncSetAttribute(product_kernel<CN, Out, MODE>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)S::smem);
+    static LaunchCache cache;
+    const cudaError_t e = allow_smem(product_kernel<CN, Out, MODE>, S::smem, cache);
     if (e != cudaSuccess) return e;
-    product_kernel<CN, Out, MODE><<<std::min<uint32_t>(p.tiles, sms), S::threads, S::smem, st>>>(lane_map, col_map, p);
-    return cudaGetLastError();
+    return launch(product_kernel<CN, Out, MODE>, std::min<uint32_t>(p.tiles, sms), S::threads, S::smem, st, lane_map, col_map, p);
 }
 
 // Users of a tile: as many as there are, up to 256, but fewer where that leaves SMs without a tile.
