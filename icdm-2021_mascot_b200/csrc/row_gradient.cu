@@ -541,6 +541,7 @@ __global__ void __launch_bounds__(kReduceBlock, PAIRS && N == 8 ? 2 : 3) reduce_
         after = entry_at(g + 3 * team + tl);
         pair = pair_of(after);
     }
+    if constexpr (ALIGNED) asm volatile("cp.async.wait_all;" ::: "memory");      // zeros behind the last entry: none is written after the block has ended
     flush();
 }
 

@@ -246,3 +246,19 @@ def test_odd_addresses_are_refused(mascot):
         for k, name in enumerate(names):
             for off in (1, 2, 3):
                 refused(M, call(at[:k] + [at[k] + off] + at[k + 1:]), name, "address")
+
+
+def test_kernels_end_with_no_copy_under_way():
+    """Whatever a kernel copies into shared memory asynchronously has arrived when it ends: the memory is another block's then."""
+    import os
+    import re
+    csrc = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "icdm-2021_mascot_b200", "csrc")
+    seen = []
+    for name in sorted(os.listdir(csrc)):
+        if name.endswith(".cu"):
+            for body in re.split(r"(?=\n(?:template <[^\n]*>\n)?__global__ )", open(os.path.join(csrc, name)).read())[1:]:
+                if re.search(r"cp_commit\(|fetch_piece<|fetch_word\(|cp\.async\.commit", body):
+                    kernel = re.search(r"(\w+)\(const", body).group(1)
+                    seen.append(kernel)
+                    assert re.search(r"cp\.async\.wait_all|cp_wait<0>", body), f"{name}: {kernel}"
+    assert {"reduce_kernel", "product_kernel"} <= set(seen), seen
