@@ -421,6 +421,8 @@ def rmse_host(P, Q, test, k, device=0):
 # ---- operators on factor rows in device memory: torch tensors in, torch tensors out, on torch's current stream ----
 # Outputs that the caller does not hand over, and scratch, come from torch's allocator, so that the calls can be captured
 # into a torch.cuda.graph.  `flags` is an int32 tensor of one element that gathers FLAG_BAD_ID and FLAG_GAVE_UP.
+# Autograd does not see these calls, and a gradient must not get lost in one: while gradients are recorded, a tensor that requires one is
+# refused (as torch does for its own calls with out=), and what a call writes into counts as changed.
 
 F32, F16, BF16, E4M3 = 0, 1, 2, 3
 FLAG_BAD_ID, FLAG_GAVE_UP = 1, 2
@@ -434,6 +436,8 @@ class _Ops:
         self.torch = torch
         self.types = {torch.float32: F32, torch.float16: F16, torch.bfloat16: BF16, torch.float8_e4m3fn: E4M3}
         self.bits = {torch.int32: 32, torch.int64: 64}
+        self.recording = torch.is_grad_enabled
+        self.changed = torch.autograd.graph.increment_version
         # the raw handle where torch offers it: the stream object around it costs 2 us a call
         raw = getattr(torch._C, "_cuda_getCurrentRawStream", None)
         self.stream = raw or (lambda index: torch.cuda.current_stream(index).cuda_stream)
@@ -450,8 +454,24 @@ def _refuse(message):
     raise MascotError(ERR_BAD_ARG, message)
 
 
+def _unrecorded(what, t):
+    """Refuses a tensor that requires a gradient while gradients are recorded."""
+    if _torch_ops().recording():
+        _refuse(f"{what}: requires a gradient, which this call does not record: make it under torch.no_grad(), or with {what}.detach(); "
+                "rows_gradient and pair_gradient compute the gradients of rows_lookup and pair_loss")
+
+
+def _changed(*tensors):
+    """Tells autograd that a call has written into these tensors of the caller's (None: not the caller's)."""
+    for t in tensors:
+        if t is not None and not t.is_inference():
+            _torch_ops().changed(t)
+
+
 def _rows(what, t, device):
     """The Rows of a 2-d tensor on `device` whose rows are contiguous."""
+    if t.requires_grad:
+        _unrecorded(what, t)
     kind = _torch_ops().types.get(t.dtype)
     if kind is None:
         _refuse(f"{what}: must be float32, float16, bfloat16 or float8_e4m3fn, not {t.dtype}")
@@ -483,6 +503,8 @@ def _plain(what, t, dtype, device, shape):
     """Address of a contiguous tensor of that type, device and shape; None stays None."""
     if t is None:
         return None
+    if t.requires_grad:
+        _unrecorded(what, t)
     if t.dtype != dtype or t.device != device or tuple(t.shape) != tuple(shape) or not t.is_contiguous():
         _refuse(f"{what}: must be a contiguous {dtype} tensor of shape {tuple(shape)} on {device}")
     return t.data_ptr()
@@ -539,8 +561,9 @@ def rows_lookup(table, ids, scale=1.0, table_scale=None, out=None, out_dtype=Non
         each, ts = _scale_rows("table_scale", table_scale, t.rows, t.width, device)
     if out_dtype is None and out is None:
         out_dtype = _torch_ops().torch.float32 if t.type == E4M3 else table.dtype
-    out = _result("out", out, (i.count, t.width), out_dtype, table)
+    given, out = out, _result("out", out, (i.count, t.width), out_dtype, table)
     _call(device, "mascot_rows_lookup", t, ts, each, i, scale, _rows("out", out, device), _flag_word(flags, device))
+    _changed(given, flags)
     return out
 
 
@@ -562,9 +585,10 @@ def rows_gradient(grad, ids, rows, scale=1.0, out=None, out_dtype=None, accumula
     g, i = _rows("grad", grad, device), _id_vector("ids", ids, device)
     if accumulate and out is None:
         _refuse("accumulate: needs an out")
-    out = _result("out", out, (rows, g.width), out_dtype if out_dtype is not None or out is not None else grad.dtype, grad)
+    given, out = out, _result("out", out, (rows, g.width), out_dtype if out_dtype is not None or out is not None else grad.dtype, grad)
     keep, ws, size = _workspace(workspace, "mascot_rows_gradient_workspace", grad, device, i.count, rows, g.width)
     _call(device, "mascot_rows_gradient", g, i, scale, _rows("out", out, device), 1 if accumulate else 0, ws, size, _flag_word(flags, device))
+    _changed(given, workspace, flags)
     return out
 
 
@@ -579,6 +603,7 @@ def pair_loss(P, Q, users, preferred, other, beta=1.0, smoothing=0.0, reference=
     loss, margin, coef = P.new_empty((3, n), dtype=torch.float32).unbind(0)
     _call(device, "mascot_pair_loss", p, q, u, i, j, beta, smoothing, ref, w, loss.data_ptr(), margin.data_ptr(), coef.data_ptr(),
           _flag_word(flags, device))
+    _changed(flags)
     return loss, margin, coef
 
 
@@ -590,12 +615,14 @@ def pair_gradient(P, Q, users, preferred, other, coef, scale=1.0, dP=None, dQ=No
     u, i, j = _id_vector("users", users, device), _id_vector("preferred", preferred, device), _id_vector("other", other, device)
     if accumulate and (dP is None or dQ is None):
         _refuse("accumulate: needs dP and dQ")
+    given = dP, dQ
     dP = _result("dP", dP, P.shape, out_dtype if out_dtype is not None or dP is not None else P.dtype, P)
     dQ = _result("dQ", dQ, Q.shape, out_dtype if out_dtype is not None or dQ is not None else Q.dtype, Q)
     c = _plain("coef", coef, _torch_ops().torch.float32, device, (u.count,))
     keep, ws, size = _workspace(workspace, "mascot_pair_gradient_workspace", P, device, u.count, p.rows, q.rows, p.width)
     _call(device, "mascot_pair_gradient", p, q, u, i, j, c, scale, _rows("dP", dP, device), _rows("dQ", dQ, device), 1 if accumulate else 0, ws,
           size, _flag_word(flags, device))
+    _changed(*given, workspace, flags)
     return dP, dQ
 
 
@@ -605,6 +632,7 @@ def rows_quantize(x, block_rows=1, q=None, scale=None):
     device = _device_of("x", x)
     torch = _torch_ops().torch
     r = _rows("x", x, device)
+    given = q, scale
     if q is None:
         q = torch.empty((r.rows, -(-r.width // 128) * 128), dtype=torch.float8_e4m3fn, device=device)[:, :r.width]
     else:
@@ -614,6 +642,7 @@ def rows_quantize(x, block_rows=1, q=None, scale=None):
         scale = torch.empty(shape, dtype=torch.float32, device=device)
     s = _plain("scale", scale, torch.float32, device, shape)
     _call(device, "mascot_rows_quantize", r, block_rows, _rows("q", q, device), s)
+    _changed(*given)
     return q, scale
 
 
@@ -625,6 +654,7 @@ def rows_product(a, a_scale, b, b_scale, out=None, out_dtype=None, flags=None):
     x, y = _rows("a", a, device), _rows("b", b, device)
     sa = _plain("a_scale", a_scale, torch.float32, device, (-(-x.width // 128), x.rows))
     each, sb = _scale_rows("b_scale", b_scale, y.rows, y.width, device)
-    out = _result("out", out, (x.rows, y.rows), out_dtype if out_dtype is not None or out is not None else torch.float32, a)
+    given, out = out, _result("out", out, (x.rows, y.rows), out_dtype if out_dtype is not None or out is not None else torch.float32, a)
     _call(device, "mascot_rows_product", x, sa, y, sb, each, _rows("out", out, device), _flag_word(flags, device))
+    _changed(given, flags)
     return out

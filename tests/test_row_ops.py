@@ -262,3 +262,22 @@ def test_kernels_end_with_no_copy_under_way():
                     seen.append(kernel)
                     assert re.search(r"cp\.async\.wait_all|cp_wait<0>", body), f"{name}: {kernel}"
     assert {"reduce_kernel", "product_kernel"} <= set(seen), seen
+
+
+def test_what_autograd_is_told(mascot):
+    """The two halves of it on the CPU, where the calls themselves stop at the device."""
+    import torch
+    leaf = torch.zeros(2, 3, requires_grad=True)
+    for refuse in (lambda: mascot._rows("P", leaf, leaf.device), lambda: mascot._plain("weight", leaf[0], torch.float32, leaf.device, (3,))):
+        with pytest.raises(mascot.MascotError) as e:
+            refuse()
+        assert e.value.status == mascot.ERR_BAD_ARG and "requires a gradient" in str(e.value)
+        with torch.no_grad():
+            refuse()
+    t = torch.zeros(4, 4)
+    was = t._version
+    mascot._changed(None, t[1:])
+    assert t._version == was + 1
+    with torch.inference_mode():
+        inside = torch.zeros(2)
+    mascot._changed(inside)
