@@ -1,11 +1,11 @@
-"""GPU tests of the scores, by kernel: scales at the ends of fp32.
+"""GPU tests of the scores, by kernel: scales at the ends of fp32, and how each stores.
 
 Which kernel a call takes follows from its sizes: up to 128 columns one that sums nothing up (ONE), for longer rows one with items in the
 lanes (ROWS), or one with users there for more than 128 users and square blocks (SQUARE), each with tiles of several widths."""
 import pytest
 import torch
 
-from test_gpu_row_ops import DEV, U, flag, gen, half, within
+from test_gpu_row_ops import DEV, TYPES, U, check_product, flag, gen, half, within
 
 pytestmark = pytest.mark.gpu
 
@@ -73,3 +73,34 @@ def test_scales_over_all_of_fp32(mascot, kernel):
     fits = mass < 2.0 ** 126                                # neither a term nor a partial sum leaves fp32
     assert fits.float().mean() > 0.3 and (want[fits].abs() > 2.0 ** -126).float().mean() > 0.3
     within(torch.where(fits, got.double(), 0.0), torch.where(fits, want, 0.0), tol)
+
+
+@pytest.mark.parametrize("dst", TYPES)
+@pytest.mark.parametrize("m,width,each", [(129, 129, 128), (300, 256, 128), (130, 256, 1), (70, 300, 1), (120, 256, 128)])
+@pytest.mark.parametrize("n", [264, 262, 263, 18_944, 18_942])
+def test_long_rows_into_strided_scores(mascot, dst, m, width, each, n):
+    """Rows of scores at 16-, 4- and 2-byte boundaries, and nothing written beside them."""
+    for extra, offset in ((0, 0), (8, 0), (0, 1), (2, 2), (1, 0)):
+        if n > 1000 and (extra, offset) not in ((0, 0), (2, 2), (1, 0)):
+            continue
+        store = torch.full((m * (n + extra) + offset + 9,), 5.0, device=DEV, dtype=dst)
+        out = store[offset:offset + m * (n + extra)].view(m, n + extra)[:, :n]
+        check_product(mascot, m, n, width, each, dst, out=out)
+        rest = torch.ones_like(store, dtype=torch.bool)
+        rest[offset:offset + m * (n + extra)].view(m, n + extra)[:, :n] = False
+        assert (store[rest] == 5).all()
+
+
+@pytest.mark.parametrize("kernel", KERNELS)
+def test_a_row_of_zeros_meets_a_nan(mascot, kernel):
+    """Scores of a row of zeros are zeros but for the item that holds a NaN."""
+    m, n, width, each = KERNELS[kernel]
+    a, b = of_value(m, width, 1), of_value(n, width, 1)
+    a.view(torch.uint8)[2] = 0
+    b.view(torch.uint8)[77, 3] = 0xff
+    blocks = -(-width // 128)
+    got = mascot.rows_product(a, powers((blocks, m), 0), b, powers((blocks, -(-n // each)), 3))
+    want = torch.full((m, n), 8.0 * width, device=DEV)
+    want[2] = 0
+    want[:, 77] = float("nan")
+    assert torch.equal(got.nan_to_num(-1), want.nan_to_num(-1))
