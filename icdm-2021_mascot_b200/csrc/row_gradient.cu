@@ -36,9 +36,8 @@ constexpr int kReduceBlock = 256, kCombineBlock = 512;
 // What is summed: where entries come from and what their values are.
 struct Job {
     Ids ids[3];                                 // lookup: one; pairs: users, preferred, other
-    uint32_t per;                               // ids of one kind; entry e of pairs is id e / 3 of kind e % 3, so that a tile of entries is one of pairs
-    uint32_t kinds;                             // 1: lookup, 3: pairs
-    uint32_t n;                                 // entries: kinds * per
+    uint32_t kinds;                             // 1: lookup, 3: pairs; entry e of pairs is id e / 3 of kind e % 3, so that a tile of entries is one of pairs
+    uint32_t n;                                 // entries: kinds * ids of one kind
     uint32_t rows[2];                           // of the table; of both tables
     uint32_t total;                             // all rows; the sort key of an entry that names none
     const void* src[2];                         // lookup: gradient rows; pairs: P, Q
@@ -262,22 +261,19 @@ __global__ void __launch_bounds__(kSortBlock) count_kernel(const Job j, const Sp
     for (int b = threadIdx.x; b < bins; b += kSortBlock) s.counts[(size_t)blockIdx.x * bins + b] = hist[b];
 }
 
-// A block for 32 bins, a warp for a run of tiles: counts of the tiles become offsets within the bin, the sums go to totals.
+// A block for 32 bins of 256 or 1024, a warp for a run of tiles: counts of the tiles become offsets within the bin, the sums go to totals.
 __global__ void __launch_bounds__(1024) scan_kernel(const Space s, int bins) {
     __shared__ uint32_t sums[32][32];
     follow();
     const uint32_t lane = threadIdx.x & 31, warp = threadIdx.x >> 5, bin = blockIdx.x * 32 + lane;
     const uint32_t per = (s.tiles + 31) / 32, t0 = min(s.tiles, warp * per), t1 = min(s.tiles, t0 + per);
     uint32_t sum = 0;
-    if (bin < bins) {
 #pragma unroll 8
-        for (uint32_t t = t0; t < t1; t++) sum += s.counts[(size_t)t * bins + bin];
-    }
+    for (uint32_t t = t0; t < t1; t++) sum += s.counts[(size_t)t * bins + bin];
     sums[warp][lane] = sum;
     __syncthreads();
     uint32_t run = 0;
-    for (uint32_t w = 0; w < 32; w++) { const uint32_t x = sums[w][lane]; if (w < warp) run += x; else if (w == 31) break; }
-    if (bin >= bins) return;
+    for (uint32_t w = 0; w < warp; w++) run += sums[w][lane];
 #pragma unroll 8
     for (uint32_t t = t0; t < t1; t++) {
         const uint32_t x = s.counts[(size_t)t * bins + bin];
@@ -385,7 +381,7 @@ template <bool PAIRS> __device__ __forceinline__ Term term_of(const Job& j, uint
     return t;
 }
 
-// 8 or 16 bytes on their way to shared memory, past L1 (with it, pairs on a popular law take 6 % longer).
+// 8 or 16 bytes on their way to shared memory.  16 go past L1 (with it, pairs on a popular law take 6 % longer); for 8 there is only the form through it.
 // Zeros instead where it is not there: nothing is read then.
 template <int BYTES> __device__ __forceinline__ void fetch_piece(uint32_t to, const void* from, bool there) {
     if constexpr (BYTES == 16) asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to), "l"(from), "r"(there ? 16 : 0) : "memory");
@@ -845,7 +841,7 @@ int mascot_rows_gradient(const mascot_rows* grad, const mascot_ids* ids, float s
     ROW_CHECK(check_memory("flags", flags, device));
     Job j = {};
     j.ids[0] = ids_of(*ids);
-    j.per = j.n = (uint32_t)ids->count;
+    j.n = (uint32_t)ids->count;
     j.kinds = 1;
     j.rows[0] = j.total = (uint32_t)out->rows;
     j.src[0] = grad->data; j.src_stride[0] = grad->stride;
@@ -910,7 +906,7 @@ int mascot_pair_gradient(const mascot_rows* P, const mascot_rows* Q, const masco
     ROW_CHECK(check_memory("flags", flags, device));
     Job j = {};
     j.ids[0] = ids_of(*users); j.ids[1] = ids_of(*preferred); j.ids[2] = ids_of(*other);
-    j.per = (uint32_t)n; j.kinds = 3; j.n = (uint32_t)(3 * n);
+    j.kinds = 3; j.n = (uint32_t)(3 * n);
     j.rows[0] = (uint32_t)P->rows; j.rows[1] = (uint32_t)Q->rows; j.total = (uint32_t)total;
     j.src[0] = P->data; j.src[1] = Q->data;
     j.src_stride[0] = P->stride; j.src_stride[1] = Q->stride;

@@ -8,7 +8,7 @@
 // operands by TMA, one issues the matrix instructions, one fetches scales, the others read back, scale and store: warp w the
 // lanes 32 (w % 4) on, and columns of the group w / 4.  Rows of a (users) are the inner index of the tiles, so that rows
 // of b (items) are fetched from HBM once and from L2 after that.  What differs is which side the lanes are (Mode):
-//   ONE     rows of 128 columns and less: items.  What is written bounds it.  Four warps read 8 columns of all lanes at a time, meet
+//   ONE     rows of 128 columns and less: items.  What is written bounds it.  Four warps read 16 columns of all lanes at a time, meet
 //           over shared memory and store whole rows of 128 scores, in pieces as wide as the row's address allows (32 scores a
 //           warp, straight from the accumulator, took 1.4 times as long; that is how up to 16 users are stored).  Nothing is summed up, so registers allow 16 such warps.
 //   ROWS    longer rows, a scale for each row of b, or few users: items too.  A column's scale is a broadcast from shared memory,

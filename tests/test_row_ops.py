@@ -281,3 +281,21 @@ def test_what_autograd_is_told(mascot):
     with torch.inference_mode():
         inside = torch.zeros(2)
     mascot._changed(inside)
+
+
+def test_workspace_on_both_sides_of_the_one_launch_sort(mascot):
+    """Up to 32,768 entries one cluster sorts, and needs neither keys nor counts; one entry more needs both: 4 bytes an entry, and 1024 counts
+    for each of 17 tiles of 2,048 entries and their sums."""
+    lib, n = mascot.load(), C.c_uint64()
+
+    def rows(count):
+        assert lib.mascot_rows_gradient_workspace(count, 1000, 64, C.byref(n)) == mascot.OK
+        return n.value
+
+    def pairs(count):
+        assert lib.mascot_pair_gradient_workspace(count, 600, 400, 64, C.byref(n)) == mascot.OK
+        return n.value
+    more = 4 * 32_769 + 4 * 1024 * 17 + 4 * 1024
+    assert more <= rows(32_769) - rows(32_768) < more + 5000
+    assert more <= pairs(10_923) - pairs(10_922) < more + 10_000            # 32,769 and 32,766 entries
+    assert rows(32_768) - rows(32_767) < 5000 and rows(32_770) - rows(32_769) < 5000
