@@ -391,10 +391,10 @@ template <int BYTES> __device__ __forceinline__ void fetch_piece(uint32_t to, co
 // A team's lanes take a group of entries each and hand their rows round; what a lane can work out for a group (where rows begin, which
 // entries add nothing) it does, and the team reads it off ballots.  What bounds it is the rows, random ones from HBM or
 // L2, so AHEAD of them are under way for each team: every lane copies its pieces into shared memory of its own, which needs
-// no registers and no meeting of threads.  4M rows of 256 bytes into 480k of 512: 211 us for 1.29 GB, 6.1 TB/s (286 with four rows in
-// flight in registers).  The gradients of 1M pairs, binary16 rows of 128: 237 us, bound by instructions and by the latency of L2.
+// no registers and no meeting of threads.  4M rows of 256 bytes into 480k of 512: 213 us for 1.29 GB, 6.1 TB/s (286 with four rows in
+// flight in registers).  The gradients of 1M pairs, binary16 rows of 128: 235 us, bound by instructions and by the latency of L2.
 // Rows that cannot be moved in pieces are loaded where they are added, element by element, four for each lane a team's width apart
-// (20,000 rows of 333 binary16 numbers: 41 us in all; 91 with one for each lane).
+// (20,000 rows of 333 binary16 numbers into as many: 43 us on the GPU in all; 91 with one for each lane).
 template <typename T, int N, bool PAIRS, bool ALIGNED> struct Ring {
     static constexpr int piece = sizeof(T) * N, ahead = PAIRS ? 8 : 16, sides = PAIRS ? 2 : 1;      // rows of an entry
     static constexpr size_t smem = ALIGNED ? (size_t)ahead * sides * kReduceBlock * piece : 0;
@@ -554,7 +554,7 @@ __device__ __forceinline__ uint32_t row_end(const uint2* entry, uint32_t at, uin
 }
 
 // Blocks below `combine_blocks` add up the parts of the rows that the owners name: a warp each, and all warps of the block a slice
-// each where a row has more parts than the block has warps (200,000 entries on 30 rows of 336: 77 us in all, 234 when neighbouring owners
+// each where a row has more parts than the block has warps (200,000 binary16 rows of 336 into 30: 68 us on the GPU in all, some 230 when neighbouring owners
 // shared a block).  The other blocks clear the rows that no entry names, a warp for 32 of them.
 template <int N> __device__ __forceinline__ void add_parts(const Space& s, uint32_t first, uint32_t end, uint32_t col, float (&sum)[N]) {
 #pragma unroll 16
@@ -652,8 +652,8 @@ __global__ void __launch_bounds__(kCombineBlock, 2) combine_kernel(const Job j, 
 
 // ---- host ---------------------------------------------------------------------------------------------------
 
-// Entries of a chunk: enough chunks to fill the GPU, and no more parts than that needs (4M entries: 128, 367 us in all; 256, 377 us;
-// 64, 385 us.  12,288 entries: 8, 31 us; 16, 34 us; 32, 40 us).
+// Entries of a chunk: enough chunks to fill the GPU, and no more parts than that needs (4M entries: 128, 364 us in all; 256, 377 us;
+// 64, 385 us.  12,288 entries, of 4,096 pairs: 8, 31 us with the loss; 16, 34 us; 32, 40 us).
 int chunk_log2(uint64_t n) { return n < (1u << 14) ? 3 : n < (1u << 17) ? 4 : n < (1u << 19) ? 5 : n < (1u << 21) ? 6 : 7; }
 int bits_for(uint64_t keys) { int b = 1; while (b < 32 && (1ull << b) < keys) b++; return b; }      // of the largest key, keys - 1
 

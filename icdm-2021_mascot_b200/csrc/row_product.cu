@@ -5,18 +5,18 @@
 // back from tensor memory, scaled and added in fp32 registers while the tensor cores work on the next one in another part of it.
 //
 // A block of threads is persistent and takes every gridDim.x-th tile of 128 lanes x CN columns of an accumulator.  One warp fetches
-// operands by TMA, one issues the matrix instructions, one fetches scales, the others read back, scale and store: warp w the
+// operands by TMA, one issues the matrix instructions, one fetches scales, one looks whether they are in a safe range, the others read back, scale and store: warp w the
 // lanes 32 (w % 4) on, and columns of the group w / 4.  Rows of a (users) are the inner index of the tiles, so that rows
 // of b (items) are fetched from HBM once and from L2 after that.  What differs is which side the lanes are (Mode):
 //   ONE     rows of 128 columns and less: items.  What is written bounds it.  Four warps read 16 columns of all lanes at a time, meet
 //           over shared memory and store whole rows of 128 scores, in pieces as wide as the row's address allows (32 scores a
 //           warp, straight from the accumulator, took 1.4 times as long; that is how up to 16 users are stored).  Nothing is summed up, so registers allow 16 such warps.
 //   ROWS    longer rows, a scale for each row of b, or few users: items too.  A column's scale is a broadcast from shared memory,
-//           whose 128 bytes to a warp bound the step at 4 CN cycles, twice what the matrix instructions take (4,096 x 17,770 x 4,096:
-//           414 us).
+//           whose 128 bytes to a warp bound the step at 4 CN cycles, twice what the matrix instructions take (4,096 x 17,770 x 4,096
+//           to bf16: 460 us a call, 409 in a burst too short for the power limit).
 //   SQUARE  longer rows, a scale for 128 rows of b: users.  The scale of a lane and half of the columns is one number, kept in a
-//           register; scores go through shared memory to be stored along the rows of `out` (the same sizes: 297 us, 2.0 PFLOP/s; the
-//           tensor cores are busy half of the time, the rest they wait for accumulators to be read back).
+//           register; scores go through shared memory to be stored along the rows of `out` (the same sizes: 353 us a call,
+//           1.69 PFLOP/s, and 301 us in a short burst; the tensor cores are busy half of the time, the rest they wait for accumulators to be read back).
 #include <cuda.h>
 
 #include <algorithm>
@@ -349,7 +349,7 @@ __global__ void __launch_bounds__(Shape<CN, MODE>::threads, 1) product_kernel(co
             }
             asm volatile("cp.async.wait_all;" ::: "memory");
         }
-        if (warp == S::readers + 3) {                           // looks for far scales ahead of the readers, whom a look and a branch of their own cost a fifth
+        if (warp == S::readers + 3) {                           // looks for far scales ahead of the readers, whom a look and a branch of their own cost a quarter
             bool far = false;                                   // of any step
             for (uint32_t t = blockIdx.x; ok && t < p.tiles; t += gridDim.x)
                 for (uint32_t c = 0; c < p.blocks; c++, step++) {

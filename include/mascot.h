@@ -420,7 +420,7 @@ MASCOT_API int mascot_rmse_device_noalloc(const float* d_P, const float* d_Q, ui
  * For programs that keep factor tables of their own on the GPU: rows by id and their gradient, training from
  * preferences instead of ratings, tables held in 8 bits and the scores of all items from them.  No counterpart in the
  * reference.  Conventions of this section:
- *   - buffers are device (or managed) memory of the current device, checked by address; the call queues its kernels on
+ *   - buffers are device (or managed) memory of the current device, checked by address, at multiples of their element's size; the call queues its kernels on
  *     `stream` (a cudaStream_t of that device, NULL = the default stream) and returns without waiting.  It allocates
  *     nothing and keeps nothing, so it may be captured into a graph (make one call of the same kind and types before:
  *     the first one loads the kernels);
@@ -438,7 +438,7 @@ enum { MASCOT_FLAG_BAD_ID = 1, MASCOT_FLAG_GAVE_UP = 2 };                      /
 
 typedef struct mascot_rows {
     void* data;
-    uint64_t rows;           /* below 2^31 */
+    uint64_t rows;           /* below 2^31 - 1 */
     uint64_t stride;         /* elements from one row to the next */
     uint32_t width;          /* elements of a row, 1 .. 65536 */
     uint32_t type;           /* MASCOT_F32 ... */
@@ -446,7 +446,7 @@ typedef struct mascot_rows {
 
 typedef struct mascot_ids {
     const void* data;        /* signed integers of `bits` bits, one after the other */
-    uint64_t count;          /* below 2^31 */
+    uint64_t count;          /* below 2^31 - 1 */
     uint32_t bits;           /* 32 or 64 */
     uint32_t reserved;       /* 0 */
 } mascot_ids;
